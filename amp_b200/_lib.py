@@ -50,6 +50,14 @@ SIGNATURES: dict[str, tuple] = {
     "amp_flash_attn_bwd_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "amp_flash_attn_bwd_bf16_dev": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32,
                                            _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
+    "amp_flash_attn_varlen_workspace_bytes": (_sz, [_i32]),
+    "amp_flash_attn_varlen_fwd_bf16_dev": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32,
+                                                  _i32, _i32, _i32, _i32, _vp, _i32, _f32, _vp,
+                                                  _sz, _vp]),
+    "amp_flash_attn_varlen_bwd_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "amp_flash_attn_varlen_bwd_bf16_dev": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                  _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
+                                                  _vp, _i32, _f32, _vp, _sz, _vp]),
     "amp_user_flash_attn_fwd_bf16": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
                                             _i32, _i32, _i32, _f32]),
     "amp_paged_decode_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
@@ -122,6 +130,17 @@ def lib() -> C.CDLL:
                     f.restype, f.argtypes = res, args
                 _lib = h
     return _lib
+
+
+def call_on(device, name: str, *args) -> int:
+    """call() with `device` (a torch CUDA device) current and its current stream as the
+    last argument: the library works on the current device, and tensors may live on another."""
+    import torch
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        return call(name, *args, stream)
+    with torch.cuda.device(device):
+        return call(name, *args, stream)
 
 
 def call(name: str, *args) -> int:

@@ -38,6 +38,17 @@
 //              than 2^8; otherwise the stale maximum is kept.
 //              Epilogue: O / l to bf16, lse = (m + log2 l) * ln 2.
 //
+// Packed mode (sequences of different lengths one after another, [total, heads, D] with
+// any token and head strides; bottom-right aligned causal mask, as paged prefill):
+// persistent CTAs draw items from the plan's list (varlen.cuh).  An item is two (query
+// tile, query head) pairs that are neighbours in the order (tile major, then the heads
+// of one kv head), so with an even GQA group its two query tiles are the same 128 rows
+// of two heads: they need the same K/V tiles, and a sequence of less than 129 tokens
+// fills both.  Warp 3 draws and decodes items ahead into a two-slot ring.  The maps know
+// only the end of the whole tensor, so a sequence's last K/V tile brings rows of the next
+// sequence: their scores are masked, and warp 2 zeroes those rows of V in shared memory
+// before the PV product may read them (0 * NaN of a neighbour would be NaN).
+//
 // All-gather mode ((batch*head)-sharded attention on the GPUs of one node: the
 // reference's launch + ncclAllGather of O / lse, include/collective.hpp:87-89):
 // each softmax warp stages its 32 output rows in the tile's Q buffer (free once
@@ -47,17 +58,21 @@
 // sequence number with every rank through the peer mailboxes (bounded wait).
 #include <cuda.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "common.cuh"
 #include "peer.cuh"
 #include "runtime.h"
 #include "tc_common.cuh"
+#include "varlen.cuh"
 
 namespace ampb {
 
 int fa_make_tmap_3d(CUtensorMap* m, const void* base, int64_t d, int64_t s, int64_t bh);
 int fa_make_tmap_pool(CUtensorMap* m, const void* base, int64_t d, int64_t hkv, int64_t pages);
+int fa_make_tmap_packed(CUtensorMap* m, const void* base, int64_t d, int64_t tokens, int64_t heads,
+                        int64_t tok_stride, int64_t head_stride);
 
 namespace {
 
@@ -92,6 +107,17 @@ struct FaParams {
     unsigned long long* const* mbox;
     unsigned seq;
     unsigned* done;
+    // packed mode: strides in elements of O, rows of the whole O, the work list
+    int64_t o_tok, o_head;
+    int total_q;
+    VarlenPlan plan;
+};
+
+// One item of the packed mode, as warp 3 publishes it (n1 == 0: no more items).
+struct PackedItem {
+    int q_tok, q_len, k_tok, k_len;   // the sequence's rows in Q and in K / V
+    int row0[2], head[2];             // first query row and query head of each tile
+    int kv_head, n0, n1;
 };
 
 // Softmax warps of the all-gather attention that have stored their rows; one
@@ -116,7 +142,8 @@ template <int D>
 struct FaCfg {
     static constexpr int SLABS = D / 64;
     static constexpr int TILE = SLABS * SLAB_BYTES;
-    static constexpr int SMEM = 2 * TILE + KV_STAGES * 2 * TILE + 1024 + 256;
+    // barriers and the TMEM slot take 224 bytes, the packed items two slots of 44
+    static constexpr int SMEM = 2 * TILE + KV_STAGES * 2 * TILE + 1024 + 384;
     static constexpr uint32_t IDESC_QK = make_idesc(1, 1, 0, 0, BQ, BKV);
     static constexpr uint32_t IDESC_PV = make_idesc(1, 1, 0, 1, BQ, D);
     static constexpr uint32_t O_COL = 2 * BKV;            // S0 | S1 | O0 | O1
@@ -125,11 +152,13 @@ struct FaCfg {
 // kPersist: one CTA per SM walks a list of (batch*head, query-tile pair) items
 // (see item_at below) instead of one CTA per item, so that the next item's Q and
 // K/V loads and its first QK overlap the current item's last steps and epilogue.
-template <int D, bool kPaged, bool kAllGather = false, bool kPersist = false>
+// kPacked (with kPersist): the items come from the plan's list of packed sequences.
+template <int D, bool kPaged, bool kAllGather = false, bool kPersist = false, bool kPacked = false>
 __global__ void __launch_bounds__(kThreads, 1)
     k_flash_fwd(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
            const __grid_constant__ CUtensorMap tmV, const FaParams p) {
     static_assert(!(kPersist && kAllGather), "the all-gather epilogue stages in Q: one item per CTA");
+    static_assert(!kPacked || (kPersist && !kPaged), "packed items are drawn by persistent CTAs");
     using CF = FaCfg<D>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -149,7 +178,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* pv_done = p_full + 2;     // [2]
     uint64_t* o_free = pv_done + 2;     // [2] the epilogue has read O_t out of TMEM
     uint64_t* drain = o_free + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    // packed mode: item slots' barriers, and the V tiles that hold a sequence's end
+    uint64_t* it_full = drain + 1;      // [2]
+    uint64_t* it_empty = it_full + 2;   // [2] load, MMA and zeroing warps, 8 softmax warps
+    uint64_t* v_raw = it_empty + 2;     // [KV_STAGES] loaded, rows past the end not yet zeroed
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_raw + KV_STAGES);
+    PackedItem* items = reinterpret_cast<PackedItem*>(tmem_slot + 2);   // [2]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n_qb = (p.S_q + 2 * BQ - 1) / (2 * BQ);
@@ -176,14 +210,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     };
     struct Geo {
-        int b, h, bh_kv, q0, S_kv, coff, n0, n1;
+        int b, h, bh, bh_kv, S_q, S_kv, coff, n0, n1;
+        int q0[2];              // first query row of each tile
+        int q_tok, k_tok;       // packed: the sequence's first row in Q and in K / V
+        int head[2];            // packed: query head of each tile
     };
     auto geo = [&](int bh, int qb) {
         Geo g;
         g.b = bh / p.Hq;
+        g.bh = bh;
+        g.q_tok = g.k_tok = 0;
+        g.head[0] = g.head[1] = bh;
         g.h = bh % p.Hq;
         g.bh_kv = g.b * p.Hkv + g.h / (p.Hq / p.Hkv);
-        g.q0 = qb * 2 * BQ;
+        g.q0[0] = qb * 2 * BQ;
+        g.q0[1] = g.q0[0] + BQ;
+        g.S_q = p.S_q;
         g.S_kv = p.S_kv;
         g.coff = p.causal_offset;
         if constexpr (kPaged) {
@@ -199,9 +241,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             return max(n, 1);
         };
-        g.n0 = nblk(g.q0);
-        g.n1 = max(nblk(g.q0 + BQ), g.n0);
+        g.n0 = nblk(g.q0[0]);
+        g.n1 = max(nblk(g.q0[1]), g.n0);
         return g;
+    };
+    // k-th item of this CTA into g: 0 = no more (or a wait ran out), 1 = an item, 2 = an
+    // empty slot.  Packed: read from the ring; the reader releases its slot with it_done.
+    auto next_item = [&](int k, Geo& g) -> int {
+        if constexpr (kPacked) {
+            if (!mbar_wait(&it_full[k & 1], (k >> 1) & 1, p.status)) return 0;
+            const volatile PackedItem& it = items[k & 1];
+            g.n1 = it.n1;
+            if (g.n1 == 0) return 0;
+            g.n0 = it.n0;
+            g.b = 0;
+            g.h = g.bh = 0;
+            g.bh_kv = it.kv_head;
+            g.S_q = it.q_len;
+            g.S_kv = it.k_len;
+            g.coff = it.k_len - it.q_len;
+            g.q_tok = it.q_tok;
+            g.k_tok = it.k_tok;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                g.q0[t] = it.row0[t];
+                g.head[t] = it.head[t];
+            }
+            return 1;
+        } else {
+            int bh, qb;
+            const int st = item_at(k, bh, qb);
+            if (st == 1) g = geo(bh, qb);
+            return st;
+        }
+    };
+    auto it_done = [&](int k) {
+        if constexpr (kPacked) mbar_arrive(&it_empty[k & 1]);
     };
 
     if (threadIdx.x == 0) {
@@ -222,6 +297,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&pv_done[i], 1);
         }
         mbar_init(drain, 1);
+        if constexpr (kPacked) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&it_full[i], 1);
+                mbar_init(&it_empty[i], 11);
+            }
+            for (int s = 0; s < KV_STAGES; ++s) mbar_init(&v_raw[s], 1);
+        }
         fence_barrier_init();
         fence_proxy_async_smem();
     }
@@ -233,6 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    if constexpr (kPacked) pdl_wait();   // the plan
 
     if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegCtl));
@@ -246,11 +329,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             int gkv = 0, li = 0;
             bool ok = true;
             for (int k = 0; ok; ++k) {
-                int bh, qb;
-                const int st = item_at(k, bh, qb);
+                Geo g;
+                const int st = next_item(k, g);
                 if (st == 0) break;
                 if (st == 2) continue;
-                const Geo g = geo(bh, qb);
+                it_done(k);
                 // Q_t of this item once the previous item's last QK_t has read Q_t.
                 // Persistent order: Q_0, K/V 0, Q_1, K/V 1.. -- Q_1 is freed last
                 // (tile 1 runs the previous item's last step), and the next item's
@@ -261,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int sl = 0; sl < CF::SLABS; ++sl)
                         tma_load_3d(q_s + t * CF::TILE + sl * SLAB_BYTES, &tmQ, &q_full[t],
-                                    sl * 64, g.q0 + t * BQ, bh);
+                                    sl * 64, g.q_tok + g.q0[t], g.head[t]);
                     return true;
                 };
                 if (!load_q(0)) break;
@@ -293,21 +376,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 tma_load_4d(dst + i * kPageTokens * 128, &tmK, &k_full[s], sl * 64,
                                             0, hk, pages[i]);
                         } else {
-                            tma_load_3d(dst, &tmK, &k_full[s], sl * 64, j * BKV, g.bh_kv);
+                            tma_load_3d(dst, &tmK, &k_full[s], sl * 64, g.k_tok + j * BKV, g.bh_kv);
                         }
                     }
                     if (!mbar_wait(&v_empty[s], ph ^ 1, p.status)) { ok = false; break; }
-                    mbar_arrive_expect_tx(&v_full[s], CF::TILE);
+                    // packed: a tile past the sequence's end goes to warp 2 first
+                    uint64_t* v_bar = kPacked && (j + 1) * BKV > g.S_kv ? &v_raw[s] : &v_full[s];
+                    mbar_arrive_expect_tx(v_bar, CF::TILE);
 #pragma unroll
                     for (int sl = 0; sl < CF::SLABS; ++sl) {
                         uint8_t* dst = v_s + s * CF::TILE + sl * SLAB_BYTES;
                         if constexpr (kPaged) {
 #pragma unroll
                             for (int i = 0; i < BKV / kPageTokens; ++i)
-                                tma_load_4d(dst + i * kPageTokens * 128, &tmV, &v_full[s], sl * 64,
+                                tma_load_4d(dst + i * kPageTokens * 128, &tmV, v_bar, sl * 64,
                                             0, hk, pages[i]);
                         } else {
-                            tma_load_3d(dst, &tmV, &v_full[s], sl * 64, j * BKV, g.bh_kv);
+                            tma_load_3d(dst, &tmV, v_bar, sl * 64, g.k_tok + j * BKV, g.bh_kv);
                         }
                     }
                     if (kPersist && j == 0 && !load_q(1)) { ok = false; break; }
@@ -336,11 +421,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             int gkv = 0, li = 0, c[2] = {0, 0};
             bool ok = true, pre0 = false;   // pre0: this item's QK_0 was issued early
             for (int k = 0; ok; ++k) {
-                int bh, qb;
-                const int st = item_at(k, bh, qb);
+                Geo g;
+                const int st = next_item(k, g);
                 if (st == 0) break;
                 if (st == 2) continue;
-                const Geo g = geo(bh, qb);
+                it_done(k);
                 const int n0 = g.n0, n1 = g.n1;
                 // S_t = Q_t K_0^T of this item.  S_t may still hold P_t of the previous
                 // item's last step: its PV was issued earlier, and runs first.
@@ -372,14 +457,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int t = 0; t < 2; ++t) {
                         const int nt = t ? n1 : n0;
                         if (j >= nt) continue;
-                        if (t == 1 && j == n1 - 1 && j >= n0) {
+                        // (packed: also when both tiles end with this step, PV_0 of which
+                        // was just issued -- two heads of the same rows always do)
+                        if (t == 1 && j == n1 - 1 && j >= (kPacked ? n0 - 1 : n0)) {
                             // Tile 0 is done with this item: S_0 of the next item now,
                             // while tile 1 runs its last step (S_0 held P_0 of this
                             // item's last tile-0 step, whose PV was issued before).
-                            int kn = k + 1, bh2, qb2, st2;
-                            while ((st2 = item_at(kn, bh2, qb2)) == 2) ++kn;
+                            Geo gn2;
+                            int kn = k + 1, st2;
+                            while ((st2 = next_item(kn, gn2)) == 2) ++kn;
                             if (st2 == 1) {
-                                const int n0n = geo(bh2, qb2).n0;
+                                const int n0n = gn2.n0;
                                 const int gn = gkv + n1, sn = gn % KV_STAGES;
                                 if (!mbar_wait(&k_full[sn], (gn / KV_STAGES) & 1, p.status) ||
                                     !mbar_wait(&q_full[0], (li + 1) & 1, p.status)) {
@@ -435,6 +523,84 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_commit(drain);
             mbar_wait(drain, 0, p.status);
         }
+    } else if (kPacked && warp == 2) {
+        // rows of V past the sequence's end: zeroed in shared memory
+        int gkv = 0, fixed[KV_STAGES] = {};   // tiles before this item; v_raw phases used
+        for (int k = 0;; ++k) {
+            Geo g;
+            const int st = __all_sync(0xffffffffu, next_item(k, g) == 1);
+            if (!st) break;
+            __syncwarp();
+            if (lane == 0) it_done(k);
+            const int valid = g.S_kv - (g.n1 - 1) * BKV;   // of the last tile
+            if (valid < BKV) {
+                const int s = (gkv + g.n1 - 1) % KV_STAGES;
+                bool ok = false;
+#pragma unroll
+                for (int i = 0; i < KV_STAGES; ++i)
+                    if (i == s) ok = mbar_wait_warp(&v_raw[i], fixed[i]++ & 1, p.status);
+                if (!ok) break;
+                for (int i = max(valid, 0) * 8 + lane; i < BKV * 8; i += 32)
+#pragma unroll
+                    for (int sl = 0; sl < CF::SLABS; ++sl)
+                        *reinterpret_cast<uint4*>(v_s + s * CF::TILE + sl * SLAB_BYTES + i * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[s]);
+            }
+            gkv += g.n1;
+        }
+    } else if (kPacked && warp == 3) {
+        // draws items ahead of the other warps: the first of each CTA by its index, the
+        // rest from the counter
+        const int group = p.Hq / p.Hkv;
+        const int total = p.plan.first[0][p.plan.B];
+        for (int k = 0;; ++k) {
+            if (k >= 2 && !mbar_wait_warp(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) break;
+            int item = (int)blockIdx.x;
+            if (k > 0) {
+                if (lane == 0) item = (int)gridDim.x + atomicAdd(&p.plan.next[0], 1);
+                item = __shfl_sync(0xffffffffu, item, 0);
+            }
+            PackedItem it = {};
+            if (item < total) {
+                const int r = varlen_find(p.plan.first[0], p.plan.B, item);
+                const VarlenSeq sq = p.plan.seqs[r];
+                const int pairs = varlen_fwd_pairs(sq.q_len, group);
+                const int w = item - p.plan.first[0][r];
+                const int tiles = varlen_tiles(sq.q_len);
+                const int pair = pairs - 1 - w % pairs;   // most keys first
+                it.kv_head = w / pairs;
+                it.q_tok = sq.q_off;
+                it.q_len = sq.q_len;
+                it.k_tok = sq.k_off;
+                it.k_len = sq.k_len;
+                const int n_all = (sq.k_len + BKV - 1) / BKV;
+                int n[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int sub = 2 * pair + t;
+                    const bool none = sub >= tiles * group;   // the last pair's second half
+                    it.row0[t] = none ? tiles * BQ : sub / group * BQ;
+                    it.head[t] = none ? it.head[0] : it.kv_head * group + sub % group;
+                    n[t] = n_all;
+                    if (none) n[t] = 0;
+                    else if (p.causal) {
+                        const int last = it.row0[t] + BQ - 1 + sq.k_len - sq.q_len;
+                        n[t] = min(n_all, last < 0 ? 0 : last / BKV + 1);
+                    }
+                }
+                it.n0 = max(n[0], 1);
+                it.n1 = max(n[1], it.n0);
+            }
+            if (lane == 0) {
+                items[k & 1] = it;
+                mbar_arrive(&it_full[k & 1]);
+            }
+            __syncwarp();
+            if (item >= total) break;
+        }
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegSoftmax));
@@ -449,15 +615,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         int c_t = 0;
         bool ok = true;
         for (int it = 0; ok; ++it) {
-        int bh, qb;
-        const int st_item = item_at(it, bh, qb);
+        Geo g;
+        int st_item = next_item(it, g);
+        if constexpr (kPacked) st_item = __all_sync(0xffffffffu, st_item == 1);
         if (st_item == 0) break;
         if (st_item == 2) continue;
-        const Geo g = geo(bh, qb);
-        const int q0 = g.q0, S_kv = g.S_kv, coff = g.coff;
-        const int qi = q0 + t * BQ + r;
+        const int bh = g.bh, S_kv = g.S_kv, coff = g.coff;
+        const int q0 = t ? g.q0[1] : g.q0[0];
+        const int qi = q0 + r;
         const int nt = t ? g.n1 : g.n0;
-        const int vis_hi = p.causal ? min(S_kv - 1, qi + coff) : S_kv - 1;
+        int vis_hi = p.causal ? min(S_kv - 1, qi + coff) : S_kv - 1;
+        if (kPacked && qi >= g.S_q) vis_hi = -1;   // rows of the next sequence
         float m_run = -INFINITY, l_run = 0.0f;
         for (int j = 0; j < nt; ++j) {
             if (!mbar_wait_warp(&s_full[t], (c_t + j) & 1, p.status)) { ok = false; break; }
@@ -546,12 +714,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) {
             tc_fence_after();
             const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-            const bool row_ok = qi < p.S_q;
+            const bool row_ok = qi < g.S_q;
             const float lse_v =
                 l_run > 0.0f ? (m_run + lg2_approx(l_run)) * 0.69314718055994531f : -INFINITY;
             if constexpr (!kAllGather) {
-                __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.O) +
-                                      ((int64_t)bh * p.S_q + (row_ok ? qi : 0)) * D;
+                const int head = t ? g.head[1] : g.head[0];
+                const int64_t o_off =
+                    kPacked ? (int64_t)(g.q_tok + (row_ok ? qi : 0)) * p.o_tok + head * p.o_head
+                            : ((int64_t)bh * p.S_q + (row_ok ? qi : 0)) * D;
+                __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.O) + o_off;
                 __syncwarp();
                 // all of O_t into registers (one wait), then O_t is free for the next
                 // item's first PV while this warp normalises and stores
@@ -576,7 +747,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             *reinterpret_cast<uint4*>(orow + oc * 32 + e) = w;
                         }
                 }
-                if (row_ok && p.lse) p.lse[(int64_t)bh * p.S_q + qi] = lse_v;
+                if (row_ok && p.lse)
+                    p.lse[kPacked ? (int64_t)head * p.total_q + g.q_tok + qi
+                                  : (int64_t)bh * p.S_q + qi] = lse_v;
             } else {
                 // stage this warp's 32 rows (D * 2 bytes each, 16-byte slots swizzled by
                 // row) in the tile's Q buffer: every MMA that read it has completed
@@ -602,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
                 // the warp's rows are contiguous in O: whole 512-byte stores to every rank
-                const int row0 = q0 + t * BQ + quad * 32;
+                const int row0 = q0 + quad * 32;
                 const int nrows = max(0, min(32, p.S_q - row0));
                 const int64_t grow = (int64_t)(p.bh_base + bh) * p.S_q + row0;
                 for (int i = 1; i <= p.world; ++i) {
@@ -618,6 +791,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         c_t += nt;
+        if constexpr (kPacked) {
+            __syncwarp();
+            if (lane == 0) it_done(it);
+        }
         }
     }
     if constexpr (kAllGather) {
@@ -699,6 +876,9 @@ int launch_fa(const void* Q, const void* K, const void* V, void* O, float* lse, 
     p.mbox = nullptr;
     p.seq = 0;
     p.done = nullptr;
+    p.o_tok = p.o_head = 0;
+    p.total_q = 0;
+    p.plan = VarlenPlan{};
     auto kern = k_flash_fwd<D, kPaged, false>;
     if constexpr (!kPaged) {
         if (ag) {
@@ -734,8 +914,64 @@ int launch_fa(const void* Q, const void* K, const void* V, void* O, float* lse, 
     return AMP_OK;
 }
 
+struct PackedArgs {
+    const void *Q, *K, *V;
+    void* O;
+    float* lse;
+    const int *cu_q, *cu_kv;
+    int B, total_q, total_kv, Hq, Hkv, causal;
+    const int64_t* strides;   // token and head stride of Q, K, V, O in elements
+    float scale;
+    void* ws;
+};
+
+template <int D>
+int launch_packed(const PackedArgs& a, cudaStream_t st) {
+    CUtensorMap tq, tk, tv;
+    int rc;
+    if ((rc = fa_make_tmap_packed(&tq, a.Q, D, a.total_q, a.Hq, a.strides[0], a.strides[1]))) return rc;
+    if (a.total_kv > 0) {
+        if ((rc = fa_make_tmap_packed(&tk, a.K, D, a.total_kv, a.Hkv, a.strides[2], a.strides[3]))) return rc;
+        if ((rc = fa_make_tmap_packed(&tv, a.V, D, a.total_kv, a.Hkv, a.strides[4], a.strides[5]))) return rc;
+    } else {
+        tk = tv = tq;   // no key anywhere: what a tile brings is masked and zeroed
+    }
+    FaParams p = {};
+    if ((rc = device_status(&p.status))) return rc;
+    p.B = a.B;
+    p.Hq = a.Hq;
+    p.Hkv = a.Hkv;
+    p.causal = a.causal;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.O = a.O;
+    p.lse = a.lse;
+    p.o_tok = a.strides[6];
+    p.o_head = a.strides[7];
+    p.total_q = a.total_q;
+    p.plan = varlen_plan_at(a.ws, a.B);
+    if ((rc = varlen_make_plan(p.plan, a.cu_q, a.cu_kv, a.total_q, a.total_kv, a.Hq, a.Hkv, false, st)))
+        return rc;
+    auto kern = k_flash_fwd<D, false, false, true, true>;
+    AMPB_CHECK_CUDA(
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FaCfg<D>::SMEM));
+    // no more CTAs than there can be items
+    const int64_t most = ((int64_t)a.total_q / BQ + a.B) * a.Hq;
+    AMPB_CHECK_CUDA(launch_pdl(kern, dim3((unsigned)std::min<int64_t>(most, sm_count())),
+                               dim3(kThreads), FaCfg<D>::SMEM, st, tq, tk, tv, p));
+    return AMP_OK;
+}
+
 }  // namespace
 
+// Packed [tokens][heads][d] bf16 tensor with the given strides (elements) as a 3-D TMA
+// map (d, token, head), box [1][128][64], 128-byte swizzle.
+int fa_make_tmap_packed(CUtensorMap* m, const void* base, int64_t d, int64_t tokens, int64_t heads,
+                        int64_t tok_stride, int64_t head_stride) {
+    cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)tokens, (cuuint64_t)heads};
+    cuuint64_t strides[2] = {(cuuint64_t)(tok_stride * 2), (cuuint64_t)(head_stride * 2)};
+    cuuint32_t box[3] = {64, 128, 1};
+    return encode_tmap(m, base, 2, 3, dims, strides, box);
+}
 
 // [bh][s][d] bf16 tensor as a 3-D TMA map, box [1][128][64], 128-byte swizzle.
 int fa_make_tmap_3d(CUtensorMap* m, const void* base, int64_t d, int64_t s, int64_t bh) {
@@ -814,9 +1050,60 @@ int paged_prefill_dev(const void* q, const void* k_pool, const void* v_pool,
     }
 }
 
+int varlen_check(int B, int total_q, int total_kv, int Hq, int Hkv, int D, const int* cu_q,
+                 const int* cu_kv, const int64_t* strides, int n_strides, const void* ws,
+                 size_t ws_bytes, size_t need) {
+    AMPB_REQUIRE(B > 0 && Hq > 0 && Hkv > 0 && total_q >= 0 && total_kv >= 0, AMP_ERR_INVALID,
+                 "packed attention: B, Hq and Hkv must be positive, token counts >= 0");
+    AMPB_REQUIRE(Hq % Hkv == 0, AMP_ERR_INVALID, "num_q_heads (%d) must be a multiple of "
+                 "num_kv_heads (%d)", Hq, Hkv);
+    AMPB_REQUIRE(D == 64 || D == 128, AMP_ERR_UNSUPPORTED,
+                 "packed attention: head_dim %d not supported (64, 128)", D);
+    AMPB_REQUIRE(cu_q && cu_kv && strides, AMP_ERR_INVALID, "NULL offsets or strides");
+    // tokens and the rows a tile reads past them, and items, are 32-bit numbers
+    AMPB_REQUIRE(total_q <= INT32_MAX - 512 && total_kv <= INT32_MAX - 512 && Hq <= 65535 &&
+                     ((int64_t)(std::max(total_q, total_kv) / 128) + B) * Hq <= INT32_MAX / 2 &&
+                     (int64_t)total_q * Hq <= INT32_MAX,
+                 AMP_ERR_UNSUPPORTED, "packed attention too large");
+    for (int i = 0; i < n_strides; ++i)
+        AMPB_REQUIRE(strides[i] > 0 && strides[i] % 8 == 0 && strides[i] < (1ll << 38),
+                     AMP_ERR_INVALID,
+                     "packed attention: stride %d (%lld elements) must be a positive multiple of 8",
+                     i, (long long)strides[i]);
+    AMPB_REQUIRE(ws && aligned16(ws), AMP_ERR_INVALID, "workspace must be 16-byte aligned");
+    AMPB_REQUIRE(ws_bytes >= need, AMP_ERR_INVALID, "workspace too small: %zu < %zu", ws_bytes, need);
+    return AMP_OK;
+}
+
 }  // namespace ampb
 
 using namespace ampb;
+
+extern "C" size_t amp_flash_attn_varlen_workspace_bytes(int B) {
+    return B > 0 ? varlen_plan_bytes(B) : 0;
+}
+
+extern "C" int amp_flash_attn_varlen_fwd_bf16_dev(const void* Q, const void* K, const void* V,
+                                                  void* O, float* lse, const int32_t* cu_seqlens_q,
+                                                  const int32_t* cu_seqlens_kv, int B, int total_q,
+                                                  int total_kv, int Hq, int Hkv, int head_dim,
+                                                  const int64_t* strides, int causal, float scale,
+                                                  void* workspace, size_t workspace_bytes,
+                                                  void* stream) {
+    int rc = varlen_check(B, total_q, total_kv, Hq, Hkv, head_dim, cu_seqlens_q, cu_seqlens_kv,
+                          strides, 8, workspace, workspace_bytes,
+                          amp_flash_attn_varlen_workspace_bytes(B));
+    if (rc) return rc;
+    if (total_q == 0) return AMP_OK;
+    AMPB_REQUIRE(Q && O && (total_kv == 0 || (K && V)), AMP_ERR_INVALID, "NULL tensor");
+    AMPB_REQUIRE(aligned16(Q) && aligned16(K) && aligned16(V) && aligned16(O), AMP_ERR_INVALID,
+                 "Q, K, V, O must be 16-byte aligned");
+    if (!(scale > 0.0f)) scale = 1.0f / sqrtf((float)head_dim);
+    const PackedArgs a = {Q,  K,       V,        O,  lse, cu_seqlens_q, cu_seqlens_kv, B, total_q,
+                          total_kv, Hq, Hkv, causal, strides, scale, workspace};
+    return head_dim == 128 ? launch_packed<128>(a, as_stream(stream))
+                           : launch_packed<64>(a, as_stream(stream));
+}
 
 extern "C" int amp_paged_attn_prefill_bf16_dev(const void* q, const void* k_pool,
                                                const void* v_pool, const int32_t* block_table,

@@ -23,7 +23,14 @@
 // dV_t, S^T_{t+1}, dK_t, dP^T_{t+1}); the dQ pass keeps two S buffers in TMEM
 // (S_{j+1}, dQ_j, dP_{j+1}).
 // Each pass recomputes P from lse, so there are no atomics and no fp32 dQ
-// accumulator in global memory.  Both kernels: 384 threads; warp 0 TMA, warp 1
+// accumulator in global memory.
+// Packed mode (sequences of different lengths one after another, varlen.cuh): both
+// passes draw their tiles from the plan's lists, longest sequence and most steps first;
+// warp 3 decodes items ahead into a two-slot ring.  A tile that runs past its sequence
+// brings rows of the next one.  Where those rows would be summed over (Q and dO in the
+// dK/dV pass, K and V in the dQ pass) warp 2 zeroes them in shared memory before the
+// MMAs may read them; where they are rows of the output they are just not stored.
+// Both kernels: 384 threads; warp 0 TMA, warp 1
 // TMEM + MMA issue (warps 2-3 only lend their registers, setmaxnreg 72 / 216);
 // warps 4-11 the element-wise work, two warps per TMEM lane quadrant (one row
 // per thread), each taking one 64-column half of the 128-column tile.
@@ -36,10 +43,16 @@
 #include "common.cuh"
 #include "runtime.h"
 #include "tc_common.cuh"
+#include "varlen.cuh"
 
 namespace ampb {
 
 int fa_make_tmap_3d(CUtensorMap* m, const void* base, int64_t d, int64_t s, int64_t bh);
+int fa_make_tmap_packed(CUtensorMap* m, const void* base, int64_t d, int64_t tokens, int64_t heads,
+                        int64_t tok_stride, int64_t head_stride);
+int varlen_check(int B, int total_q, int total_kv, int Hq, int Hkv, int D, const int* cu_q,
+                 const int* cu_kv, const int64_t* strides, int n_strides, const void* ws,
+                 size_t ws_bytes, size_t need);
 
 namespace {
 
@@ -55,6 +68,9 @@ template <int D>
 struct BwdCfg {
     static constexpr int SLABS = D / 64;
     static constexpr int TILE = SLABS * SLAB_BYTES;          // 128 rows x D bf16
+    // tiles, lse and Delta columns, alignment, barriers with the packed items
+    static constexpr int SMEM_KV = 6 * TILE + 2 * 2 * BT * 4 + 1024 + 384;
+    static constexpr int SMEM_Q = 6 * TILE + 1024 + 384;
     static constexpr uint32_t IDESC_SS = make_idesc(1, 1, 0, 0, BT, BT);
     static constexpr uint32_t IDESC_TS = make_idesc(1, 1, 0, 1, BT, D);
 };
@@ -69,7 +85,95 @@ struct BwdParams {
     void* dk;                    // [B*Hkv][S_kv][D] bf16
     void* dv;
     int* status;
+    // packed mode: rows of the whole Q (lse, delta are [Hq][total_q]), strides of the
+    // gradients in elements, the work lists
+    int total_q;
+    int64_t dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
+    VarlenPlan plan;
 };
+
+// One item: a 128-row tile of one head of one sequence (dense: of one batch entry).
+struct BwdItem {
+    int live;                   // packed: 0 ends the list
+    int b, head, tile;          // head: kv head (dK/dV) or query head (dQ) within b
+    int q_tok, k_tok;           // packed: the sequence's first rows
+    int S_q, S_kv, coff;
+};
+
+// Packed mode, warp 3: draws item after item of list `which` and publishes it.
+template <bool kKeys>
+__device__ __forceinline__ void draw_items(const BwdParams& p, BwdItem* items, uint64_t* it_full,
+                                           uint64_t* it_empty) {
+    constexpr int which = kKeys ? 0 : 1;
+    const int lane = threadIdx.x & 31;
+    const int total = p.plan.first[which][p.plan.B];
+    for (int k = 0;; ++k) {
+        if (k >= 2 && !mbar_wait_warp(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) return;
+        int item = (int)blockIdx.x;
+        if (k > 0) {
+            if (lane == 0) item = (int)gridDim.x + atomicAdd(&p.plan.next[which], 1);
+            item = __shfl_sync(0xffffffffu, item, 0);
+        }
+        BwdItem it = {};
+        if (item < total) {
+            const int r = varlen_find(p.plan.first[which], p.plan.B, item);
+            const VarlenSeq sq = p.plan.seqs[r];
+            const int n = varlen_tiles(kKeys ? sq.k_len : sq.q_len);
+            const int w = item - p.plan.first[which][r];
+            it.live = 1;
+            it.head = w / n;
+            // under a causal mask the first keys and the last queries have the most steps
+            it.tile = kKeys ? w % n : n - 1 - w % n;
+            it.q_tok = sq.q_off;
+            it.k_tok = sq.k_off;
+            it.S_q = sq.q_len;
+            it.S_kv = sq.k_len;
+            it.coff = sq.k_len - sq.q_len;
+        }
+        if (lane == 0) {
+            items[k & 1] = it;
+            mbar_arrive(&it_full[k & 1]);
+        }
+        __syncwarp();
+        if (item >= total) return;
+    }
+}
+
+// Reads the k-th published item; false at the end (or when a wait ran out).
+__device__ __forceinline__ bool read_item(int k, const BwdItem* items, uint64_t* it_full,
+                                          int* status, BwdItem& it) {
+    if (!mbar_wait(&it_full[k & 1], (k >> 1) & 1, status)) return false;
+    const volatile BwdItem& src = items[k & 1];
+    it.live = src.live;
+    it.b = 0;
+    it.head = src.head;
+    it.tile = src.tile;
+    it.q_tok = src.q_tok;
+    it.k_tok = src.k_tok;
+    it.S_q = src.S_q;
+    it.S_kv = src.S_kv;
+    it.coff = src.coff;
+    return it.live != 0;
+}
+
+// Packed mode, warp 2: once the tile has landed, zeroes its rows from `valid` on (one
+// or two tiles of `slabs` slabs each) and passes it on to the MMA warp.
+__device__ __forceinline__ bool zero_tail(uint64_t* raw, uint32_t parity, uint64_t* full,
+                                          uint8_t* tile0, uint8_t* tile1, int slabs, int valid,
+                                          int* status) {
+    if (!mbar_wait_warp(raw, parity, status)) return false;
+    const int lane = threadIdx.x & 31;
+    for (int i = valid * 8 + lane; i < BT * 8; i += 32)
+        for (int sl = 0; sl < slabs; ++sl) {
+            *reinterpret_cast<uint4*>(tile0 + sl * SLAB_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            if (tile1)
+                *reinterpret_cast<uint4*>(tile1 + sl * SLAB_BYTES + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(full);
+    return true;
+}
 
 // SS product of two 128-row K-major tiles over D: acc[128 x 128] (+)= A B^T
 template <int D>
@@ -100,10 +204,17 @@ __device__ __forceinline__ void mma_ts(uint32_t acc, uint32_t t_col, uint32_t b_
 // once): D/8 lanes per row with 16-byte loads, kDeltaLoads rows per lane group in
 // flight, and the row's partial sums reduced within its lane group.
 constexpr int kDeltaLoads = 4;
-template <int D>
+// Packed: row r is head r % H of token r / H (the order in which a contiguous
+// [total, H, D] lies in memory), read through the strides and stored at [head][token].
+struct DeltaStrides {
+    int64_t o_tok, o_head, do_tok, do_head;
+    int H, total;
+};
+template <int D, bool kPacked = false>
 __global__ void __launch_bounds__(256) k_fa_bwd_delta(const __nv_bfloat16* __restrict__ O,
                                                       const __nv_bfloat16* __restrict__ dO,
-                                                      float* __restrict__ delta, int64_t rows) {
+                                                      float* __restrict__ delta, int64_t rows,
+                                                      DeltaStrides st = {}) {
     pdl_wait();
     pdl_trigger();
     constexpr int LPR = D / 8;            // lanes per row, 8 bf16 (16 bytes) each
@@ -120,8 +231,14 @@ __global__ void __launch_bounds__(256) k_fa_bwd_delta(const __nv_bfloat16* __res
         for (int u = 0; u < kDeltaLoads; ++u) {
             const int64_t r = r0 + u * RPW + sub;
             if (r < rows) {
-                o[u] = *reinterpret_cast<const uint4*>(O + r * D + col);
-                g[u] = *reinterpret_cast<const uint4*>(dO + r * D + col);
+                if constexpr (kPacked) {
+                    const int t = (int)r / st.H, h = (int)r % st.H;
+                    o[u] = *reinterpret_cast<const uint4*>(O + t * st.o_tok + h * st.o_head + col);
+                    g[u] = *reinterpret_cast<const uint4*>(dO + t * st.do_tok + h * st.do_head + col);
+                } else {
+                    o[u] = *reinterpret_cast<const uint4*>(O + r * D + col);
+                    g[u] = *reinterpret_cast<const uint4*>(dO + r * D + col);
+                }
             } else {
                 o[u] = make_uint4(0u, 0u, 0u, 0u);
                 g[u] = o[u];
@@ -140,7 +257,12 @@ __global__ void __launch_bounds__(256) k_fa_bwd_delta(const __nv_bfloat16* __res
 #pragma unroll
             for (int m = LPR / 2; m > 0; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
             const int64_t r = r0 + u * RPW + sub;
-            if (lane % LPR == 0 && r < rows) delta[r] = acc;
+            if (lane % LPR == 0 && r < rows) {
+                if constexpr (kPacked)
+                    delta[(int64_t)((int)r % st.H) * st.total + (int)r / st.H] = acc;
+                else
+                    delta[r] = acc;
+            }
         }
     }
 }
@@ -179,7 +301,7 @@ __device__ __forceinline__ void store_zero_row(__nv_bfloat16* row, int half) {
 }
 
 // ---------------------------------------------------------------- dK, dV
-template <int D>
+template <int D, bool kPacked = false>
 __global__ void __launch_bounds__(kThreads, 1)
     k_fa_bwd_dkdv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -210,10 +332,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* kv_empty = bars + 14;   // the item's last MMA reading K / V has completed
     uint64_t* dkv_free = bars + 15;   // the item's epilogue has read dK, dV out of TMEM
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+    uint64_t* it_full = bars + 17;    // [2] packed items
+    uint64_t* it_empty = bars + 19;   // [2] load, MMA and zeroing warps, 8 element-wise warps
+    uint64_t* qs_raw = bars + 21;     // [2] Q / dO loaded, rows past the end not yet zeroed
+    BwdItem* items = reinterpret_cast<BwdItem*>(bars + 23);   // [2]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.Hq / p.Hkv;
-    const int n_qt = (p.S_q + BT - 1) / BT;
     const int n_kt = (p.S_kv + BT - 1) / BT;
     // Persistent: unit u = blockIdx.x + (k/2) * gridDim.x pairs key tile n_kt-1-q with
     // key tile q of one kv head (under a causal mask they see the fewest and the most
@@ -229,15 +354,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         jt = (k & 1) ? q : n_kt - 1 - q;
         return ((k & 1) && q == n_kt - 1 - q) ? 2 : 1;
     };
-    // first query tile with a query that sees a key of tile jt
-    auto first_tile = [&](int jt) {
+    // the same with the item's geometry; packed: from the ring, released with it_done
+    auto next_item = [&](int k, BwdItem& it) -> int {
+        if constexpr (kPacked) {
+            return read_item(k, items, it_full, p.status, it) ? 1 : 0;
+        } else {
+            int bh_kv, jt;
+            const int st = item_at(k, bh_kv, jt);
+            if (st == 1) {
+                it.b = bh_kv / p.Hkv;
+                it.head = bh_kv % p.Hkv;
+                it.tile = jt;
+                it.q_tok = it.k_tok = 0;
+                it.S_q = p.S_q;
+                it.S_kv = p.S_kv;
+                it.coff = p.causal_offset;
+            }
+            return st;
+        }
+    };
+    auto it_done = [&](int k) {
+        if constexpr (kPacked) mbar_arrive(&it_empty[k & 1]);
+    };
+    // first query tile with a query that sees a key of the item's tile
+    auto first_tile = [&](const BwdItem& it) {
         int i_lo = 0;
         if (p.causal) {
-            const int first_q = jt * BT - p.causal_offset;
+            const int first_q = it.tile * BT - it.coff;
             i_lo = first_q <= 0 ? 0 : first_q / BT;
         }
         return i_lo;
     };
+    auto q_tiles = [&](const BwdItem& it) { return (it.S_q + BT - 1) / BT; };
 
     if (threadIdx.x == 0) {
         mbar_init(kv_full, 1);
@@ -255,6 +403,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(drain, 1);
         mbar_init(&cols_ready[0], 256);
         mbar_init(&cols_ready[1], 256);
+        if constexpr (kPacked) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&it_full[i], 1);
+                mbar_init(&it_empty[i], 11);
+                mbar_init(&qs_raw[i], 1);
+            }
+        }
         fence_barrier_init();
         fence_proxy_async_smem();
     }
@@ -277,35 +432,39 @@ __global__ void __launch_bounds__(kThreads, 1)
             int g = 0, li = 0;   // Q/dO tiles loaded (ring stage g & 1); items with work
             bool ok = true;
             for (int k = 0; ok; ++k) {
-                int bh_kv, jt;
-                const int st = item_at(k, bh_kv, jt);
+                BwdItem it;
+                const int st = next_item(k, it);
                 if (st == 0) break;
                 if (st == 2) continue;
-                const int i_lo = first_tile(jt);
-                const int per_head = max(0, n_qt - i_lo);
+                it_done(k);
+                const int i_lo = first_tile(it);
+                const int per_head = max(0, q_tiles(it) - i_lo);
                 const int steps = G * per_head;
                 if (steps == 0) continue;
-                const int b = bh_kv / p.Hkv, hk = bh_kv % p.Hkv;
+                const int b = it.b, hk = it.head, bh_kv = b * p.Hkv + hk;
+                const int k_row = it.k_tok + it.tile * BT;
                 // K_j / V_j once the previous item's last MMA reading them has completed
                 if (li > 0 && !mbar_wait(kv_empty, (li - 1) & 1, p.status)) break;
                 mbar_arrive_expect_tx(kv_full, 2 * CF::TILE);
 #pragma unroll
                 for (int sl = 0; sl < CF::SLABS; ++sl) {
-                    tma_load_3d(k_s + sl * SLAB_BYTES, &tmK, kv_full, sl * 64, jt * BT, bh_kv);
-                    tma_load_3d(v_s + sl * SLAB_BYTES, &tmV, kv_full, sl * 64, jt * BT, bh_kv);
+                    tma_load_3d(k_s + sl * SLAB_BYTES, &tmK, kv_full, sl * 64, k_row, bh_kv);
+                    tma_load_3d(v_s + sl * SLAB_BYTES, &tmV, kv_full, sl * 64, k_row, bh_kv);
                 }
                 for (int t = 0; t < steps; ++t, ++g) {
                     const int s = g & 1;
                     if (!mbar_wait(&qs_empty[s], ((g >> 1) & 1) ^ 1, p.status)) { ok = false; break; }
-                    const int gq = t / per_head, it = i_lo + t % per_head;
+                    const int gq = t / per_head, qt = i_lo + t % per_head;
                     const int bh_q = b * p.Hq + hk * G + gq;
-                    mbar_arrive_expect_tx(&qs_full[s], 2 * CF::TILE);
+                    // packed: a tile past the sequence's end goes to warp 2 first
+                    uint64_t* bar = kPacked && (qt + 1) * BT > it.S_q ? &qs_raw[s] : &qs_full[s];
+                    mbar_arrive_expect_tx(bar, 2 * CF::TILE);
 #pragma unroll
                     for (int sl = 0; sl < CF::SLABS; ++sl) {
-                        tma_load_3d(q_s + s * CF::TILE + sl * SLAB_BYTES, &tmQ, &qs_full[s],
-                                    sl * 64, it * BT, bh_q);
-                        tma_load_3d(o_s + s * CF::TILE + sl * SLAB_BYTES, &tmdO, &qs_full[s],
-                                    sl * 64, it * BT, bh_q);
+                        tma_load_3d(q_s + s * CF::TILE + sl * SLAB_BYTES, &tmQ, bar, sl * 64,
+                                    it.q_tok + qt * BT, bh_q);
+                        tma_load_3d(o_s + s * CF::TILE + sl * SLAB_BYTES, &tmdO, bar, sl * 64,
+                                    it.q_tok + qt * BT, bh_q);
                     }
                 }
                 ++li;
@@ -321,11 +480,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             int g = 0, li = 0;   // steps before this item; items with work before it
             bool ok = true;
             for (int k = 0; ok; ++k) {
-                int bh_kv, jt;
-                const int st = item_at(k, bh_kv, jt);
+                BwdItem it;
+                const int st = next_item(k, it);
                 if (st == 0) break;
                 if (st == 2) continue;
-                const int steps = G * max(0, n_qt - first_tile(jt));
+                it_done(k);
+                const int steps = G * max(0, q_tiles(it) - first_tile(it));
                 if (steps == 0) continue;
                 const uint32_t ka = opaque_u32(ka0), va = opaque_u32(va0);
                 if (!(mbar_wait(kv_full, li & 1, p.status) &&
@@ -379,6 +539,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_commit(drain);
             mbar_wait(drain, 0, p.status);
         }
+    } else if (kPacked && warp == 2) {
+        // rows of Q and dO past the sequence's end: zeroed in shared memory
+        int g = 0;                           // tiles loaded before this item
+        uint32_t phase0 = 0, phase1 = 0;     // qs_raw phases used
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+            BwdItem it;
+            const bool any = __all_sync(0xffffffffu, read_item(k, items, it_full, p.status, it));
+            if (!any) break;
+            __syncwarp();
+            if (lane == 0) it_done(k);
+            const int per_head = max(0, q_tiles(it) - first_tile(it));
+            const int valid = it.S_q - (q_tiles(it) - 1) * BT;   // rows of the last tile
+            if (per_head > 0 && valid < BT)
+                for (int gq = 0; ok && gq < G; ++gq) {           // the last tile of each head
+                    const int s = (g + gq * per_head + per_head - 1) & 1;
+                    ok = zero_tail(&qs_raw[s], (s ? phase1 : phase0) & 1, &qs_full[s],
+                                   q_s + s * CF::TILE, o_s + s * CF::TILE, CF::SLABS, valid,
+                                   p.status);
+                    if (s) ++phase1; else ++phase0;
+                }
+            g += G * per_head;
+        }
+    } else if (kPacked && warp == 3) {
+        draw_items<true>(p, items, it_full, it_empty);
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegEw));
@@ -396,32 +581,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         int gs = 0;   // steps before this item
         bool ok = true;
         for (int k = 0; ok; ++k) {
-        int bh_kv, jt;
-        const int st = item_at(k, bh_kv, jt);
+        BwdItem item;
+        int st = next_item(k, item);
+        if constexpr (kPacked) st = __all_sync(0xffffffffu, st == 1);
         if (st == 0) break;
         if (st == 2) continue;
-        const int b = bh_kv / p.Hkv, hk = bh_kv % p.Hkv;
-        const int kj = jt * BT + kr;
-        const int i_lo = first_tile(jt);
-        const int per_head = max(0, n_qt - i_lo);
+        const int b = item.b, hk = item.head, bh_kv = b * p.Hkv + hk;
+        const int kj = item.tile * BT + kr;
+        const int i_lo = first_tile(item);
+        const int per_head = max(0, q_tiles(item) - i_lo);
         const int steps = G * per_head;
-        __nv_bfloat16* dk_row = static_cast<__nv_bfloat16*>(p.dk) + ((int64_t)bh_kv * p.S_kv + (kj < p.S_kv ? kj : 0)) * D;
-        __nv_bfloat16* dv_row = static_cast<__nv_bfloat16*>(p.dv) + ((int64_t)bh_kv * p.S_kv + (kj < p.S_kv ? kj : 0)) * D;
+        const bool row_ok = kj < item.S_kv;
+        const int64_t dense_row = ((int64_t)bh_kv * p.S_kv + (row_ok ? kj : 0)) * D;
+        const int64_t tok = item.k_tok + (row_ok ? kj : 0);
+        __nv_bfloat16* dk_row = static_cast<__nv_bfloat16*>(p.dk) +
+                                (kPacked ? tok * p.dk_tok + hk * p.dk_head : dense_row);
+        __nv_bfloat16* dv_row = static_cast<__nv_bfloat16*>(p.dv) +
+                                (kPacked ? tok * p.dv_tok + hk * p.dv_head : dense_row);
         if (steps == 0) {   // no query sees these keys: dK = dV = 0, no barriers
-            if (kj < p.S_kv) {
+            if (row_ok) {
                 store_zero_row<D>(dk_row, half);
                 store_zero_row<D>(dv_row, half);
+            }
+            if constexpr (kPacked) {
+                __syncwarp();
+                if (lane == 0) it_done(k);
             }
             continue;
         }
         // -lse2 / -Delta of query `tid` of step t's tile (threads tid < 128)
         auto fetch = [&](int t, float& nl2, float& ndl) {
-            const int gq = t / per_head, it = i_lo + t % per_head;
-            const int q = it * BT + tid;
-            const int64_t row = (int64_t)(b * p.Hq + hk * G + gq) * p.S_q + q;
-            const float lse = q < p.S_q ? p.lse[row] : -INFINITY;
+            const int gq = t / per_head, qt = i_lo + t % per_head;
+            const int q = qt * BT + tid;
+            const int64_t row = (int64_t)(b * p.Hq + hk * G + gq) * (kPacked ? p.total_q : p.S_q) +
+                                item.q_tok + q;
+            const float lse = q < item.S_q ? p.lse[row] : -INFINITY;
             nl2 = lse == -INFINITY ? -INFINITY : -lse * kLog2e;   // -inf: the column's P is 0
-            ndl = q < p.S_q ? -p.delta[row] : 0.0f;
+            ndl = q < item.S_q ? -p.delta[row] : 0.0f;
         };
         float nl2 = 0.0f, ndl = 0.0f;
         if (tid < BT) fetch(0, nl2, ndl);
@@ -442,8 +638,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             // e < lo are masked (q = q0 + e)
             const int q0 = (i_lo + t % per_head) * BT + half * 64;
             int lo = 0;
-            if (kj >= p.S_kv) lo = 64;
-            else if (p.causal) lo = min(64, max(0, kj - p.causal_offset - q0));
+            if (!row_ok) lo = 64;
+            else if (p.causal) lo = min(64, max(0, kj - item.coff - q0));
             const bool dense = __all_sync(0xffffffffu, lo == 0);
             const float* hcl = cl + half * 64;
             // phase P (needs S^T only): P^T = exp2(S^T c - lse2), kept as bf16 pairs
@@ -512,12 +708,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && !mbar_wait_warp(dk_done, (gs + steps - 1) & 1, p.status)) ok = false;
         if (!ok) break;
         tc_fence_after();
-        store_row<D>(T_dK + lane_base, p.scale, dk_row, kj < p.S_kv, half);
-        store_row<D>(T_dV + lane_base, 1.0f, dv_row, kj < p.S_kv, half);
+        store_row<D>(T_dK + lane_base, p.scale, dk_row, row_ok, half);
+        store_row<D>(T_dV + lane_base, 1.0f, dv_row, row_ok, half);
         // both accumulators are read out of TMEM: the next item's dV / dK may run
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(dkv_free);
+        if (lane == 0) {
+            mbar_arrive(dkv_free);
+            it_done(k);
+        }
         gs += steps;
         }
     }
@@ -538,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // S buffer g & 1); Q/dO reload once the item's last dP has been issued (q_empty),
 // and an item's first dQ MMA waits for the previous item's epilogue to have read
 // dQ out of TMEM (dq_free).
-template <int D>
+template <int D, bool kPacked = false>
 __global__ void __launch_bounds__(kThreads, 1)
     k_fa_bwd_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -567,6 +766,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* q_empty = bars + 15;    // the item's last MMA reading Q / dO has completed
     uint64_t* dq_free = bars + 16;    // the item's epilogue has read dQ out of TMEM
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+    uint64_t* it_full = bars + 18;    // [2] packed items
+    uint64_t* it_empty = bars + 20;   // [2] load, MMA and zeroing warps, 8 element-wise warps
+    uint64_t* k_raw = bars + 22;      // [2] loaded, rows past the end not yet zeroed
+    uint64_t* v_raw = bars + 24;      // [2]
+    BwdItem* items = reinterpret_cast<BwdItem*>(bars + 26);   // [2]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n_qt = (p.S_q + BT - 1) / BT;
@@ -581,10 +785,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         it = (k & 1) ? q : n_qt - 1 - q;
         return ((k & 1) && q == n_qt - 1 - q) ? 2 : 1;
     };
-    auto kv_tiles = [&](int it) {
-        int n_kv = (p.S_kv + BT - 1) / BT;
+    // the same with the item's geometry; packed: from the ring, released with it_done
+    auto next_item = [&](int k, BwdItem& it) -> int {
+        if constexpr (kPacked) {
+            return read_item(k, items, it_full, p.status, it) ? 1 : 0;
+        } else {
+            int bh, tile;
+            const int st = item_at(k, bh, tile);
+            if (st == 1) {
+                it.b = bh / p.Hq;
+                it.head = bh % p.Hq;
+                it.tile = tile;
+                it.q_tok = it.k_tok = 0;
+                it.S_q = p.S_q;
+                it.S_kv = p.S_kv;
+                it.coff = p.causal_offset;
+            }
+            return st;
+        }
+    };
+    auto it_done = [&](int k) {
+        if constexpr (kPacked) mbar_arrive(&it_empty[k & 1]);
+    };
+    auto kv_tiles = [&](const BwdItem& it) {
+        int n_kv = (it.S_kv + BT - 1) / BT;
         if (p.causal) {
-            const int last = it * BT + BT - 1 + p.causal_offset;
+            const int last = it.tile * BT + BT - 1 + it.coff;
             n_kv = min(n_kv, last < 0 ? 0 : last / BT + 1);
         }
         return n_kv;
@@ -606,6 +832,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(ds_full, 8);
         mbar_init(dq_done, 1);
         mbar_init(drain, 1);
+        if constexpr (kPacked) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&it_full[i], 1);
+                mbar_init(&it_empty[i], 11);
+                mbar_init(&k_raw[i], 1);
+                mbar_init(&v_raw[i], 1);
+            }
+        }
         fence_barrier_init();
         fence_proxy_async_smem();
     }
@@ -629,35 +863,41 @@ __global__ void __launch_bounds__(kThreads, 1)
             int g = 0, li = 0;   // K/V tiles loaded; items with work loaded
             bool ok = true;
             for (int k = 0; ok; ++k) {
-                int bh, it;
-                const int st = item_at(k, bh, it);
+                BwdItem it;
+                const int st = next_item(k, it);
                 if (st == 0) break;
+                if (st == 1) it_done(k);
                 const int n_kv = st == 1 ? kv_tiles(it) : 0;
                 if (n_kv == 0) continue;
-                const int b = bh / p.Hq, h = bh % p.Hq;
+                const int b = it.b, h = it.head, bh = b * p.Hq + h;
                 const int bh_kv = b * p.Hkv + h / (p.Hq / p.Hkv);
+                const int q_row = it.q_tok + it.tile * BT;
                 if (li > 0 && !mbar_wait(q_empty, (li - 1) & 1, p.status)) break;
                 mbar_arrive_expect_tx(q_full, 2 * CF::TILE);
 #pragma unroll
                 for (int sl = 0; sl < CF::SLABS; ++sl) {
-                    tma_load_3d(q_s + sl * SLAB_BYTES, &tmQ, q_full, sl * 64, it * BT, bh);
-                    tma_load_3d(o_s + sl * SLAB_BYTES, &tmdO, q_full, sl * 64, it * BT, bh);
+                    tma_load_3d(q_s + sl * SLAB_BYTES, &tmQ, q_full, sl * 64, q_row, bh);
+                    tma_load_3d(o_s + sl * SLAB_BYTES, &tmdO, q_full, sl * 64, q_row, bh);
                 }
                 for (int j = 0; j < n_kv; ++j, ++g) {
                     const int s = g & 1;
                     const uint32_t ph = ((g >> 1) & 1) ^ 1;
+                    // packed: a tile past the sequence's end goes to warp 2 first
+                    const bool raw = kPacked && (j + 1) * BT > it.S_kv;
+                    uint64_t* kb = raw ? &k_raw[s] : &k_full[s];
+                    uint64_t* vb = raw ? &v_raw[s] : &v_full[s];
                     if (!mbar_wait(&k_empty[s], ph, p.status)) { ok = false; break; }
-                    mbar_arrive_expect_tx(&k_full[s], CF::TILE);
+                    mbar_arrive_expect_tx(kb, CF::TILE);
 #pragma unroll
                     for (int sl = 0; sl < CF::SLABS; ++sl)
-                        tma_load_3d(k_s + s * CF::TILE + sl * SLAB_BYTES, &tmK, &k_full[s],
-                                    sl * 64, j * BT, bh_kv);
+                        tma_load_3d(k_s + s * CF::TILE + sl * SLAB_BYTES, &tmK, kb, sl * 64,
+                                    it.k_tok + j * BT, bh_kv);
                     if (!mbar_wait(&v_empty[s], ph, p.status)) { ok = false; break; }
-                    mbar_arrive_expect_tx(&v_full[s], CF::TILE);
+                    mbar_arrive_expect_tx(vb, CF::TILE);
 #pragma unroll
                     for (int sl = 0; sl < CF::SLABS; ++sl)
-                        tma_load_3d(v_s + s * CF::TILE + sl * SLAB_BYTES, &tmV, &v_full[s],
-                                    sl * 64, j * BT, bh_kv);
+                        tma_load_3d(v_s + s * CF::TILE + sl * SLAB_BYTES, &tmV, vb, sl * 64,
+                                    it.k_tok + j * BT, bh_kv);
                 }
                 ++li;
             }
@@ -671,9 +911,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             int g = 0, li = 0;   // steps before this item; items with work before it
             bool ok = true;
             for (int k = 0; ok; ++k) {
-                int bh, it;
-                const int st = item_at(k, bh, it);
+                BwdItem it;
+                const int st = next_item(k, it);
                 if (st == 0) break;
+                if (st == 1) it_done(k);
                 const int n_kv = st == 1 ? kv_tiles(it) : 0;
                 if (n_kv == 0) continue;
                 const uint32_t qa = opaque_u32(qa0), oa = opaque_u32(oa0);
@@ -728,6 +969,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_commit(drain);
             mbar_wait(drain, 0, p.status);
         }
+    } else if (kPacked && warp == 2) {
+        // rows of K and V past the sequence's end: zeroed in shared memory
+        int g = 0;                           // tiles loaded before this item
+        uint32_t phase0 = 0, phase1 = 0;     // k_raw / v_raw phases used
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+            BwdItem it;
+            const bool any = __all_sync(0xffffffffu, read_item(k, items, it_full, p.status, it));
+            if (!any) break;
+            __syncwarp();
+            if (lane == 0) it_done(k);
+            const int n_kv = kv_tiles(it);
+            const int valid = it.S_kv - (n_kv - 1) * BT;   // rows of the last tile
+            if (n_kv > 0 && valid < BT) {
+                const int s = (g + n_kv - 1) & 1;
+                const uint32_t ph = (s ? phase1++ : phase0++) & 1;
+                ok = zero_tail(&k_raw[s], ph, &k_full[s], k_s + s * CF::TILE, nullptr, CF::SLABS,
+                               valid, p.status) &&
+                     zero_tail(&v_raw[s], ph, &v_full[s], v_s + s * CF::TILE, nullptr, CF::SLABS,
+                               valid, p.status);
+            }
+            g += n_kv;
+        }
+    } else if (kPacked && warp == 3) {
+        draw_items<false>(p, items, it_full, it_empty);
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegEw));
@@ -743,23 +1009,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         int g = 0;   // steps before this item
         bool ok = true;
         for (int k = 0; ok; ++k) {
-        int bh, it;
-        const int st = item_at(k, bh, it);
+        BwdItem item;
+        int st = next_item(k, item);
+        if constexpr (kPacked) st = __all_sync(0xffffffffu, st == 1);
         if (st == 0) break;
         if (st == 2) continue;
-        const int n_kv = kv_tiles(it);
-        const int qi = it * BT + r;
-        const int64_t row = (int64_t)bh * p.S_q + qi;
-        __nv_bfloat16* dq_row = static_cast<__nv_bfloat16*>(p.dq) + ((int64_t)bh * p.S_q + (qi < p.S_q ? qi : 0)) * D;
+        const int bh = item.b * p.Hq + item.head;
+        const int n_kv = kv_tiles(item);
+        const int qi = item.tile * BT + r;
+        const bool row_ok = qi < item.S_q;
+        const int64_t row = (int64_t)bh * (kPacked ? p.total_q : p.S_q) + item.q_tok + qi;
+        __nv_bfloat16* dq_row =
+            static_cast<__nv_bfloat16*>(p.dq) +
+            (kPacked ? (int64_t)(item.q_tok + (row_ok ? qi : 0)) * p.dq_tok + item.head * p.dq_head
+                     : ((int64_t)bh * p.S_q + (row_ok ? qi : 0)) * D);
         if (n_kv == 0) {   // no visible key: dQ = 0, no barriers
-            if (qi < p.S_q) store_zero_row<D>(dq_row, half);
+            if (row_ok) store_zero_row<D>(dq_row, half);
+            if constexpr (kPacked) {
+                __syncwarp();
+                if (lane == 0) it_done(k);
+            }
             continue;
         }
-        const float lse = qi < p.S_q ? p.lse[row] : -INFINITY;
+        const float lse = row_ok ? p.lse[row] : -INFINITY;
         const float nl2 = lse == -INFINITY ? -INFINITY : -lse * kLog2e;   // -inf: P = 0
-        const float ndl = qi < p.S_q ? -p.delta[row] : 0.0f;
+        const float ndl = row_ok ? -p.delta[row] : 0.0f;
         const uint64_t nl2x2 = f2pack(nl2, nl2), ndlx2 = f2pack(ndl, ndl);
-        const int vis_hi = p.causal ? min(p.S_kv - 1, qi + p.causal_offset) : p.S_kv - 1;
+        const int vis_hi = p.causal ? min(item.S_kv - 1, qi + item.coff) : item.S_kv - 1;
         for (int j = 0; j < n_kv; ++j) {
             const int gj = g + j;
             // this half's key columns e > hi are masked
@@ -815,11 +1091,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && !mbar_wait_warp(dq_done, (g + n_kv - 1) & 1, p.status)) ok = false;
         if (!ok) break;
         tc_fence_after();
-        store_row<D>(T_dQ + lane_base, p.scale, dq_row, qi < p.S_q, half);
+        store_row<D>(T_dQ + lane_base, p.scale, dq_row, row_ok, half);
         // store_row has read this half of dQ out of TMEM: the next item's dQ may run
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(dq_free);
+        if (lane == 0) {
+            mbar_arrive(dq_free);
+            it_done(k);
+        }
         g += n_kv;
         }
     }
@@ -845,7 +1124,7 @@ int launch_bwd(const void* Q, const void* K, const void* V, const void* O, const
     if ((rc = fa_make_tmap_3d(&tv, V, D, S_kv, (int64_t)B * Hkv))) return rc;
     int* status = nullptr;
     if ((rc = device_status(&status))) return rc;
-    BwdParams p;
+    BwdParams p = {};
     p.B = B;
     p.Hq = Hq;
     p.Hkv = Hkv;
@@ -867,9 +1146,9 @@ int launch_bwd(const void* Q, const void* K, const void* V, const void* O, const
                                              (int64_t)sm_count() * 8);
     AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_delta<D>, dim3(dgrid), dim3(256), 0, st,
                                static_cast<const __nv_bfloat16*>(O),
-                               static_cast<const __nv_bfloat16*>(dO), delta, rows));
-    constexpr int SMEM_KV = 6 * CF::TILE + 2 * 2 * BT * 4 + 1024 + 256;
-    constexpr int SMEM_Q = 6 * CF::TILE + 1024 + 256;
+                               static_cast<const __nv_bfloat16*>(dO), delta, rows,
+                               DeltaStrides{}));
+    constexpr int SMEM_KV = CF::SMEM_KV, SMEM_Q = CF::SMEM_Q;
     static std::atomic<uint64_t> attr_done{0};
     int dev = 0;
     AMPB_CHECK_CUDA(cudaGetDevice(&dev));
@@ -890,6 +1169,89 @@ int launch_bwd(const void* Q, const void* K, const void* V, const void* O, const
     AMPB_REQUIRE(dq_units <= INT32_MAX / 2, AMP_ERR_UNSUPPORTED, "attention too large");
     AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_dq<D>, dim3((unsigned)std::min<int64_t>(dq_units, sm_count())),
                                dim3(kThreads), SMEM_Q, st, tq, tk, tv, to, p));
+    return AMP_OK;
+}
+
+struct PackedBwdArgs {
+    const void *Q, *K, *V, *O, *dO;
+    const float* lse;
+    void *dQ, *dK, *dV;
+    const int *cu_q, *cu_kv;
+    int B, total_q, total_kv, Hq, Hkv, causal;
+    const int64_t* strides;   // token and head stride of Q, K, V, O, dO, dQ, dK, dV
+    float scale;
+    void* ws;
+};
+
+template <int D>
+int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
+    using CF = BwdCfg<D>;
+    const int64_t* s = a.strides;
+    CUtensorMap tq, tk, tv, to;
+    int rc;
+    if (a.total_q > 0) {
+        if ((rc = fa_make_tmap_packed(&tq, a.Q, D, a.total_q, a.Hq, s[0], s[1]))) return rc;
+        if ((rc = fa_make_tmap_packed(&to, a.dO, D, a.total_q, a.Hq, s[8], s[9]))) return rc;
+    }
+    if (a.total_kv > 0) {
+        if ((rc = fa_make_tmap_packed(&tk, a.K, D, a.total_kv, a.Hkv, s[2], s[3]))) return rc;
+        if ((rc = fa_make_tmap_packed(&tv, a.V, D, a.total_kv, a.Hkv, s[4], s[5]))) return rc;
+    }
+    // with no query or no key at all every item is one without steps: no load is issued
+    if (a.total_q == 0) tq = to = tk;
+    if (a.total_kv == 0) tk = tv = tq;
+    BwdParams p = {};
+    if ((rc = device_status(&p.status))) return rc;
+    p.B = a.B;
+    p.Hq = a.Hq;
+    p.Hkv = a.Hkv;
+    p.causal = a.causal;
+    p.scale = a.scale;
+    p.scale_log2 = a.scale * kLog2e;
+    p.lse = a.lse;
+    p.dq = a.dQ;
+    p.dk = a.dK;
+    p.dv = a.dV;
+    p.total_q = a.total_q;
+    p.dq_tok = s[10];
+    p.dq_head = s[11];
+    p.dk_tok = s[12];
+    p.dk_head = s[13];
+    p.dv_tok = s[14];
+    p.dv_head = s[15];
+    p.plan = varlen_plan_at(a.ws, a.B);
+    float* delta = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) +
+                                            (varlen_plan_bytes(a.B) + 15) / 16 * 16);
+    p.delta = delta;
+    if ((rc = varlen_make_plan(p.plan, a.cu_q, a.cu_kv, a.total_q, a.total_kv, a.Hq, a.Hkv, true, st)))
+        return rc;
+    const int64_t rows = (int64_t)a.total_q * a.Hq;
+    if (rows > 0) {
+        const int64_t per_block = 8 * (32 / (D / 8)) * kDeltaLoads;
+        const DeltaStrides ds = {s[6], s[7], s[8], s[9], a.Hq, a.total_q};
+        AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_delta<D, true>,
+                                   dim3((unsigned)std::min<int64_t>((rows + per_block - 1) / per_block,
+                                                                    (int64_t)sm_count() * 8)),
+                                   dim3(256), 0, st, static_cast<const __nv_bfloat16*>(a.O),
+                                   static_cast<const __nv_bfloat16*>(a.dO), delta, rows, ds));
+    }
+    AMPB_CHECK_CUDA(cudaFuncSetAttribute(k_fa_bwd_dkdv<D, true>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, CF::SMEM_KV));
+    AMPB_CHECK_CUDA(cudaFuncSetAttribute(k_fa_bwd_dq<D, true>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, CF::SMEM_Q));
+    // no more CTAs than there can be items
+    if (a.total_kv > 0) {
+        const int64_t most = ((int64_t)a.total_kv / BT + a.B) * a.Hkv;
+        AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_dkdv<D, true>,
+                                   dim3((unsigned)std::min<int64_t>(most, sm_count())),
+                                   dim3(kThreads), CF::SMEM_KV, st, tq, tk, tv, to, p));
+    }
+    if (a.total_q > 0) {
+        const int64_t most = ((int64_t)a.total_q / BT + a.B) * a.Hq;
+        AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_dq<D, true>,
+                                   dim3((unsigned)std::min<int64_t>(most, sm_count())),
+                                   dim3(kThreads), CF::SMEM_Q, st, tq, tk, tv, to, p));
+    }
     return AMP_OK;
 }
 
@@ -937,6 +1299,36 @@ int flash_attn_bwd_dev(const void* Q, const void* K, const void* V, const void* 
 using namespace ampb;
 
 extern "C" {
+
+size_t amp_flash_attn_varlen_bwd_workspace_bytes(int B, int Hq, int total_q) {
+    if (B <= 0 || Hq <= 0 || total_q < 0) return 0;
+    return (varlen_plan_bytes(B) + 15) / 16 * 16 + (size_t)Hq * total_q * 4;
+}
+
+int amp_flash_attn_varlen_bwd_bf16_dev(const void* Q, const void* K, const void* V, const void* O,
+                                       const void* dO, const float* lse, void* dQ, void* dK,
+                                       void* dV, const int32_t* cu_seqlens_q,
+                                       const int32_t* cu_seqlens_kv, int B, int total_q,
+                                       int total_kv, int Hq, int Hkv, int head_dim,
+                                       const int64_t* strides, int causal, float scale,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = varlen_check(B, total_q, total_kv, Hq, Hkv, head_dim, cu_seqlens_q, cu_seqlens_kv,
+                          strides, 16, workspace, workspace_bytes,
+                          amp_flash_attn_varlen_bwd_workspace_bytes(B, Hq, total_q));
+    if (rc) return rc;
+    if (total_q == 0 && total_kv == 0) return AMP_OK;
+    AMPB_REQUIRE((total_q == 0 || (Q && O && dO && lse && dQ)) && (total_kv == 0 || (K && V && dK && dV)),
+                 AMP_ERR_INVALID, "NULL tensor");
+    AMPB_REQUIRE(aligned16(Q) && aligned16(K) && aligned16(V) && aligned16(O) && aligned16(dO) &&
+                     aligned16(dQ) && aligned16(dK) && aligned16(dV),
+                 AMP_ERR_INVALID, "tensors must be 16-byte aligned");
+    if (!(scale > 0.0f)) scale = 1.0f / sqrtf((float)head_dim);
+    const PackedBwdArgs a = {Q,  K,  V,       O,        dO, lse, dQ,     dK,      dV,   cu_seqlens_q,
+                             cu_seqlens_kv, B, total_q, total_kv, Hq, Hkv, causal, strides, scale,
+                             workspace};
+    return head_dim == 128 ? launch_bwd_packed<128>(a, as_stream(stream))
+                           : launch_bwd_packed<64>(a, as_stream(stream));
+}
 
 size_t amp_flash_attn_bwd_workspace_bytes(int B, int Hq, int S_q) {
     return fa_bwd_ws_bytes(B, Hq, S_q);

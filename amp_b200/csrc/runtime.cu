@@ -146,7 +146,7 @@ int device_status(int** out) {
     std::lock_guard<std::mutex> lk(g_status_mu);
     if ((int)g_status.size() <= dev) g_status.resize(dev + 1, nullptr);
     if (!g_status[dev]) {
-        // status word (int 0) + wait limit (u64 at byte 8), see tc_common.cuh
+        // status word (int 0), bad-index word (int 1), wait limit (u64 at byte 8): tc_common.cuh
         struct Block { int status[2]; unsigned long long limit_ns; };
         static_assert(offsetof(Block, limit_ns) == kStatusLimitOffsetInts * sizeof(int), "layout");
         const Block init = {{AMP_DEV_OK, 0}, kWaitTimeoutNs};
@@ -171,13 +171,19 @@ int amp_device_status(int clear) {
     int* p = nullptr;
     int rc = ampb::device_status(&p);
     if (rc) return rc;
-    int v = 0;
+    int words[2] = {0, 0};
     AMPB_CHECK_CUDA(cudaDeviceSynchronize());
-    AMPB_CHECK_CUDA(cudaMemcpy(&v, p, sizeof(int), cudaMemcpyDeviceToHost));
-    if (v && clear) AMPB_CHECK_CUDA(cudaMemset(p, 0, sizeof(int)));
+    AMPB_CHECK_CUDA(cudaMemcpy(words, p, sizeof(words), cudaMemcpyDeviceToHost));
+    const int v = words[0] ? words[0] : words[ampb::kStatusBadIndexInt];
+    if (v && clear) AMPB_CHECK_CUDA(cudaMemset(p, 0, sizeof(words)));
     if (v == 2) {
         ampb::set_error(AMP_ERR_INVALID, "a kernel met a page id outside the KV pool "
                         "(device status 2); the affected pages were skipped");
+        return AMP_ERR_INVALID;
+    }
+    if (v == ampb::AMP_DEV_ERR_BAD_INDEX) {
+        ampb::set_error(AMP_ERR_INVALID, "a kernel met a sequence offset, row or page number outside "
+                        "its tensor (device status 3); what it names was skipped");
         return AMP_ERR_INVALID;
     }
     if (v) {

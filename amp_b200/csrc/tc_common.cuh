@@ -16,14 +16,23 @@
 namespace ampb {
 
 constexpr uint64_t kWaitTimeoutNs = 2000000000ull;  // 2 s, the default wait limit
-enum : int { AMP_DEV_OK = 0, AMP_DEV_ERR_TIMEOUT = 1, AMP_DEV_ERR_BAD_PAGE = 2 };
+enum : int {
+    AMP_DEV_OK = 0,
+    AMP_DEV_ERR_TIMEOUT = 1,
+    AMP_DEV_ERR_BAD_PAGE = 2,
+    AMP_DEV_ERR_BAD_INDEX = 3,
+};
 
 // The per-device status block (runtime.cu) is 16 bytes: the status word at
-// int [0] and the wait limit in ns as a u64 at byte 8.  Kernels receive the
+// int [0], a word for bad indexes at int [1] and the wait limit in ns as a u64 at
+// byte 8.  Bad indexes (sequence offsets, page and row numbers that a kernel
+// skipped) have a word of their own because a nonzero status word also ends the
+// waits of the pipelined kernels, and a skipped index breaks no pipeline.  Kernels receive the
 // status word's address, so the limit needs no argument of its own.  It is
 // read only once a wait has lasted kLimitFloorNs: a global load on every wait
 // would put its latency on the pipelines' hand-offs (it cost the GEMM ~20%),
 // so limits below the floor act as the floor.
+constexpr int kStatusBadIndexInt = 1;
 constexpr int kStatusLimitOffsetInts = 2;
 constexpr uint64_t kLimitFloorNs = 1000000ull;  // 1 ms
 __device__ __forceinline__ uint64_t wait_limit_ns(const int* status) {

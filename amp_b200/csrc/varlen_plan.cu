@@ -1,0 +1,129 @@
+// varlen_plan.cu -- orders the sequences of a packed batch for the attention
+// kernels (varlen.cuh): longest first by a counting sort on the length's leading
+// bits, with the running number of work items before each.
+//
+// One CTA: the work is 16 bytes a sequence, and a grid-wide sort would cost more
+// launches than it saves.  The order within one bucket follows from the
+// scheduling of the atomics; it decides only which CTA computes an item.
+#include <algorithm>
+
+#include "common.cuh"
+#include "runtime.h"
+#include "tc_common.cuh"
+#include "varlen.cuh"
+
+namespace ampb {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kBuckets = 1024;   // == kPlanThreads: one bucket a thread in the scan
+
+// Buckets descend with the length: 5 leading mantissa bits and the exponent of
+// the length as a float (31 octaves * 32 < 1024).
+__device__ __forceinline__ int length_bucket(int len) {
+    if (len <= 0) return kBuckets - 1;
+    const unsigned u = __float_as_uint((float)len) >> 18;
+    return kBuckets - 2 - (int)(u - (0x3f800000u >> 18));
+}
+
+// Inclusive scan over the block's 1024 threads (`part`: 32 ints of shared memory).
+__device__ __forceinline__ int block_scan(int v, int* part) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    __syncthreads();   // `part` may still be read from the call before
+    if (lane == 31) part[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        int w = part[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += t;
+        }
+        part[lane] = w;
+    }
+    __syncthreads();
+    return v + (warp ? part[warp - 1] : 0);
+}
+
+__global__ void __launch_bounds__(kPlanThreads)
+    k_varlen_plan(VarlenPlan pl, const int* __restrict__ cu_q, const int* __restrict__ cu_kv,
+                  int total_q, int total_kv, int Hq, int Hkv, int backward, int* status) {
+    __shared__ int at[kBuckets];
+    __shared__ int part[32];
+    const int tid = threadIdx.x;
+    at[tid] = 0;
+    pdl_wait();
+    pdl_trigger();   // the attention kernel's CTAs set up meanwhile
+    if (tid < 2) pl.next[tid] = 0;
+    __syncthreads();
+    // a sequence whose bounds are not within its tensor, in order, counts as empty
+    auto load = [&](int b) {
+        VarlenSeq s;
+        const int q0 = cu_q[b], q1 = cu_q[b + 1], k0 = cu_kv[b], k1 = cu_kv[b + 1];
+        const bool ok = q0 >= 0 && q1 >= q0 && q1 <= total_q && k0 >= 0 && k1 >= k0 && k1 <= total_kv;
+        s.q_off = ok ? q0 : 0;
+        s.q_len = ok ? q1 - q0 : 0;
+        s.k_off = ok ? k0 : 0;
+        s.k_len = ok ? k1 - k0 : 0;
+        if (!ok) status[kStatusBadIndexInt] = AMP_DEV_ERR_BAD_INDEX;
+        return s;
+    };
+    for (int b = tid; b < pl.B; b += kPlanThreads) {
+        const VarlenSeq s = load(b);
+        atomicAdd(&at[length_bucket(max(s.q_len, s.k_len))], 1);
+    }
+    __syncthreads();
+    const int mine = at[tid];
+    const int end = block_scan(mine, part);
+    at[tid] = end - mine;
+    __syncthreads();
+    for (int b = tid; b < pl.B; b += kPlanThreads) {
+        const VarlenSeq s = load(b);
+        pl.seqs[atomicAdd(&at[length_bucket(max(s.q_len, s.k_len))], 1)] = s;
+    }
+    __syncthreads();
+    const int group = Hq / Hkv;
+    int carry0 = 0, carry1 = 0;
+    for (int r0 = 0; r0 < pl.B; r0 += kPlanThreads) {
+        const int r = r0 + tid;
+        int n0 = 0, n1 = 0;
+        if (r < pl.B) {
+            const VarlenSeq s = pl.seqs[r];
+            n0 = backward ? varlen_tiles(s.k_len) * Hkv : varlen_fwd_pairs(s.q_len, group) * Hkv;
+            n1 = backward ? varlen_tiles(s.q_len) * Hq : 0;
+        }
+        const int e0 = carry0 + block_scan(n0, part);
+        const int last0 = part[31];
+        if (r < pl.B) pl.first[0][r] = e0 - n0;
+        carry0 += last0;
+        if (backward) {
+            const int e1 = carry1 + block_scan(n1, part);
+            const int last1 = part[31];
+            if (r < pl.B) pl.first[1][r] = e1 - n1;
+            carry1 += last1;
+        }
+    }
+    if (tid == 0) {
+        pl.first[0][pl.B] = carry0;
+        pl.first[1][pl.B] = carry1;
+    }
+}
+
+}  // namespace
+
+int varlen_make_plan(const VarlenPlan& plan, const int* cu_q, const int* cu_kv, int total_q,
+                     int total_kv, int Hq, int Hkv, bool backward, cudaStream_t st) {
+    int* status = nullptr;
+    int rc = device_status(&status);
+    if (rc) return rc;
+    AMPB_CHECK_CUDA(launch_pdl(k_varlen_plan, dim3(1), dim3(kPlanThreads), 0, st, plan, cu_q, cu_kv,
+                               total_q, total_kv, Hq, Hkv, backward ? 1 : 0, status));
+    return AMP_OK;
+}
+
+}  // namespace ampb

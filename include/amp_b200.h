@@ -267,6 +267,45 @@ AMP_API int amp_flash_attn_bwd_bf16_dev(const void* Q, const void* K, const void
                                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * FlashAttention-2 over packed sequences of different lengths, forward and
+ * backward (AMP has rectangular batches only, kernels/flash_attn.cuh:50-58).
+ * Q, O [total_q, Hq, head_dim], K, V [total_kv, Hkv, head_dim] bf16: sequence
+ * b's queries are rows cu_seqlens_q[b] .. cu_seqlens_q[b+1]-1, its keys rows
+ * cu_seqlens_kv[b] .. cu_seqlens_kv[b+1]-1 (device int32 [B+1]; pass one array
+ * twice for self-attention).  Lengths may differ and may be 0.  causal != 0:
+ * query i sees key j iff j <= i + (keys - queries), i.e. aligned at the end, as
+ * paged prefill; a query that sees no key gets O = 0, lse = -inf and zero
+ * gradients.  lse [Hq, total_q] fp32 (natural log; may be NULL forward).
+ * strides: HOST array of the token and the head stride, in elements, of
+ * Q, K, V, O (forward) and of Q, K, V, O, dO, dQ, dK, dV (backward); each a
+ * positive multiple of 8, the head dimension contiguous.  scale <= 0 selects
+ * 1/sqrt(head_dim).  head_dim 64 or 128.
+ * Rows outside every sequence are neither read into a result (they may hold
+ * anything, NaN included) nor written.  K and V rows inside a sequence must be
+ * finite, also where the mask hides them from some of its queries.  A sequence whose offsets
+ * are out of order or outside the tensors is skipped and reported by
+ * amp_device_status (AMP_ERR_INVALID).
+ * The workspace must not be shared by calls that may overlap. */
+AMP_API size_t amp_flash_attn_varlen_workspace_bytes(int B);
+AMP_API int amp_flash_attn_varlen_fwd_bf16_dev(const void* Q, const void* K, const void* V,
+                                               void* O, float* lse, const int32_t* cu_seqlens_q,
+                                               const int32_t* cu_seqlens_kv, int B, int total_q,
+                                               int total_kv, int Hq, int Hkv, int head_dim,
+                                               const int64_t* strides, int causal, float scale,
+                                               void* workspace, size_t workspace_bytes,
+                                               void* stream);
+AMP_API size_t amp_flash_attn_varlen_bwd_workspace_bytes(int B, int Hq, int total_q);
+AMP_API int amp_flash_attn_varlen_bwd_bf16_dev(const void* Q, const void* K, const void* V,
+                                               const void* O, const void* dO, const float* lse,
+                                               void* dQ, void* dK, void* dV,
+                                               const int32_t* cu_seqlens_q,
+                                               const int32_t* cu_seqlens_kv, int B, int total_q,
+                                               int total_kv, int Hq, int Hkv, int head_dim,
+                                               const int64_t* strides, int causal, float scale,
+                                               void* workspace, size_t workspace_bytes,
+                                               void* stream);
+
+/* ------------------------------------------------------------------------
  * Attention over a paged KV cache (block tables of 16-token pages, the
  * format of Sequence::kv_page_ids / kv_page_size_tokens in the reference's
  * include/scheduler.hpp:61,88; the reference has no kernel that reads it).

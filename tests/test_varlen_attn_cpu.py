@@ -1,0 +1,73 @@
+"""Refusals of the packed-sequence attention: argument errors return before any CUDA work."""
+import ctypes as C
+
+import pytest
+import torch
+
+from amp_b200 import attention
+from amp_b200._lib import AmpError, call
+
+FWD, BWD = "amp_flash_attn_varlen_fwd_bf16_dev", "amp_flash_attn_varlen_bwd_bf16_dev"
+P = 1 << 20   # an aligned address that is never read: every call below is refused
+
+
+def fwd(q=P, k=P, v=P, o=P, lse=P, cu=P, cu_kv=P, B=2, tq=10, tk=10, Hq=4, Hkv=2, D=64,
+        strides=(256, 64, 128, 64, 128, 64, 256, 64), ws=P, ws_bytes=1 << 20):
+    call(FWD, q, k, v, o, lse, cu, cu_kv, B, tq, tk, Hq, Hkv, D,
+         (C.c_int64 * 8)(*strides) if strides else None, 1, 0.0, ws, ws_bytes, None)
+
+
+def bwd(q=P, k=P, v=P, o=P, do=P, lse=P, dq=P, dk=P, dv=P, cu=P, cu_kv=P, B=2, tq=10, tk=10, Hq=4,
+        Hkv=2, D=64, strides=(256, 64) * 8, ws=P, ws_bytes=1 << 20):
+    call(BWD, q, k, v, o, do, lse, dq, dk, dv, cu, cu_kv, B, tq, tk, Hq, Hkv, D,
+         (C.c_int64 * 16)(*strides) if strides else None, 1, 0.0, ws, ws_bytes, None)
+
+
+BAD = [(dict(B=0), -1), (dict(Hq=0), -1), (dict(Hkv=0), -1), (dict(Hq=5), -1), (dict(tq=-1), -1),
+       (dict(tk=-1), -1), (dict(D=80), -2), (dict(D=256), -2), (dict(cu=None), -1),
+       (dict(cu_kv=None), -1), (dict(strides=None), -1), (dict(ws=None), -1), (dict(ws=P + 8), -1),
+       (dict(ws_bytes=16), -1), (dict(q=None), -1), (dict(k=None), -1), (dict(q=P + 2), -1),
+       (dict(v=P + 8), -1), (dict(tq=1 << 30, Hq=4), -2), (dict(B=1 << 30), -2)]
+
+
+@pytest.mark.parametrize("kw,code", BAD, ids=[str(b[0]) for b in BAD])
+@pytest.mark.parametrize("entry", [fwd, bwd])
+def test_refused_arguments(entry, kw, code, amp_lib):
+    if "tq" in kw or "B" in kw:
+        kw = dict(kw, ws_bytes=1 << 62)
+    with pytest.raises(AmpError) as e:
+        entry(**kw)
+    assert e.value.code == code
+
+
+@pytest.mark.parametrize("stride", [0, -64, 4, 65, 1 << 40])
+@pytest.mark.parametrize("entry,n", [(fwd, 8), (bwd, 16)])
+def test_refused_strides(entry, n, stride, amp_lib):
+    for i in range(n):
+        s = [256, 64] * (n // 2)
+        s[i] = stride
+        with pytest.raises(AmpError) as e:
+            entry(strides=s)
+        assert e.value.code == -1
+
+
+def test_no_tokens_is_no_work(amp_lib):
+    fwd(tq=0, q=None, o=None)
+    bwd(tq=0, tk=0, q=None, k=None)
+
+
+def test_workspace_sizes(amp_lib):
+    assert amp_lib.amp_flash_attn_varlen_workspace_bytes(0) == 0
+    small, large = (amp_lib.amp_flash_attn_varlen_workspace_bytes(b) for b in (1, 1000))
+    assert 0 < small < large
+    assert amp_lib.amp_flash_attn_varlen_bwd_workspace_bytes(1, 8, 100) >= small + 8 * 100 * 4
+    assert amp_lib.amp_flash_attn_varlen_bwd_workspace_bytes(1, 8, -1) == 0
+
+
+def test_python_refuses_what_the_kernels_cannot_read(amp_lib):
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(ValueError):
+        attention.flash_attn_varlen_fwd(q, q, q, cu)          # not on a GPU
+    with pytest.raises(ValueError):
+        attention.flash_attn_varlen_fwd(q[0], q, q, cu)       # not packed

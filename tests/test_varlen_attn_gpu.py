@@ -1,0 +1,300 @@
+"""Packed-sequence attention (forward and backward) on the B200 vs fp64, element by element.
+
+The bounds count roundings (u = 2^-8, half a bf16 step relative to the value):
+  O     rounded once, from P rounded once:          u |O| + u P|V|
+  lse   fp32 sums of D products:                    D 2^-23 max scale |q|.|k| + a few 2^-22
+  dV    rounded once, from P rounded once:          u |dV| + u P^T|dO|
+  dS    P and dS rounded, Delta from the bf16 O:    2u |dS| + P dDelta,
+        dDelta = sum |dO| (u |O| + u P|V|)
+  dQ    u |dQ| + scale |err dS| |K|;  dK  u |dK| + scale |err dS|^T |Q|
+each with 5% for products of roundings and 1e-5 for the fp32 sums.  The scores' fp32 error
+enters P through exp: it is the lse bound, and is added to u wherever P is.
+"""
+import numpy as np
+import pytest
+import torch
+
+from amp_b200 import attention
+from amp_b200._lib import lib
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -8
+
+
+def make(lens_q, lens_kv, Hq, Hkv, D, seed=0, pad_q=0, pad_kv=0):
+    g = torch.Generator().manual_seed(seed)
+    tq, tk = sum(lens_q) + pad_q, sum(lens_kv) + pad_kv
+    q, do = (torch.randn(tq, Hq, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    k, v = (torch.randn(tk, Hkv, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    cu = [torch.tensor(np.concatenate([[0], np.cumsum(x)]), dtype=torch.int32) for x in (lens_q, lens_kv)]
+    return q, k, v, do, *cu
+
+
+def reference(q, k, v, do, lens_q, lens_kv, causal, scale=0.0):
+    """fp64 results and bounds: {name: (value, bound)} for o, lse, dq, dk, dv."""
+    q, k, v, do = (x.double().numpy() for x in (q, k, v, do))
+    Hq, Hkv, D = q.shape[1], k.shape[1], q.shape[2]
+    G, sc = Hq // Hkv, scale if scale > 0 else 1 / np.sqrt(D)
+    val = {n: np.zeros(x.shape) for n, x in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+    err = {n: np.zeros(x.shape) for n, x in val.items()}
+    val["lse"], err["lse"] = np.full((Hq, q.shape[0]), -np.inf), np.zeros((Hq, q.shape[0]))
+    a = b = 0
+    for lq, lk in zip(lens_q, lens_kv):
+        Q, K = slice(a, a + lq), slice(b, b + lk)
+        a, b = a + lq, b + lk
+        if lq == 0 or lk == 0:
+            continue
+        seen = np.tril(np.ones((lq, lk), bool), lk - lq) if causal else np.ones((lq, lk), bool)
+        for h in range(Hq):
+            qh, kh, vh, doh = q[Q, h], k[K, h // G], v[K, h // G], do[Q, h]
+            s = np.where(seen, sc * (qh @ kh.T), -np.inf)
+            e_s = D * 2.0 ** -23 * sc * (np.abs(qh) @ np.abs(kh).T).max() + 4 * 2.0 ** -22
+            m = s.max(1, keepdims=True)
+            m = np.where(np.isfinite(m), m, 0)
+            p = np.exp(s - m)
+            l = p.sum(1, keepdims=True)
+            with np.errstate(divide="ignore"):
+                val["lse"][h, Q] = (m + np.log(l))[:, 0]
+            p = p / np.where(l > 0, l, 1)
+            err["lse"][h, Q] = e_s + np.where(l[:, 0] > 0, np.abs(m[:, 0]) * 2.0 ** -22, 0)
+            u = U + 2 * e_s
+            o, o_abs = p @ vh, p @ np.abs(vh)
+            val["o"][Q, h] = o
+            e_o = err["o"][Q, h] = U * np.abs(o) + u * o_abs
+            val["dv"][K, h // G] += p.T @ doh
+            err["dv"][K, h // G] += u * (p.T @ np.abs(doh))
+            dp = doh @ vh.T
+            ds = p * (dp - (doh * o).sum(1, keepdims=True))
+            e_ds = (u + U) * np.abs(ds) + p * ((np.abs(doh) * e_o).sum(1, keepdims=True)
+                                               + D * 2.0 ** -23 * (np.abs(doh) @ np.abs(vh).T))
+            val["dq"][Q, h] = sc * (ds @ kh)
+            err["dq"][Q, h] = sc * (e_ds @ np.abs(kh))
+            val["dk"][K, h // G] += sc * (ds.T @ qh)
+            err["dk"][K, h // G] += sc * (e_ds.T @ np.abs(qh))
+    for n in ("dq", "dk", "dv"):
+        err[n] += U * np.abs(val[n])
+    return {n: (val[n], 1.05 * err[n] + 1e-5) for n in val}
+
+
+def check(got, ref, names):
+    for n in names:
+        x, (want, bound) = got[n].double().cpu().numpy(), ref[n]
+        x = x[:want.shape[0]] if n != "lse" else x[:, :want.shape[1]]
+        fin = np.isfinite(want)
+        assert np.array_equal(np.isfinite(x), fin), n
+        assert np.array_equal(x[~fin], want[~fin]), n
+        over = np.abs(x - want)[fin] / bound[fin]
+        assert over.size == 0 or over.max() <= 1, (n, float(over.max()))
+
+
+def run(q, k, v, do, cu_q, cu_kv, causal, **kw):
+    q, k, v, do, cu_q, cu_kv = (x.cuda() for x in (q, k, v, do, cu_q, cu_kv))
+    o, lse = attention.flash_attn_varlen_fwd(q, k, v, cu_q, cu_kv, causal=causal, **kw)
+    dq, dk, dv = attention.flash_attn_varlen_bwd(q, k, v, o, do, lse, cu_q, cu_kv, causal=causal, **kw)
+    torch.cuda.synchronize()
+    assert lib().amp_device_status(1) == 0
+    return {"o": o, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+
+
+ALL = ("o", "lse", "dq", "dk", "dv")
+SAME = [[1], [128], [129], [17, 0, 1, 127, 300], [256, 5, 0, 0, 640]]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 4, 128), (8, 2, 128), (6, 2, 64), (5, 1, 128), (8, 1, 64)])
+@pytest.mark.parametrize("lens", SAME, ids=str)
+def test_self_attention_lengths(lens, Hq, Hkv, D, causal, cuda, amp_lib):
+    q, k, v, do, cu, _ = make(lens, lens, Hq, Hkv, D, seed=len(lens) + Hq)
+    check(run(q, k, v, do, cu, cu, causal), reference(q, k, v, do, lens, lens, causal), ALL)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 2, 128), (3, 3, 64)])
+@pytest.mark.parametrize("pairs", [
+    [(5, 300), (300, 5), (0, 10), (10, 0), (130, 131)],   # rows and whole sequences that see nothing
+    [(1, 1000), (1, 1), (0, 0), (200, 129)],
+    [(3, 0), (130, 0)],                                   # no key anywhere
+], ids=str)
+def test_query_and_key_lengths_differ(pairs, Hq, Hkv, D, causal, cuda, amp_lib):
+    lq, lk = zip(*pairs)
+    q, k, v, do, cu_q, cu_kv = make(lq, lk, Hq, Hkv, D, seed=7)
+    check(run(q, k, v, do, cu_q, cu_kv, causal), reference(q, k, v, do, lq, lk, causal), ALL)
+
+
+def test_keys_without_any_query_get_zero_gradients(cuda, amp_lib):
+    q, k, v, do, cu_q, cu_kv = make([0, 0], [5, 140], 4, 2, 128)
+    got = run(q, k, v, do, cu_q, cu_kv, True)
+    assert got["o"].shape[0] == 0 and not got["dk"].any() and not got["dv"].any()
+
+
+@pytest.mark.parametrize("scale", [0.02, 0.5])
+def test_scale(scale, cuda, amp_lib):
+    lens = [100, 200]
+    q, k, v, do, cu, _ = make(lens, lens, 4, 2, 64, seed=3)
+    check(run(q, k, v, do, cu, cu, True, scale=scale),
+          reference(q, k, v, do, lens, lens, True, scale), ALL)
+
+
+def test_more_sequences_than_the_plan_has_threads(cuda, amp_lib):
+    lens = [int(n) for n in np.random.default_rng(5).integers(0, 4, 2100)]
+    q, k, v, do, cu, _ = make(lens, lens, 2, 1, 64, seed=5)
+    check(run(q, k, v, do, cu, cu, True), reference(q, k, v, do, lens, lens, True), ALL)
+
+
+def test_parts_of_a_fused_projection_and_strided_gradients(cuda, amp_lib):
+    lens, Hq, Hkv, D = [70, 200, 1], 8, 2, 128
+    q, k, v, do, cu, _ = make(lens, lens, Hq, Hkv, D, seed=9)
+    ref = reference(q, k, v, do, lens, lens, True)
+    qkv = torch.cat([q, k, v], 1).cuda()
+    parts = qkv.split([Hq, Hkv, Hkv], 1)
+    o = torch.full((Hq, 271, D), 7.0, dtype=torch.bfloat16, device="cuda").transpose(0, 1)   # head major
+    grad = torch.full_like(qkv, 7.0)
+    dq, dk, dv = grad.split([Hq, Hkv, Hkv], 1)
+    _, lse = attention.flash_attn_varlen_fwd(*parts, cu.cuda(), out=o)
+    attention.flash_attn_varlen_bwd(*parts, o, do.cuda(), lse, cu.cuda(), dq=dq, dk=dk, dv=dv)
+    check({"o": o, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, ref, ALL)
+
+
+def test_rows_of_no_sequence_are_not_read_nor_written(cuda, amp_lib):
+    lens, Hq, Hkv, D = [60, 130], 4, 2, 128
+    for bad in (float("nan"), float("inf")):
+        q, k, v, do, cu, _ = make(lens, lens, Hq, Hkv, D, seed=11, pad_q=100, pad_kv=100)
+        n = sum(lens)
+        ref = reference(q[:n], k[:n], v[:n], do[:n], lens, lens, True)
+        for x in (q, k, v, do):
+            x[n:] = bad
+        qc, kc, vc, doc, cuc = (x.cuda() for x in (q, k, v, do, cu))
+        o, dq = (torch.full_like(qc, 7.0) for _ in range(2))
+        dk, dv = (torch.full_like(kc, 7.0) for _ in range(2))
+        lse = torch.full((Hq, n + 100), 7.0, device="cuda")
+        attention.flash_attn_varlen_fwd(qc, kc, vc, cuc, out=o, lse=lse)
+        attention.flash_attn_varlen_bwd(qc, kc, vc, o, doc, lse, cuc, dq=dq, dk=dk, dv=dv)
+        for x in (o, dq, dk, dv):
+            assert (x[n:] == 7.0).all()
+        assert (lse[:, n:] == 7.0).all()
+        check({"o": o, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, ref, ALL)
+
+
+def test_a_sequence_of_nan_leaves_its_neighbours_alone(cuda, amp_lib):
+    lens, Hq, Hkv, D = [60, 33, 200, 7], 4, 2, 64
+    q, k, v, do, cu, _ = make(lens, lens, Hq, Hkv, D, seed=13)
+    clean = run(q, k, v, do, cu, cu, True)
+    bad = slice(60, 93)
+    for x in (q, k, v, do):
+        x[bad] = float("nan")
+    got = run(q, k, v, do, cu, cu, True)
+    keep = torch.ones(300, dtype=torch.bool)
+    keep[bad] = False
+    for n in ("o", "dq", "dk", "dv"):
+        assert torch.equal(got[n][keep], clean[n][keep]), n
+    assert torch.equal(got["lse"][:, keep], clean["lse"][:, keep])
+
+
+def test_gradients_agree_with_differences(cuda, amp_lib):
+    """d/de of sum(dO * O(x + e w)) at e = 0 equals sum(grad * w), in fp64 on the oracle's
+    formula for the loss and the kernel's gradients: the bf16 gradients are off by at most
+    their bound, weighted with |w|."""
+    lens = [33, 150]
+    q, k, v, do, cu, _ = make(lens, lens, 4, 2, 64, seed=17)
+    got = run(q, k, v, do, cu, cu, True)
+    ref = reference(q, k, v, do, lens, lens, True)
+    g = torch.Generator().manual_seed(1)
+
+    def loss(x):
+        return (do.double().numpy() * reference(*x, do, lens, lens, True)["o"][0]).sum()
+
+    for i, n in enumerate(("dq", "dk", "dv")):
+        w = torch.randn(ref[n][0].shape, generator=g, dtype=torch.float64)
+        e, x = 1e-4, [t.double() for t in (q, k, v)]
+        ahead, back = list(x), list(x)
+        ahead[i], back[i] = x[i] + e * w, x[i] - e * w
+        slope = (loss(ahead) - loss(back)) / (2 * e)
+        mine = (got[n].double().cpu() * w).sum().item()
+        assert abs(mine - slope) <= (ref[n][1] * w.abs().numpy()).sum() + 1e-6 * abs(slope)
+
+
+def test_matches_the_rectangular_kernels(cuda, amp_lib):
+    B, S, Hq, Hkv, D = 3, 384, 8, 2, 128
+    q, k, v, do, cu, _ = make([S] * B, [S] * B, Hq, Hkv, D, seed=19)
+    got = run(q, k, v, do, cu, cu, True)
+    dense = [x.cuda().view(B, S, -1, D).transpose(1, 2).contiguous() for x in (q, k, v, do)]
+    o, lse = attention.flash_attn_fwd(*dense[:3], True)
+    assert torch.equal(got["lse"], lse.transpose(0, 1).reshape(Hq, B * S))
+    assert torch.equal(got["o"].view(B, S, Hq, D).transpose(1, 2), o)
+    grads = attention.flash_attn_bwd(*dense[:3], o, dense[3], lse, True)
+    for n, x in zip(("dq", "dk", "dv"), grads):
+        assert torch.equal(got[n].view(B, S, -1, D).transpose(1, 2), x), n
+
+
+def test_same_bits_again_on_another_stream_and_from_a_graph(cuda, amp_lib):
+    lens = [300, 5, 0, 129, 700]
+    q, k, v, do, cu, _ = (x.cuda() for x in make(lens, lens, 8, 2, 128, seed=23))
+    do = do.contiguous()
+
+    def step():
+        o, lse = attention.flash_attn_varlen_fwd(q, k, v, cu)
+        return (o, lse, *attention.flash_attn_varlen_bwd(q, k, v, o, do, lse, cu))
+
+    first = step()
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        second = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        third = step()
+    for x in third:
+        x.fill_(7.0)
+    # the graph reads the lengths when it runs: other lengths, then the first ones again
+    cu2 = cu.clone()
+    cu.copy_(torch.tensor([0, 10, 10, 500, 600, 1134], dtype=torch.int32))
+    graph.replay()
+    expect = step()
+    for a, b in zip(third, expect):
+        assert torch.equal(a, b)
+    cu.copy_(cu2)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b, c in zip(first, second, third):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    assert lib().amp_device_status(1) == 0
+
+
+def test_two_calls_at_once_on_two_streams(cuda, amp_lib):
+    jobs = []
+    for i in range(2):
+        lens = [500, 20, 900] if i else [40, 1200]
+        jobs.append([x.cuda() for x in make(lens, lens, 8, 4, 128, seed=29 + i)])
+    alone = [attention.flash_attn_varlen_fwd(q, k, v, cu) for q, k, v, _, cu, _ in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    out = [[] for _ in jobs]
+    for _ in range(5):
+        for i, (q, k, v, _, cu, _) in enumerate(jobs):
+            with torch.cuda.stream(streams[i]):
+                out[i].append(attention.flash_attn_varlen_fwd(q, k, v, cu))
+    torch.cuda.synchronize()
+    for a, many in zip(alone, out):
+        for b in many:
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("offsets", [[0, 50, 40, 100], [0, -3, 100, 100], [0, 50, 100, 101]], ids=str)
+def test_offsets_outside_the_tensors_are_skipped_and_reported(offsets, cuda, amp_lib):
+    q, k, v, do, _, _ = make([100], [100], 2, 2, 64, seed=31)
+    qc, kc, vc = (x.cuda() for x in (q, k, v))
+    cu = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    out = torch.full_like(qc, 7.0)
+    attention.flash_attn_varlen_fwd(qc, kc, vc, cu, out=out)
+    torch.cuda.synchronize()
+    assert lib().amp_device_status(1) == -1 and lib().amp_device_status(1) == 0
+    good = [(a, b) for a, b in zip(offsets, offsets[1:]) if 0 <= a <= b <= 100]
+    first = good[0]
+    if first == (0, 50):
+        n = [50]
+        # rows that a later sequence names again are that sequence's
+        rows = slice(0, 40)
+        ref = reference(q[:50], k[:50], v[:50], do[:50], n, n, True)["o"]
+        x = out[rows].double().cpu().numpy()
+        assert (np.abs(x - ref[0][rows]) <= ref[1][rows]).all()
