@@ -65,6 +65,11 @@ SIGNATURES: dict[str, tuple] = {
                                               _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
     "amp_paged_attn_prefill_bf16_dev": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32,
                                                _i32, _i32, _i32, _i32, _i32, _f32, _vp]),
+    "amp_rope_dev": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _i32,
+                            _vp, _vp, _i32, _i32, _vp]),
+    "amp_paged_rope_append_bf16_dev": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp,
+                                              _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp,
+                                              _i32, _i32, _i32, _vp]),
     "amp_paged_validate_block_table": (_i32, [_vp, _vp, _i32, _i32, _i32]),
     "amp_paged_pack_block_table": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp]),
     "amp_paged_pool_bytes": (_sz, [_i32, _i32, _i32]),

@@ -1,0 +1,356 @@
+// rope.cu -- rotary positions with one or more axes, and their fusion with the
+// paged cache's append.
+//
+// Pair i of a head's first R = 2 * pairs elements is turned by
+//   phi = pos[axis(i)][token] * inv_freq[i]:   (x, y) -> (x cos - y sin, y cos + x sin)
+// (the backward pass by -phi).  Pairs are (i, i + R/2), or (2i, 2i + 1) when
+// interleaved; elements from R on pass through.  axis(i) comes from the sections:
+// the first sections[0] pairs follow axis 0 (time), the next sections[1] axis 1
+// (height), and so on.  The reference has no positional encoding.
+//
+// HBM-bound: every element is read and written once.  A unit of work is two
+// vectors of VE elements that hold VE pairs (or 2 VE elements that pass through);
+// a block takes 256 * U consecutive units in (token, head, unit) order, so loads
+// and stores of a warp cover whole rows.  The angles of the block's tokens are
+// computed once into shared memory, after the block's loads have been issued:
+// they are shared by all heads, and their arithmetic hides behind the loads.
+//
+// The angle is reduced in 64 bits (turns = pos * inv_freq / 2 pi, less the nearest
+// whole number): in 32 bits a position of 10^5 is off by 2^-7 of a radian.  The
+// rotation itself is fp32, rounded once to the tensor's type.
+//
+// Append mode writes k (turned) and v of each new token into its page of the
+// cache instead of an output tensor.  Token t belongs to the sequence b with
+// cu[b] <= t < cu[b+1] and is number ctx[b] - len(b) + (t - cu[b]) of its context
+// (ctx counts the new tokens, as paged prefill expects).  One warp per token
+// searches cu while the rows are being loaded.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "runtime.h"
+#include "tc_common.cuh"
+#include "varlen.cuh"
+
+namespace ampb {
+namespace {
+
+constexpr int kRopeThreads = 256;
+constexpr int kMaxAxes = 4;
+constexpr int kPage = 16;
+
+struct RopeTensor {
+    const void* in;
+    void* out;
+    int64_t in_tok, in_head, out_tok, out_head;   // strides in elements
+};
+
+struct RopeParams {
+    RopeTensor x[3];       // q, k, v (append: k and v have no `out`)
+    int heads[3];
+    int T, H, D;           // H: heads of all tensors
+    int pairs;             // R / 2
+    int units;             // per head: (R + passed) / (2 VE)
+    float sign;            // -1: backward
+    const int* pos;        // [axes][T]
+    int64_t pos_stride;
+    int axis_end[kMaxAxes - 1];   // first pair of axes 1, 2, 3
+    const float* inv_freq;
+    // append
+    void *k_pool, *v_pool;        // [pages][heads][16][D]
+    const int *block_table, *ctx_lens, *cu;
+    int B, num_pages, max_pages;
+    int* status;
+};
+
+template <typename T, int VE>
+struct alignas(sizeof(T) * VE) Vec {
+    T v[VE];
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x) {
+    if constexpr (std::is_same<T, float>::value) return x;
+    else return __float2bfloat16_rn(x);
+}
+
+__device__ __forceinline__ float2 angle(const RopeParams& p, int t, int i) {
+    int axis = 0;
+#pragma unroll
+    for (int a = 0; a < kMaxAxes - 1; ++a) axis += i >= p.axis_end[a];
+    const double turns = (double)p.pos[axis * p.pos_stride + t] * (double)p.inv_freq[i] *
+                         0.15915494309189533577;   // 1 / (2 pi)
+    float s, c;
+    sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+    return make_float2(c, s * p.sign);
+}
+
+constexpr int64_t kNoSequence = -1, kNoPage = -2;
+
+// Append: where token t's row of head 0 starts in the pools, in elements, or one of the
+// two above.  All lanes of a warp call it.
+__device__ __forceinline__ int64_t cache_row(const RopeParams& p, int t, int Hkv) {
+    const int b = varlen_find(p.cu, p.B, t);
+    const int q0 = p.cu[b], q1 = p.cu[b + 1];
+    if (t < q0 || t >= q1) return kNoSequence;
+    const int64_t at = (int64_t)p.ctx_lens[b] - (q1 - q0) + (t - q0);
+    int page = -1;
+    if (at >= 0 && at / kPage < p.max_pages)
+        page = p.block_table[(int64_t)b * p.max_pages + at / kPage];
+    if (page < 0 || page >= p.num_pages) {
+        if ((threadIdx.x & 31) == 0) p.status[kStatusBadIndexInt] = AMP_DEV_ERR_BAD_INDEX;
+        return kNoPage;
+    }
+    return ((int64_t)page * Hkv * kPage + at % kPage) * p.D;
+}
+
+template <typename T, int VE, bool kInter, bool kAppend, int U>
+__global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ RopeParams p) {
+    // cos, sin [tokens of this block][VE][pairs / VE]: a warp's lanes read neighbours
+    extern __shared__ float2 trig[];
+    using V = Vec<T, VE>;
+    pdl_wait();
+    const int per_token = p.H * p.units;
+    const int64_t total = (int64_t)p.T * per_token;
+    const int64_t u0 = (int64_t)blockIdx.x * (kRopeThreads * U);
+    const int64_t u1 = min(u0 + kRopeThreads * U, total);
+    const int t0 = (int)(u0 / per_token);
+    const int ntok = (int)((u1 - 1) / per_token) - t0 + 1;
+    const int first = (int)(u0 - (int64_t)t0 * per_token);   // u0 within token t0
+    int64_t* rows = reinterpret_cast<int64_t*>(trig + (size_t)ntok * p.pairs);   // append
+
+    V a[U], b[U];
+    int tok[U], off_a[U], off_b[U], hd[U], which[U], pair0[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int w = first + i * kRopeThreads + threadIdx.x;
+        which[i] = -1;
+        if (u0 + i * kRopeThreads + threadIdx.x >= u1) continue;
+        tok[i] = w / per_token;
+        const int r = w - tok[i] * per_token;
+        int h = r / p.units;
+        const int c = r - h * p.units;
+        int x = 0;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (x == k && h >= p.heads[k]) {
+                h -= p.heads[k];
+                x = k + 1;
+            }
+        which[i] = x;
+        hd[i] = h;
+        pair0[i] = c * VE;
+        const bool turned = c * VE < p.pairs;
+        off_a[i] = turned && !kInter ? c * VE : c * 2 * VE;
+        off_b[i] = turned && !kInter ? p.pairs + c * VE : c * 2 * VE + VE;
+        const T* src = static_cast<const T*>(p.x[x].in) + (t0 + tok[i]) * p.x[x].in_tok + h * p.x[x].in_head;
+        a[i] = *reinterpret_cast<const V*>(src + off_a[i]);
+        b[i] = *reinterpret_cast<const V*>(src + off_b[i]);
+    }
+    const int chunks = p.pairs / VE;
+    for (int i = threadIdx.x; i < ntok * p.pairs; i += kRopeThreads) {
+        const int t = i / p.pairs, pair = i - t * p.pairs;
+        trig[t * p.pairs + pair % VE * chunks + pair / VE] = angle(p, t0 + t, pair);
+    }
+    if constexpr (kAppend) {
+        for (int t = threadIdx.x >> 5; t < ntok; t += kRopeThreads / 32) {
+            const int64_t row = cache_row(p, t0 + t, p.heads[1]);
+            if ((threadIdx.x & 31) == 0) rows[t] = row;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        if (which[i] < 0) continue;
+        if (pair0[i] < p.pairs && !(kAppend && which[i] == 2)) {
+            const float2* cs = trig + tok[i] * p.pairs + pair0[i] / VE;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                // pair e: elements e of both vectors, or neighbours within the two
+                T& x = kInter ? (2 * e < VE ? a[i].v[(2 * e) % VE] : b[i].v[(2 * e) % VE]) : a[i].v[e];
+                T& y = kInter ? (2 * e + 1 < VE ? a[i].v[(2 * e + 1) % VE] : b[i].v[(2 * e + 1) % VE])
+                              : b[i].v[e];
+                const float fx = to_f32(x), fy = to_f32(y);
+                const float2 w = cs[e * chunks];
+                x = from_f32<T>(fx * w.x - fy * w.y);
+                y = from_f32<T>(fy * w.x + fx * w.y);
+            }
+        }
+        const int x = which[i];
+        T* dst;
+        if constexpr (kAppend) {
+            const int64_t row = rows[tok[i]];
+            if (row == kNoSequence || (row == kNoPage && x > 0)) continue;
+            if (x > 0)
+                dst = static_cast<T*>(x == 1 ? p.k_pool : p.v_pool) + row + (int64_t)hd[i] * kPage * p.D;
+            else
+                dst = static_cast<T*>(p.x[0].out) + (t0 + tok[i]) * p.x[0].out_tok + hd[i] * p.x[0].out_head;
+        } else {
+            dst = static_cast<T*>(p.x[x].out) + (t0 + tok[i]) * p.x[x].out_tok + hd[i] * p.x[x].out_head;
+        }
+        *reinterpret_cast<V*>(dst + off_a[i]) = a[i];
+        *reinterpret_cast<V*>(dst + off_b[i]) = b[i];
+    }
+}
+
+template <typename T, int VE, bool kInter, bool kAppend>
+int launch_rope_as(RopeParams& p, cudaStream_t st) {
+    p.units = p.D / (2 * VE);
+    const int64_t total = (int64_t)p.T * p.H * p.units;
+    // Four units a thread keep eight 16-byte loads in flight; with fewer blocks than two a
+    // multiprocessor (a decode step) one unit a thread spreads the latency instead, and with
+    // under four heads four units would mean more tokens' angles than shared memory should hold.
+    const bool wide = p.H >= 4 && total >= (int64_t)sm_count() * 2 * kRopeThreads * 4;
+    const int per_block = kRopeThreads * (wide ? 4 : 1);
+    const int64_t per_token = (int64_t)p.H * p.units;
+    const int64_t tokens = (per_block + per_token - 2) / per_token + 1;
+    const size_t smem = (size_t)tokens * p.pairs * sizeof(float2) + (kAppend ? tokens * 8 : 0);
+    const int64_t blocks = (total + per_block - 1) / per_block;
+    AMPB_REQUIRE(blocks <= INT32_MAX && per_token <= (1 << 24), AMP_ERR_UNSUPPORTED, "rope: too large");
+    auto kern = wide ? k_rope<T, VE, kInter, kAppend, 4> : k_rope<T, VE, kInter, kAppend, 1>;
+    AMPB_CHECK_CUDA(launch_pdl(kern, dim3((unsigned)blocks), dim3(kRopeThreads), smem, st, p));
+    return AMP_OK;
+}
+
+// The widest vector that divides the pairs, the rest of the head, every stride and every
+// address: 16 bytes for the usual head sizes, one element for the odd ones.
+template <typename T, bool kAppend>
+int launch_rope(RopeParams& p, bool interleaved, cudaStream_t st) {
+    auto fits = [&](int ve) {
+        bool ok = p.pairs % ve == 0 && (p.D - 2 * p.pairs) % (2 * ve) == 0;
+        const size_t bytes = ve * sizeof(T);
+        auto address = [&](const void* q) { return reinterpret_cast<uintptr_t>(q) % bytes == 0; };
+        for (int i = 0; i < 3; ++i)
+            if (p.heads[i] > 0)
+                ok = ok && address(p.x[i].in) && address(p.x[i].out) && p.x[i].in_tok % ve == 0 &&
+                     p.x[i].in_head % ve == 0 && p.x[i].out_tok % ve == 0 && p.x[i].out_head % ve == 0;
+        return ok && address(p.k_pool) && address(p.v_pool);
+    };
+    constexpr int kWide = 16 / sizeof(T);
+    if (fits(kWide))
+        return interleaved ? launch_rope_as<T, kWide, true, kAppend>(p, st)
+                           : launch_rope_as<T, kWide, false, kAppend>(p, st);
+    if (kWide > 4 && fits(4))
+        return interleaved ? launch_rope_as<T, 4, true, kAppend>(p, st)
+                           : launch_rope_as<T, 4, false, kAppend>(p, st);
+    return interleaved ? launch_rope_as<T, 1, true, kAppend>(p, st)
+                       : launch_rope_as<T, 1, false, kAppend>(p, st);
+}
+
+// Positions, sections and frequencies into p; `heads` and D are set.
+int set_angles(RopeParams& p, const int32_t* positions, int64_t pos_stride, int n_axes,
+               const int32_t* sections, const float* inv_freq) {
+    AMPB_REQUIRE(n_axes >= 0 && n_axes <= kMaxAxes, AMP_ERR_UNSUPPORTED,
+                 "rope: %d axes not supported (at most %d)", n_axes, kMaxAxes);
+    AMPB_REQUIRE(n_axes == 0 || (positions && sections && inv_freq), AMP_ERR_INVALID,
+                 "rope: NULL positions, sections or inv_freq");
+    int64_t pairs = 0;
+    for (int a = 0; a < n_axes; ++a) {
+        AMPB_REQUIRE(sections[a] >= 0, AMP_ERR_INVALID, "rope: section %d is negative", a);
+        pairs += sections[a];
+        if (a < kMaxAxes - 1) p.axis_end[a] = (int)std::min<int64_t>(pairs, INT32_MAX);
+    }
+    // pairs past the last axis do not exist: later ends are never reached
+    for (int a = std::max(n_axes - 1, 0); a < kMaxAxes - 1; ++a) p.axis_end[a] = INT32_MAX;
+    AMPB_REQUIRE(2 * pairs <= p.D, AMP_ERR_INVALID, "rope: sections name %lld pairs, head_dim is %d",
+                 (long long)pairs, p.D);
+    AMPB_REQUIRE(n_axes <= 1 || pos_stride >= p.T, AMP_ERR_INVALID,
+                 "rope: the axes' positions overlap (stride %lld < %d tokens)", (long long)pos_stride,
+                 p.T);
+    p.pairs = (int)pairs;
+    p.pos = positions;
+    p.pos_stride = pos_stride;
+    p.inv_freq = inv_freq;
+    return AMP_OK;
+}
+
+int set_tensor(RopeParams& p, int i, const void* in, void* out, int heads, const int64_t* in_strides,
+               const int64_t* out_strides, bool has_out) {
+    p.heads[i] = heads;
+    if (heads == 0) return AMP_OK;
+    AMPB_REQUIRE(in && (out || !has_out), AMP_ERR_INVALID, "rope: NULL tensor");
+    for (int s = 0; s < 2; ++s)
+        AMPB_REQUIRE(in_strides[s] > 0 && (!has_out || out_strides[s] > 0), AMP_ERR_INVALID,
+                     "rope: strides must be positive");
+    AMPB_REQUIRE(!has_out || in != out || (in_strides[0] == out_strides[0] && in_strides[1] == out_strides[1]),
+                 AMP_ERR_INVALID, "rope: in place, the output's strides must be the input's");
+    p.x[i] = {in, out, in_strides[0], in_strides[1], has_out ? out_strides[0] : 0,
+              has_out ? out_strides[1] : 0};
+    return AMP_OK;
+}
+
+int check_sizes(int T, int Hq, int Hk, int D) {
+    AMPB_REQUIRE(T >= 0 && Hq >= 0 && Hk >= 0 && D > 0, AMP_ERR_INVALID, "rope: negative size");
+    AMPB_REQUIRE(D % 2 == 0 && D <= 1024 && Hq <= 4096 && Hk <= 4096, AMP_ERR_UNSUPPORTED,
+                 "rope: head_dim %d (even, at most 1024) or %d + %d heads (at most 4096 each) not "
+                 "supported", D, Hq, Hk);
+    return AMP_OK;
+}
+
+}  // namespace
+}  // namespace ampb
+
+using namespace ampb;
+
+extern "C" int amp_rope_dev(const void* q, void* q_out, const void* k, void* k_out, int dtype, int T,
+                            int Hq, int Hk, int head_dim, const int64_t* strides,
+                            const int32_t* positions, int64_t pos_stride, int n_axes,
+                            const int32_t* sections, const float* inv_freq, int interleaved,
+                            int backward, void* stream) {
+    RopeParams p = {};
+    int rc = check_sizes(T, Hq, Hk, head_dim);
+    if (rc) return rc;
+    AMPB_REQUIRE(dtype == AMP_DTYPE_BF16 || dtype == AMP_DTYPE_F32, AMP_ERR_UNSUPPORTED,
+                 "rope: dtype %d not supported (bf16, fp32)", dtype);
+    AMPB_REQUIRE(strides, AMP_ERR_INVALID, "rope: NULL strides");
+    p.T = T;
+    p.D = head_dim;
+    p.H = Hq + Hk;
+    p.sign = backward ? -1.0f : 1.0f;
+    if ((rc = set_angles(p, positions, pos_stride, n_axes, sections, inv_freq))) return rc;
+    if (T == 0 || p.H == 0) return AMP_OK;
+    if ((rc = set_tensor(p, 0, q, q_out, Hq, strides, strides + 2, true))) return rc;
+    if ((rc = set_tensor(p, 1, k, k_out, Hk, strides + 4, strides + 6, true))) return rc;
+    return dtype == AMP_DTYPE_BF16
+               ? launch_rope<__nv_bfloat16, false>(p, interleaved != 0, as_stream(stream))
+               : launch_rope<float, false>(p, interleaved != 0, as_stream(stream));
+}
+
+extern "C" int amp_paged_rope_append_bf16_dev(
+    const void* q, void* q_out, const void* k, const void* v, int T, int Hq, int Hkv, int head_dim,
+    const int64_t* strides, const int32_t* positions, int64_t pos_stride, int n_axes,
+    const int32_t* sections, const float* inv_freq, int interleaved, void* k_pool, void* v_pool,
+    const int32_t* block_table, const int32_t* ctx_lens, const int32_t* cu_seqlens, int B,
+    int num_pages, int max_pages_per_seq, void* stream) {
+    RopeParams p = {};
+    int rc = check_sizes(T, Hq, Hkv, head_dim);
+    if (rc) return rc;
+    AMPB_REQUIRE(strides, AMP_ERR_INVALID, "append: NULL strides");
+    AMPB_REQUIRE(B > 0 && Hkv > 0 && num_pages > 0 && max_pages_per_seq > 0, AMP_ERR_INVALID,
+                 "append: sizes must be positive");
+    p.T = T;
+    p.D = head_dim;
+    p.H = Hq + 2 * Hkv;
+    p.sign = 1.0f;
+    if ((rc = set_angles(p, positions, pos_stride, n_axes, sections, inv_freq))) return rc;
+    AMPB_REQUIRE(k_pool && v_pool && block_table && ctx_lens && cu_seqlens, AMP_ERR_INVALID,
+                 "append: NULL pool or table");
+    if (T == 0) return AMP_OK;
+    if ((rc = set_tensor(p, 0, q, q_out, Hq, strides, strides + 2, true))) return rc;
+    if ((rc = set_tensor(p, 1, k, nullptr, Hkv, strides + 4, nullptr, false))) return rc;
+    if ((rc = set_tensor(p, 2, v, nullptr, Hkv, strides + 6, nullptr, false))) return rc;
+    p.k_pool = k_pool;
+    p.v_pool = v_pool;
+    p.block_table = block_table;
+    p.ctx_lens = ctx_lens;
+    p.cu = cu_seqlens;
+    p.B = B;
+    p.num_pages = num_pages;
+    p.max_pages = max_pages_per_seq;
+    if ((rc = device_status(&p.status))) return rc;
+    return launch_rope<__nv_bfloat16, true>(p, interleaved != 0, as_stream(stream));
+}

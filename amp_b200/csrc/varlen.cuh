@@ -58,8 +58,9 @@ int varlen_make_plan(const VarlenPlan& plan, const int* cu_q, const int* cu_kv, 
                      int total_kv, int Hq, int Hkv, bool backward, cudaStream_t st);
 
 // Warp-wide (all lanes call it): the sequence r whose items hold `item`, i.e. the
-// last r with first[r] <= item; sequences without items are never returned.
-// first[] ascends and item < first[B].
+// last r with first[r] <= item, where first[] ascends and first[0] <= item < first[B];
+// sequences without items are never returned.  Whatever first[] holds, the result is
+// in [0, B).
 __device__ __forceinline__ int varlen_find(const int* first, int B, int item) {
     const int lane = threadIdx.x & 31;
     int lo = 0, n = B;                 // the answer is in [lo, lo + n)
@@ -67,7 +68,7 @@ __device__ __forceinline__ int varlen_find(const int* first, int B, int item) {
         const int step = (n + 31) / 32;
         const int at = lo + lane * step;
         const bool le = lane * step < n && first[at] <= item;
-        const int k = __popc(__ballot_sync(0xffffffffu, le)) - 1;   // first[lo] <= item: k >= 0
+        const int k = max(__popc(__ballot_sync(0xffffffffu, le)) - 1, 0);
         n = min(step, n - k * step);
         lo += k * step;
     }

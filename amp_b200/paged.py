@@ -15,7 +15,8 @@ import ctypes as C
 import numpy as np
 import torch
 
-from ._lib import call, lib
+from . import rope
+from ._lib import call, call_on, lib
 
 PAGE_TOKENS = 16
 
@@ -126,3 +127,49 @@ def pack_block_table(page_lists, ctx_lens, max_pages_per_seq: int | None = None)
 def pool_bytes(num_pages: int, Hkv: int, D: int) -> int:
     """Bytes of one contiguous K or V pool [num_pages][Hkv][16][D] bf16."""
     return int(lib().amp_paged_pool_bytes(num_pages, Hkv, D))
+
+
+def _append(q, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, angles, interleaved, out_q):
+    _check_pools(k_pool, v_pool, block_table, ctx_lens)
+    num_pages, Hkv, _, D = k_pool.shape
+    T, dev = k.shape[0], k_pool.device
+    strides = list(rope.tensor_strides(q, "q", dev, k_pool.dtype, T, D)
+                   + rope.tensor_strides(out_q, "out_q", dev, k_pool.dtype, T, D)
+                   if q is not None else (D,) * 4)
+    strides += rope.tensor_strides(k, "k", dev, k_pool.dtype, T, D)
+    strides += rope.tensor_strides(v, "v", dev, k_pool.dtype, T, D)
+    if k.shape[1] != Hkv or v.shape[1] != Hkv or (q is not None and q.shape != out_q.shape):
+        raise ValueError(f"k and v must have the pools' {Hkv} heads, and out_q the shape of q")
+    B = cu_seqlens.numel() - 1
+    if cu_seqlens.device != dev or cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 \
+            or not cu_seqlens.is_contiguous() or B < 1:
+        raise ValueError(f"cu_seqlens: expected a contiguous int32 tensor [sequences + 1] on {dev}")
+    if v_pool.device != dev or block_table.device != dev or ctx_lens.device != dev \
+            or block_table.dim() != 2 or block_table.shape[0] < B or ctx_lens.numel() < B:
+        raise ValueError(f"block_table [>= {B}, pages] and ctx_lens [>= {B}] expected on {dev}")
+    call_on(dev, "amp_paged_rope_append_bf16_dev", q.data_ptr() if q is not None else None,
+            out_q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), T,
+            q.shape[1] if q is not None else 0, Hkv, D, (C.c_int64 * 8)(*strides), *angles,
+            1 if interleaved else 0, k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
+            ctx_lens.data_ptr(), cu_seqlens.data_ptr(), B, num_pages, block_table.shape[1])
+
+
+def append(k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens) -> None:
+    """Writes the new tokens' k and v [tokens, Hkv, D] (bf16, any token and head strides) into their
+    pages.  Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b+1] and the last ones of
+    its context: ctx_lens counts them already.  Tokens of no sequence are skipped; one without a
+    page in the table is not written and reported by amp_device_status."""
+    _append(None, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, (None, 0, 0, None, None),
+            False, None)
+
+
+def rope_append(q, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, positions, inv_freq,
+                sections=None, interleaved: bool = False, out_q=None):
+    """append() of k turned by its rotary position, and q turned the same way, in one pass: returns
+    q' [tokens, Hq, D] (rows of no sequence are not written).  Rotary arguments as rope.rope_fwd."""
+    if q.dim() != 3 or not q.is_cuda:
+        raise ValueError("q: expected a bf16 CUDA tensor [tokens, heads, head_dim]")
+    angles = rope.angle_args(positions, inv_freq, sections, q.device, k.shape[0])
+    out_q = out_q if out_q is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _append(q, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, angles, interleaved, out_q)
+    return out_q

@@ -306,6 +306,26 @@ AMP_API int amp_flash_attn_varlen_bwd_bf16_dev(const void* Q, const void* K, con
                                                void* stream);
 
 /* ------------------------------------------------------------------------
+ * Rotary positions with one or more axes (text; or time, height and width of
+ * images and video).  No counterpart in the reference.  For tokens [T, heads,
+ * head_dim] of q and k (either may have 0 heads), pair i < pairs = sum(sections)
+ * of every head is turned by pos[axis(i)][t] * inv_freq[i]; backward != 0 turns
+ * back (the gradient).  Pairs are elements (i, i + pairs), or (2i, 2i + 1) when
+ * interleaved != 0; elements from 2 * pairs on pass through.
+ *   positions  device int32 [n_axes][pos_stride], the first T of each row used
+ *   sections   HOST int32 [n_axes], pairs that follow each axis; n_axes <= 4
+ *   inv_freq   device float [pairs]
+ *   strides    HOST array: token and head stride in elements of q, q_out, k, k_out
+ * dtype BF16 or F32; head_dim even, at most 1024.  An output may be its input
+ * (same strides); no other overlap.  The angle is reduced in 64 bits.
+ * ---------------------------------------------------------------------- */
+AMP_API int amp_rope_dev(const void* q, void* q_out, const void* k, void* k_out, int dtype, int T,
+                         int Hq, int Hk, int head_dim, const int64_t* strides,
+                         const int32_t* positions, int64_t pos_stride, int n_axes,
+                         const int32_t* sections, const float* inv_freq, int interleaved,
+                         int backward, void* stream);
+
+/* ------------------------------------------------------------------------
  * Attention over a paged KV cache (block tables of 16-token pages, the
  * format of Sequence::kv_page_ids / kv_page_size_tokens in the reference's
  * include/scheduler.hpp:61,88; the reference has no kernel that reads it).
@@ -337,6 +357,22 @@ AMP_API int amp_paged_attn_prefill_bf16_dev(const void* q, const void* k_pool, c
                                             void* out, float* lse, int B, int Hq, int Hkv, int Lq,
                                             int head_dim, int num_pages, int max_pages_per_seq,
                                             float scale, void* stream);
+/* Writes new tokens into the cache: k (turned by its rotary position) and v of
+ * packed tokens go to their pages, and q's rotation to q_out, in one pass.
+ * Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b+1]-1 (device
+ * int32 [B+1]) and the LAST ones of its context: ctx_lens[b] counts them
+ * already, as the prefill and decode that follow expect.  Rotary arguments as
+ * for amp_rope_dev; n_axes 0 (positions, sections, inv_freq NULL) writes k as it
+ * is, and Hq 0 leaves q out.  strides (HOST): token and head stride of q, q_out,
+ * k, v.  Tokens of no sequence are skipped; a token whose page is missing from
+ * the table or outside the pool is not written and reported by
+ * amp_device_status (AMP_ERR_INVALID). */
+AMP_API int amp_paged_rope_append_bf16_dev(
+    const void* q, void* q_out, const void* k, const void* v, int T, int Hq, int Hkv, int head_dim,
+    const int64_t* strides, const int32_t* positions, int64_t pos_stride, int n_axes,
+    const int32_t* sections, const float* inv_freq, int interleaved, void* k_pool, void* v_pool,
+    const int32_t* block_table, const int32_t* ctx_lens, const int32_t* cu_seqlens, int B,
+    int num_pages, int max_pages_per_seq, void* stream);
 /* Host-side check of a block table (host arrays) before upload: ids in range,
  * no page used twice, rows long enough for the contexts. */
 AMP_API int amp_paged_validate_block_table(const int32_t* block_table, const int32_t* ctx_lens,
