@@ -70,6 +70,19 @@ SIGNATURES: dict[str, tuple] = {
     "amp_paged_rope_append_bf16_dev": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp,
                                               _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp,
                                               _i32, _i32, _i32, _vp]),
+    "amp_paged_copy_workspace_bytes": (_sz, [_i32]),
+    "amp_paged_copy_pages_dev": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _sz,
+                                        _vp]),
+    "amp_paged_fork_workspace_bytes": (_sz, [_i32, _i32]),
+    "amp_paged_fork_dev": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _vp,
+                                  _i32, _vp, _vp, _sz, _vp]),
+    "amp_paged_extend_workspace_bytes": (_sz, [_i32, _i32]),
+    "amp_paged_extend_dev": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _vp,
+                                    _vp, _vp, _sz, _vp]),
+    "amp_paged_compact_workspace_bytes": (_sz, [_i32]),
+    "amp_paged_compact_dev": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp,
+                                     _vp, _vp, _sz, _vp]),
+    "amp_paged_free_dev": (_i32, [_vp, _vp, _i32, _i32, _vp, _i32, _vp]),
     "amp_paged_validate_block_table": (_i32, [_vp, _vp, _i32, _i32, _i32]),
     "amp_paged_pack_block_table": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp]),
     "amp_paged_pool_bytes": (_sz, [_i32, _i32, _i32]),

@@ -129,4 +129,29 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Inclusive scan over a block of 1024 threads (`part`: 32 ints of shared memory; the
+// block's total is left in part[31]).
+__device__ __forceinline__ int block_scan(int v, int* part) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    __syncthreads();   // `part` may still be read from the call before
+    if (lane == 31) part[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        int w = part[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += t;
+        }
+        part[lane] = w;
+    }
+    __syncthreads();
+    return v + (warp ? part[warp - 1] : 0);
+}
+
 }  // namespace ampb

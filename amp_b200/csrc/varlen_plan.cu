@@ -26,30 +26,6 @@ __device__ __forceinline__ int length_bucket(int len) {
     return kBuckets - 2 - (int)(u - (0x3f800000u >> 18));
 }
 
-// Inclusive scan over the block's 1024 threads (`part`: 32 ints of shared memory).
-__device__ __forceinline__ int block_scan(int v, int* part) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += t;
-    }
-    __syncthreads();   // `part` may still be read from the call before
-    if (lane == 31) part[warp] = v;
-    __syncthreads();
-    if (warp == 0) {
-        int w = part[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += t;
-        }
-        part[lane] = w;
-    }
-    __syncthreads();
-    return v + (warp ? part[warp - 1] : 0);
-}
-
 __global__ void __launch_bounds__(kPlanThreads)
     k_varlen_plan(VarlenPlan pl, const int* __restrict__ cu_q, const int* __restrict__ cu_kv,
                   int total_q, int total_kv, int Hq, int Hkv, int backward, int* status) {

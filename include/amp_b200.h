@@ -373,6 +373,63 @@ AMP_API int amp_paged_rope_append_bf16_dev(
     const int32_t* sections, const float* inv_freq, int interleaved, void* k_pool, void* v_pool,
     const int32_t* block_table, const int32_t* ctx_lens, const int32_t* cu_seqlens, int B,
     int num_pages, int max_pages_per_seq, void* stream);
+/* Bookkeeping of the cache on the device.  Page p is in use iff some row b of the
+ * block table names it among its first ceil(ctx_lens[b] / 16) entries; entries
+ * past those mean nothing.  Nothing else is kept, so a host that owns the page
+ * lists (AMP's scheduler and PagePoolFast, src/pool_fast.cpp:31-60) and these
+ * calls must not hand out pages of one pool side by side.  Pages are handed out
+ * lowest first, in the order of the request.
+ *   k_pool, v_pool  [layers][num_pages][Hkv][16][head_dim] bf16: one table serves
+ *                   every layer; at most 786432 pages, 16-byte aligned
+ *   block_table     int32 [rows][max_pages_per_seq], ctx_lens int32 [rows]; at most
+ *                   65536 rows
+ * All calls are asynchronous on `stream`; a workspace (16-byte aligned) must not
+ * be shared by calls that may overlap.  Row and page numbers outside their
+ * arrays are skipped and reported by amp_device_status (AMP_ERR_INVALID). */
+/* Copies page src[i] onto page dst[i] (device int32 [n]) in every layer.  A negative
+ * number, or a page onto itself, is nothing to do.  A page named twice as a
+ * target, or as a source and as another pair's target, has no defined order:
+ * those pairs are skipped and reported. */
+AMP_API size_t amp_paged_copy_workspace_bytes(int n);
+AMP_API int amp_paged_copy_pages_dev(void* k_pool, void* v_pool, int layers, int num_pages, int Hkv,
+                                     int head_dim, const int32_t* src, const int32_t* dst, int n,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+/* Row children[i] becomes a copy of row parents[i] as both are before the call: the
+ * same full pages, and a fresh copy of a partly filled last one, so that both may
+ * be extended.  What a child held is released first (but pages of a row that is
+ * also a parent are not handed out in this call).  done[i] = 1, or 0 if no page
+ * was left (the child is then empty) or the row numbers are bad or the child is
+ * named twice (nothing is done). */
+AMP_API size_t amp_paged_fork_workspace_bytes(int n, int max_pages_per_seq);
+AMP_API int amp_paged_fork_dev(void* k_pool, void* v_pool, int layers, int num_pages, int Hkv,
+                               int head_dim, int32_t* block_table, int32_t* ctx_lens, int rows,
+                               int max_pages_per_seq, const int32_t* parents,
+                               const int32_t* children, int n, int32_t* done, void* workspace,
+                               size_t workspace_bytes, void* stream);
+/* Gives every row the pages for add[b] more tokens (device int32 [rows]): ctx_out[b] =
+ * ctx_lens[b] + add[b], done[b] = 1.  A partly filled last page that another row
+ * names too is copied first.  A row that would not fit into the table, whose
+ * add is negative, or that the pool cannot hold stays as it is, done[b] = 0; once
+ * the pool cannot hold one, no later row gets pages.  ctx_out may be ctx_lens. */
+AMP_API size_t amp_paged_extend_workspace_bytes(int rows, int num_pages);
+AMP_API int amp_paged_extend_dev(void* k_pool, void* v_pool, int layers, int num_pages, int Hkv,
+                                 int head_dim, int32_t* block_table, const int32_t* ctx_lens,
+                                 int rows, int max_pages_per_seq, const int32_t* add,
+                                 int32_t* ctx_out, int32_t* done, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+/* Moves the pages in use to the pool's front: with *used of them (device int32), those
+ * from page *used on go to the free pages below it, both in ascending order.
+ * Writes the changed table to table_out [rows][max_pages_per_seq] (-1 past each
+ * row's entries), which may be block_table. */
+AMP_API size_t amp_paged_compact_workspace_bytes(int num_pages);
+AMP_API int amp_paged_compact_dev(void* k_pool, void* v_pool, int layers, int num_pages, int Hkv,
+                                  int head_dim, const int32_t* block_table,
+                                  const int32_t* ctx_lens, int rows, int max_pages_per_seq,
+                                  int32_t* table_out, int32_t* used, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+/* Empties rows seqs[0 .. n): context 0, entries -1; pages no other row names are free. */
+AMP_API int amp_paged_free_dev(int32_t* block_table, int32_t* ctx_lens, int rows,
+                               int max_pages_per_seq, const int32_t* seqs, int n, void* stream);
 /* Host-side check of a block table (host arrays) before upload: ids in range,
  * no page used twice, rows long enough for the contexts. */
 AMP_API int amp_paged_validate_block_table(const int32_t* block_table, const int32_t* ctx_lens,
