@@ -8,12 +8,11 @@
 // the first sections[0] pairs follow axis 0 (time), the next sections[1] axis 1
 // (height), and so on.  The reference has no positional encoding.
 //
-// HBM-bound: every element is read and written once.  A unit of work is two
-// vectors of VE elements that hold VE pairs (or 2 VE elements that pass through);
-// a block takes 256 * U consecutive units in (token, head, unit) order, so loads
-// and stores of a warp cover whole rows.  The angles of the block's tokens are
-// computed once into shared memory, after the block's loads have been issued:
-// they are shared by all heads, and their arithmetic hides behind the loads.
+// HBM-bound: every element is read and written once.  A warp takes a token and walks
+// its heads (of q, k and v in turn): a lane holds a unit, two vectors of VE elements
+// with VE pairs (or 2 VE elements that pass through), 32 / units heads at a time.  The token's angles are computed once a warp
+// into its own shared memory, behind the first loads, and a lane keeps the VE it
+// needs in registers for all heads; nothing waits for another warp.
 //
 // The angle is reduced in 64 bits (turns = pos * inv_freq / 2 pi, less the nearest
 // whole number): in 32 bits a position of 10^5 is off by 2^-7 of a radian.  The
@@ -37,7 +36,13 @@
 namespace ampb {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 256, kRopeWarps = kRopeThreads / 32;
+// Two steps of loads (64 bytes a lane) in flight and 64 registers, for 32 warps a
+// multiprocessor: on 32768 tokens x 40 heads x 128 (forward and backward, 1.34 GB) 294 us;
+// four steps at 16 warps 367, one step at 40 warps 274, and 223 us (6.0 TB/s) for two steps
+// with the streaming hint on both sides (below): rows are read and written once, and
+// without it the lines written push out those that neighbouring warps are reading.
+constexpr int kSteps = 2, kBlocksPerSM = 4;
 constexpr int kMaxAxes = 4;
 constexpr int kPage = 16;
 
@@ -52,7 +57,10 @@ struct RopeParams {
     int heads[3];
     int T, H, D;           // H: heads of all tensors
     int pairs;             // R / 2
-    int units;             // per head: (R + passed) / (2 VE)
+    int units;             // of a head: D / (2 VE)
+    int lanes_heads;       // heads of a step: 32 / units, 1 if a head has more units than lanes
+    int steps;             // of a token: H / lanes_heads, rounded up
+    int steps_warp, splits;   // steps that one warp takes; warps of a token
     float sign;            // -1: backward
     const int* pos;        // [axes][T]
     int64_t pos_stride;
@@ -69,6 +77,17 @@ template <typename T, int VE>
 struct alignas(sizeof(T) * VE) Vec {
     T v[VE];
 };
+
+template <typename V>
+__device__ __forceinline__ void load_once(V& v, const void* p) {
+    if constexpr (sizeof(V) == 16) *reinterpret_cast<uint4*>(&v) = __ldcs(static_cast<const uint4*>(p));
+    else v = *static_cast<const V*>(p);
+}
+template <typename V>
+__device__ __forceinline__ void store_once(void* p, const V& v) {
+    if constexpr (sizeof(V) == 16) __stcs(static_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+    else *static_cast<V*>(p) = v;
+}
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -108,111 +127,109 @@ __device__ __forceinline__ int64_t cache_row(const RopeParams& p, int t, int Hkv
     return ((int64_t)page * Hkv * kPage + at % kPage) * p.D;
 }
 
-template <typename T, int VE, bool kInter, bool kAppend, int U>
-__global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ RopeParams p) {
-    // cos, sin [tokens of this block][VE][pairs / VE]: a warp's lanes read neighbours
-    extern __shared__ float2 trig[];
+template <typename T, int VE, bool kInter, bool kAppend>
+__global__ void __launch_bounds__(kRopeThreads, kBlocksPerSM) k_rope(const __grid_constant__ RopeParams p) {
     using V = Vec<T, VE>;
+    // cos, sin [warp][VE][pairs / VE]: the lanes of a head read neighbours
+    extern __shared__ float2 trig_all[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float2* trig = trig_all + warp * p.pairs;
     pdl_wait();
-    const int per_token = p.H * p.units;
-    const int64_t total = (int64_t)p.T * per_token;
-    const int64_t u0 = (int64_t)blockIdx.x * (kRopeThreads * U);
-    const int64_t u1 = min(u0 + kRopeThreads * U, total);
-    const int t0 = (int)(u0 / per_token);
-    const int ntok = (int)((u1 - 1) / per_token) - t0 + 1;
-    const int first = (int)(u0 - (int64_t)t0 * per_token);   // u0 within token t0
-    int64_t* rows = reinterpret_cast<int64_t*>(trig + (size_t)ntok * p.pairs);   // append
-
-    V a[U], b[U];
-    int tok[U], off_a[U], off_b[U], hd[U], which[U], pair0[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-        const int w = first + i * kRopeThreads + threadIdx.x;
-        which[i] = -1;
-        if (u0 + i * kRopeThreads + threadIdx.x >= u1) continue;
-        tok[i] = w / per_token;
-        const int r = w - tok[i] * per_token;
-        int h = r / p.units;
-        const int c = r - h * p.units;
-        int x = 0;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (x == k && h >= p.heads[k]) {
-                h -= p.heads[k];
-                x = k + 1;
-            }
-        which[i] = x;
-        hd[i] = h;
-        pair0[i] = c * VE;
-        const bool turned = c * VE < p.pairs;
-        off_a[i] = turned && !kInter ? c * VE : c * 2 * VE;
-        off_b[i] = turned && !kInter ? p.pairs + c * VE : c * 2 * VE + VE;
-        const T* src = static_cast<const T*>(p.x[x].in) + (t0 + tok[i]) * p.x[x].in_tok + h * p.x[x].in_head;
-        a[i] = *reinterpret_cast<const V*>(src + off_a[i]);
-        b[i] = *reinterpret_cast<const V*>(src + off_b[i]);
-    }
+    const int64_t task = (int64_t)blockIdx.x * kRopeWarps + warp;
+    if (task >= (int64_t)p.T * p.splits) return;
+    const int t = (int)(task / p.splits);
+    const int step0 = (int)(task - (int64_t)t * p.splits) * p.steps_warp;
+    const int step1 = min(step0 + p.steps_warp, p.steps);
     const int chunks = p.pairs / VE;
-    for (int i = threadIdx.x; i < ntok * p.pairs; i += kRopeThreads) {
-        const int t = i / p.pairs, pair = i - t * p.pairs;
-        trig[t * p.pairs + pair % VE * chunks + pair / VE] = angle(p, t0 + t, pair);
-    }
-    if constexpr (kAppend) {
-        for (int t = threadIdx.x >> 5; t < ntok; t += kRopeThreads / 32) {
-            const int64_t row = cache_row(p, t0 + t, p.heads[1]);
-            if ((threadIdx.x & 31) == 0) rows[t] = row;
-        }
-    }
-    __syncthreads();
+    const bool narrow = p.units <= 32;
+    const int sub = narrow ? lane / p.units : 0;
+    int64_t row = 0;
+    bool ready = false;
+    for (int c0 = 0; c0 < p.units; c0 += 32) {
+        const int c = narrow ? lane - sub * p.units : c0 + lane;
+        const bool live = sub < p.lanes_heads && c < p.units;
+        const bool turned = c < chunks;
+        const int off_a = turned && !kInter ? c * VE : c * 2 * VE;
+        const int off_b = turned && !kInter ? p.pairs + c * VE : c * 2 * VE + VE;
+        float2 cs[VE];
+        bool loaded = false;
+        for (int s0 = step0; s0 < step1; s0 += kSteps) {
+            V a[kSteps], b[kSteps];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-        if (which[i] < 0) continue;
-        if (pair0[i] < p.pairs && !(kAppend && which[i] == 2)) {
-            const float2* cs = trig + tok[i] * p.pairs + pair0[i] / VE;
+            for (int i = 0; i < kSteps; ++i) {
+                const int h = (s0 + i) * p.lanes_heads + sub;
+                if (!live || s0 + i >= step1 || h >= p.H) continue;
+                const int x = (h >= p.heads[0]) + (h >= p.heads[0] + p.heads[1]);
+                const int hx = h - (x > 0 ? p.heads[0] : 0) - (x > 1 ? p.heads[1] : 0);
+                const T* src = static_cast<const T*>(x == 0 ? p.x[0].in : x == 1 ? p.x[1].in : p.x[2].in) +
+                               t * (x == 0 ? p.x[0].in_tok : x == 1 ? p.x[1].in_tok : p.x[2].in_tok) +
+                               hx * (x == 0 ? p.x[0].in_head : x == 1 ? p.x[1].in_head : p.x[2].in_head);
+                load_once(a[i], src + off_a);
+                load_once(b[i], src + off_b);
+            }
+            if (!ready) {
+                ready = true;
+                for (int i = lane; i < p.pairs; i += 32) trig[i % VE * chunks + i / VE] = angle(p, t, i);
+                if constexpr (kAppend) row = cache_row(p, t, p.heads[1]);
+                __syncwarp();
+                if (kAppend && row == kNoSequence) return;
+            }
+            if (!loaded && turned && live) {
 #pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                // pair e: elements e of both vectors, or neighbours within the two
-                T& x = kInter ? (2 * e < VE ? a[i].v[(2 * e) % VE] : b[i].v[(2 * e) % VE]) : a[i].v[e];
-                T& y = kInter ? (2 * e + 1 < VE ? a[i].v[(2 * e + 1) % VE] : b[i].v[(2 * e + 1) % VE])
-                              : b[i].v[e];
-                const float fx = to_f32(x), fy = to_f32(y);
-                const float2 w = cs[e * chunks];
-                x = from_f32<T>(fx * w.x - fy * w.y);
-                y = from_f32<T>(fy * w.x + fx * w.y);
+                for (int e = 0; e < VE; ++e) cs[e] = trig[e * chunks + c];
+            }
+            loaded = true;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int h = (s0 + i) * p.lanes_heads + sub;
+                if (!live || s0 + i >= step1 || h >= p.H) continue;
+                const int x = (h >= p.heads[0]) + (h >= p.heads[0] + p.heads[1]);
+                const int hx = h - (x > 0 ? p.heads[0] : 0) - (x > 1 ? p.heads[1] : 0);
+                if (turned && !(kAppend && x == 2)) {
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) {
+                        // pair e: elements e of both vectors, or neighbours within the two
+                        T& u = kInter ? (2 * e < VE ? a[i].v[(2 * e) % VE] : b[i].v[(2 * e) % VE]) : a[i].v[e];
+                        T& v = kInter ? (2 * e + 1 < VE ? a[i].v[(2 * e + 1) % VE] : b[i].v[(2 * e + 1) % VE])
+                                      : b[i].v[e];
+                        const float fu = to_f32(u), fv = to_f32(v);
+                        // the fused product is named, so that every vector width gives the same bits
+                        u = from_f32<T>(__fmaf_rn(fu, cs[e].x, -__fmul_rn(fv, cs[e].y)));
+                        v = from_f32<T>(__fmaf_rn(fv, cs[e].x, __fmul_rn(fu, cs[e].y)));
+                    }
+                }
+                T* dst;
+                if (kAppend && x > 0) {
+                    if (row < 0) continue;
+                    dst = static_cast<T*>(x == 1 ? p.k_pool : p.v_pool) + row + (int64_t)hx * kPage * p.D;
+                } else {
+                    dst = static_cast<T*>(x == 0 ? p.x[0].out : p.x[1].out) +
+                          t * (x == 0 ? p.x[0].out_tok : p.x[1].out_tok) +
+                          hx * (x == 0 ? p.x[0].out_head : p.x[1].out_head);
+                }
+                store_once(dst + off_a, a[i]);
+                store_once(dst + off_b, b[i]);
             }
         }
-        const int x = which[i];
-        T* dst;
-        if constexpr (kAppend) {
-            const int64_t row = rows[tok[i]];
-            if (row == kNoSequence || (row == kNoPage && x > 0)) continue;
-            if (x > 0)
-                dst = static_cast<T*>(x == 1 ? p.k_pool : p.v_pool) + row + (int64_t)hd[i] * kPage * p.D;
-            else
-                dst = static_cast<T*>(p.x[0].out) + (t0 + tok[i]) * p.x[0].out_tok + hd[i] * p.x[0].out_head;
-        } else {
-            dst = static_cast<T*>(p.x[x].out) + (t0 + tok[i]) * p.x[x].out_tok + hd[i] * p.x[x].out_head;
-        }
-        *reinterpret_cast<V*>(dst + off_a[i]) = a[i];
-        *reinterpret_cast<V*>(dst + off_b[i]) = b[i];
     }
 }
 
 template <typename T, int VE, bool kInter, bool kAppend>
 int launch_rope_as(RopeParams& p, cudaStream_t st) {
     p.units = p.D / (2 * VE);
-    const int64_t total = (int64_t)p.T * p.H * p.units;
-    // Four units a thread keep eight 16-byte loads in flight; with fewer blocks than two a
-    // multiprocessor (a decode step) one unit a thread spreads the latency instead, and with
-    // under four heads four units would mean more tokens' angles than shared memory should hold.
-    const bool wide = p.H >= 4 && total >= (int64_t)sm_count() * 2 * kRopeThreads * 4;
-    const int per_block = kRopeThreads * (wide ? 4 : 1);
-    const int64_t per_token = (int64_t)p.H * p.units;
-    const int64_t tokens = (per_block + per_token - 2) / per_token + 1;
-    const size_t smem = (size_t)tokens * p.pairs * sizeof(float2) + (kAppend ? tokens * 8 : 0);
-    const int64_t blocks = (total + per_block - 1) / per_block;
-    AMPB_REQUIRE(blocks <= INT32_MAX && per_token <= (1 << 24), AMP_ERR_UNSUPPORTED, "rope: too large");
-    auto kern = wide ? k_rope<T, VE, kInter, kAppend, 4> : k_rope<T, VE, kInter, kAppend, 1>;
-    AMPB_CHECK_CUDA(launch_pdl(kern, dim3((unsigned)blocks), dim3(kRopeThreads), smem, st, p));
+    p.lanes_heads = std::max(1, 32 / p.units);
+    p.steps = (p.H + p.lanes_heads - 1) / p.lanes_heads;
+    // A warp takes all of a token's heads, so that its angles are computed once, unless that
+    // leaves multiprocessors idle (a decode step): then the heads are shared out.
+    const int64_t fill = (int64_t)sm_count() * kRopeWarps;
+    p.splits = (int)std::min<int64_t>(p.steps, std::max<int64_t>(1, fill / std::max(p.T, 1)));
+    p.steps_warp = (p.steps + p.splits - 1) / p.splits;
+    p.splits = (p.steps + p.steps_warp - 1) / p.steps_warp;
+    const size_t smem = (size_t)kRopeWarps * p.pairs * sizeof(float2);
+    const int64_t blocks = ((int64_t)p.T * p.splits + kRopeWarps - 1) / kRopeWarps;
+    AMPB_REQUIRE(blocks <= INT32_MAX, AMP_ERR_UNSUPPORTED, "rope: too large");
+    AMPB_CHECK_CUDA(launch_pdl(k_rope<T, VE, kInter, kAppend>, dim3((unsigned)blocks), dim3(kRopeThreads),
+                               smem, st, p));
     return AMP_OK;
 }
 
