@@ -60,6 +60,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "peer.cuh"
@@ -126,6 +127,9 @@ __device__ unsigned g_fa_allgather_done;
 
 constexpr int kPageTokens = 16;
 
+using Poll = std::false_type;    // how a warp waits for the packed mode's next item
+using Sleep = std::true_type;
+
 __device__ __forceinline__ float lg2_approx(float x) {
     float y;
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -149,6 +153,33 @@ struct FaCfg {
     static constexpr uint32_t O_COL = 2 * BKV;            // S0 | S1 | O0 | O1
 };
 
+// Stage and phase of a K/V tile in its ring, for tile j of the current item.  Dense: the
+// tiles of all items run through the ring in turn.  Packed: every item starts at stage 0.
+// An item's tile count then comes out of shared memory, and a stage that depended on the
+// counts of earlier items could not be known to be the same in every lane: the MMA
+// descriptors would live in vector registers, be spilled and be converted for every
+// MMA (835 against 1000 TFLOP/s at 4 x 4096, 32 / 8 heads).
+template <bool kPerItem>
+struct KvRing {
+    int used0 = 0, used1 = 0;   // per item: uses of each stage; else used0: tiles in all
+    __device__ __forceinline__ int stage(int j) const {
+        return (kPerItem ? j : used0 + j) % KV_STAGES;
+    }
+    __device__ __forceinline__ uint32_t phase(int j) const {
+        if constexpr (kPerItem) return ((j % KV_STAGES ? used1 : used0) + j / KV_STAGES) & 1;
+        else return ((used0 + j) / KV_STAGES) & 1;
+    }
+    __device__ __forceinline__ void advance(int n) {
+        if constexpr (kPerItem) {
+            static_assert(KV_STAGES == 2, "two use counts");
+            used0 += (n + 1) / 2;
+            used1 += n / 2;
+        } else {
+            used0 += n;
+        }
+    }
+};
+
 // kPersist: one CTA per SM walks a list of (batch*head, query-tile pair) items
 // (see item_at below) instead of one CTA per item, so that the next item's Q and
 // K/V loads and its first QK overlap the current item's last steps and epilogue.
@@ -160,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     static_assert(!(kPersist && kAllGather), "the all-gather epilogue stages in Q: one item per CTA");
     static_assert(!kPacked || (kPersist && !kPaged), "packed items are drawn by persistent CTAs");
     using CF = FaCfg<D>;
+    using Ring = KvRing<kPacked>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~uintptr_t(1023));
@@ -185,7 +217,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_raw + KV_STAGES);
     PackedItem* items = reinterpret_cast<PackedItem*>(tmem_slot + 2);   // [2]
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // Packed: what comes out of shared memory (items, the TMEM base) or depends on the warp
+    // is not known to be the same in every lane, and what is derived from it lives in vector
+    // registers, spills, and is converted for every MMA.  A shuffle from lane 0 makes it
+    // known, and all 512 columns can only start at column 0 (4 x 4096, 32 / 8 heads: 830
+    // -> 903 TFLOP/s).
+    const int lane = threadIdx.x & 31;
+    const int warp = kPacked ? __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0) : threadIdx.x >> 5;
     const int n_qb = (p.S_q + 2 * BQ - 1) / (2 * BQ);
     // Items of this CTA, k = 0, 1, ...: 0 = no more, 1 = item (bh, qb), 2 = empty slot.
     // Persistent: unit u = blockIdx.x + (k/2) * gridDim.x pairs query-tile pair
@@ -247,25 +285,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // k-th item of this CTA into g: 0 = no more (or a wait ran out), 1 = an item, 2 = an
     // empty slot.  Packed: read from the ring; the reader releases its slot with it_done.
-    auto next_item = [&](int k, Geo& g) -> int {
+    // kSleep: for warps 2 and 3, which have nothing to do for most of an item -- polling,
+    // they took issue slots from the softmax warps of their sub-partitions (a fifth of the
+    // kernel's rate).
+    auto next_item = [&](int k, Geo& g, auto sleep) -> int {
         if constexpr (kPacked) {
-            if (!mbar_wait(&it_full[k & 1], (k >> 1) & 1, p.status)) return 0;
-            const volatile PackedItem& it = items[k & 1];
-            g.n1 = it.n1;
+            if (!mbar_wait<decltype(sleep)::value>(&it_full[k & 1], (k >> 1) & 1, p.status)) return 0;
+            const PackedItem& it = items[k & 1];
+            const unsigned lanes = __activemask();   // lane 0, or the whole warp
+            auto same = [&](int x) { return __shfl_sync(lanes, x, 0); };
+            g.n1 = same(it.n1);
             if (g.n1 == 0) return 0;
-            g.n0 = it.n0;
+            g.n0 = same(it.n0);
             g.b = 0;
             g.h = g.bh = 0;
-            g.bh_kv = it.kv_head;
-            g.S_q = it.q_len;
-            g.S_kv = it.k_len;
-            g.coff = it.k_len - it.q_len;
-            g.q_tok = it.q_tok;
-            g.k_tok = it.k_tok;
+            g.bh_kv = same(it.kv_head);
+            g.S_q = same(it.q_len);
+            g.S_kv = same(it.k_len);
+            g.coff = g.S_kv - g.S_q;
+            g.q_tok = same(it.q_tok);
+            g.k_tok = same(it.k_tok);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                g.q0[t] = it.row0[t];
-                g.head[t] = it.head[t];
+                g.q0[t] = same(it.row0[t]);
+                g.head[t] = same(it.head[t]);
             }
             return 1;
         } else {
@@ -314,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = kPacked ? 0u : *tmem_slot;
     if constexpr (kPacked) pdl_wait();   // the plan
 
     if (warp < 4) {
@@ -324,13 +367,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_prefetch_desc(&tmQ);
             tma_prefetch_desc(&tmK);
             tma_prefetch_desc(&tmV);
-            // K/V tiles run through the rings continuously across items: tile g of
-            // this CTA uses stage g % KV_STAGES in phase (g / KV_STAGES) & 1
-            int gkv = 0, li = 0;
+            // K/V tiles run through the rings continuously across items (Ring)
+            Ring ring;
+            int li = 0;
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 Geo g;
-                const int st = next_item(k, g);
+                const int st = next_item(k, g, Poll{});
                 if (st == 0) break;
                 if (st == 2) continue;
                 it_done(k);
@@ -352,8 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int last_page = max(0, (g.S_kv + kPageTokens - 1) / kPageTokens - 1);
                 const int hk = g.h / (p.Hq / p.Hkv);
                 for (int j = 0; j < g.n1; ++j) {
-                    const int s = (gkv + j) % KV_STAGES;
-                    const uint32_t ph = ((gkv + j) / KV_STAGES) & 1;
+                    const int s = ring.stage(j);
+                    const uint32_t ph = ring.phase(j);
                     int pages[BKV / kPageTokens];
                     if constexpr (kPaged) {
                         const int* bt = p.block_table + (int64_t)g.b * p.max_pages;
@@ -397,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (kPersist && j == 0 && !load_q(1)) { ok = false; break; }
                 }
-                gkv += g.n1;
+                ring.advance(g.n1);
                 ++li;
             }
         }
@@ -414,15 +457,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                                smem_desc_sw128(k_addr + off, 16, 1024), CF::IDESC_QK, kk != 0);
                 }
             };
-            // gkv: K/V tiles consumed before this item (ring stage / phase as in the
-            // load warp); c[t]: query tile t's steps before this item (phase of
+            // ring: as in the load warp; c[t]: query tile t's steps before this item (phase of
             // s_full / p_full / pv_done); li: items before this one (q_full, q_empty,
             // o_free)
-            int gkv = 0, li = 0, c[2] = {0, 0};
+            Ring ring;
+            int li = 0, c[2] = {0, 0};
             bool ok = true, pre0 = false;   // pre0: this item's QK_0 was issued early
             for (int k = 0; ok; ++k) {
                 Geo g;
-                const int st = next_item(k, g);
+                const int st = next_item(k, g, Poll{});
                 if (st == 0) break;
                 if (st == 2) continue;
                 it_done(k);
@@ -430,8 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // S_t = Q_t K_0^T of this item.  S_t may still hold P_t of the previous
                 // item's last step: its PV was issued earlier, and runs first.
                 {
-                    const int s0 = gkv % KV_STAGES;
-                    if (!mbar_wait(&k_full[s0], (gkv / KV_STAGES) & 1, p.status)) break;
+                    const int s0 = ring.stage(0);
+                    if (!mbar_wait(&k_full[s0], ring.phase(0), p.status)) break;
                     const uint32_t k_addr = opaque_u32(smem_u32(k_s + s0 * CF::TILE));
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
@@ -447,9 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     pre0 = false;
                 }
                 for (int j = 0; ok && j < n1; ++j) {
-                    const int gj = gkv + j;
-                    const int s = gj % KV_STAGES, s1 = (gj + 1) % KV_STAGES;
-                    if (!mbar_wait(&v_full[s], (gj / KV_STAGES) & 1, p.status)) { ok = false; break; }
+                    const int s = ring.stage(j), s1 = ring.stage(j + 1);
+                    if (!mbar_wait(&v_full[s], ring.phase(j), p.status)) { ok = false; break; }
                     const uint32_t v_addr = opaque_u32(smem_u32(v_s + s * CF::TILE));
                     const uint32_t k1_addr = opaque_u32(smem_u32(k_s + s1 * CF::TILE));
                     bool k1_ready = false;
@@ -457,19 +499,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int t = 0; t < 2; ++t) {
                         const int nt = t ? n1 : n0;
                         if (j >= nt) continue;
-                        // (packed: also when both tiles end with this step, PV_0 of which
-                        // was just issued -- two heads of the same rows always do)
-                        if (t == 1 && j == n1 - 1 && j >= (kPacked ? n0 - 1 : n0)) {
+                        // (Not packed: there both tiles mostly end with the same step, where
+                        // waiting for the next item's tiles held PV_1 up -- 16 x 1024, 32 / 8
+                        // heads: 476 against 517 TFLOP/s -- and issuing only if they had
+                        // landed gained nothing.)
+                        if (!kPacked && t == 1 && j == n1 - 1 && j >= n0) {
                             // Tile 0 is done with this item: S_0 of the next item now,
                             // while tile 1 runs its last step (S_0 held P_0 of this
                             // item's last tile-0 step, whose PV was issued before).
                             Geo gn2;
                             int kn = k + 1, st2;
-                            while ((st2 = next_item(kn, gn2)) == 2) ++kn;
+                            while ((st2 = next_item(kn, gn2, Poll{})) == 2) ++kn;
                             if (st2 == 1) {
                                 const int n0n = gn2.n0;
-                                const int gn = gkv + n1, sn = gn % KV_STAGES;
-                                if (!mbar_wait(&k_full[sn], (gn / KV_STAGES) & 1, p.status) ||
+                                Ring next = ring;
+                                next.advance(n1);
+                                const int sn = next.stage(0);
+                                if (!mbar_wait(&k_full[sn], next.phase(0), p.status) ||
                                     !mbar_wait(&q_full[0], (li + 1) & 1, p.status)) {
                                     ok = false;
                                     break;
@@ -498,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (t == 1) tc_commit(&v_empty[s]);
                         if (j + 1 < nt) {
                             if (!k1_ready) {
-                                if (!mbar_wait(&k_full[s1], ((gj + 1) / KV_STAGES) & 1, p.status)) {
+                                if (!mbar_wait(&k_full[s1], ring.phase(j + 1), p.status)) {
                                     ok = false;
                                     break;
                                 }
@@ -515,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                gkv += n1;
+                ring.advance(n1);
                 c[0] += n0;
                 c[1] += n1;
                 ++li;
@@ -525,20 +571,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (kPacked && warp == 2) {
         // rows of V past the sequence's end: zeroed in shared memory
-        int gkv = 0, fixed[KV_STAGES] = {};   // tiles before this item; v_raw phases used
+        int fixed[KV_STAGES] = {};   // v_raw phases used
         for (int k = 0;; ++k) {
             Geo g;
-            const int st = __all_sync(0xffffffffu, next_item(k, g) == 1);
+            const int st = __all_sync(0xffffffffu, next_item(k, g, Sleep{}) == 1);
             if (!st) break;
             __syncwarp();
             if (lane == 0) it_done(k);
             const int valid = g.S_kv - (g.n1 - 1) * BKV;   // of the last tile
             if (valid < BKV) {
-                const int s = (gkv + g.n1 - 1) % KV_STAGES;
+                const int s = (g.n1 - 1) % KV_STAGES;
                 bool ok = false;
 #pragma unroll
                 for (int i = 0; i < KV_STAGES; ++i)
-                    if (i == s) ok = mbar_wait_warp(&v_raw[i], fixed[i]++ & 1, p.status);
+                    if (i == s) ok = mbar_wait_warp<true>(&v_raw[i], fixed[i]++ & 1, p.status);
                 if (!ok) break;
                 for (int i = max(valid, 0) * 8 + lane; i < BKV * 8; i += 32)
 #pragma unroll
@@ -549,26 +595,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[s]);
             }
-            gkv += g.n1;
         }
     } else if (kPacked && warp == 3) {
-        // draws items ahead of the other warps: the first of each CTA by its index, the
-        // rest from the counter
+        // draws items ahead of the other warps
         const int group = p.Hq / p.Hkv;
-        const int total = p.plan.first[0][p.plan.B];
+        VarlenDraw draw(p.plan, 0, [&](const VarlenSeq& s) { return varlen_fwd_pairs(s.q_len, group) * p.Hkv; },
+                        p.status);
         for (int k = 0;; ++k) {
-            if (k >= 2 && !mbar_wait_warp(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) break;
-            int item = (int)blockIdx.x;
-            if (k > 0) {
-                if (lane == 0) item = (int)gridDim.x + atomicAdd(&p.plan.next[0], 1);
-                item = __shfl_sync(0xffffffffu, item, 0);
-            }
+            if (k >= 2 && !mbar_wait_warp<true>(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) break;
+            const int item = draw.next(k);
             PackedItem it = {};
-            if (item < total) {
-                const int r = varlen_find(p.plan.first[0], p.plan.B, item);
-                const VarlenSeq sq = p.plan.seqs[r];
+            if (item < draw.total) {
+                VarlenSeq sq;
+                const int w = draw.find(item, sq);   // number within its sequence
                 const int pairs = varlen_fwd_pairs(sq.q_len, group);
-                const int w = item - p.plan.first[0][r];
                 const int tiles = varlen_tiles(sq.q_len);
                 const int pair = pairs - 1 - w % pairs;   // most keys first
                 it.kv_head = w / pairs;
@@ -599,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_arrive(&it_full[k & 1]);
             }
             __syncwarp();
-            if (item >= total) break;
+            if (item >= draw.total) break;
         }
     }
     } else {
@@ -616,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int it = 0; ok; ++it) {
         Geo g;
-        int st_item = next_item(it, g);
+        int st_item = next_item(it, g, Poll{});
         if constexpr (kPacked) st_item = __all_sync(0xffffffffu, st_item == 1);
         if (st_item == 0) break;
         if (st_item == 2) continue;
@@ -625,7 +665,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int qi = q0 + r;
         const int nt = t ? g.n1 : g.n0;
         int vis_hi = p.causal ? min(S_kv - 1, qi + coff) : S_kv - 1;
-        if (kPacked && qi >= g.S_q) vis_hi = -1;   // rows of the next sequence
+        bool row_ok = qi < g.S_q;
+        if (kPacked && !row_ok) vis_hi = -1;   // rows of the next sequence
         float m_run = -INFINITY, l_run = 0.0f;
         for (int j = 0; j < nt; ++j) {
             if (!mbar_wait_warp(&s_full[t], (c_t + j) & 1, p.status)) { ok = false; break; }
@@ -714,18 +755,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) {
             tc_fence_after();
             const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-            const bool row_ok = qi < g.S_q;
             const float lse_v =
                 l_run > 0.0f ? (m_run + lg2_approx(l_run)) * 0.69314718055994531f : -INFINITY;
             if constexpr (!kAllGather) {
-                const int head = t ? g.head[1] : g.head[0];
-                const int64_t o_off =
-                    kPacked ? (int64_t)(g.q_tok + (row_ok ? qi : 0)) * p.o_tok + head * p.o_head
-                            : ((int64_t)bh * p.S_q + (row_ok ? qi : 0)) * D;
+                // packed: where the row goes is read here, not kept over the K/V tiles -- their
+                // loop has no register to spare
+                int64_t o_off, l_off;
+                if constexpr (kPacked) {
+                    const volatile PackedItem& item = items[it & 1];
+                    const int row = item.row0[t] + r, tok = item.q_tok + row, head = item.head[t];
+                    row_ok = row < item.q_len;
+                    o_off = (int64_t)(row_ok ? tok : 0) * p.o_tok + head * p.o_head;
+                    l_off = (int64_t)head * p.total_q + tok;
+                } else {
+                    o_off = ((int64_t)bh * p.S_q + (row_ok ? qi : 0)) * D;
+                    l_off = (int64_t)bh * p.S_q + qi;
+                }
                 __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.O) + o_off;
                 __syncwarp();
                 // all of O_t into registers (one wait), then O_t is free for the next
                 // item's first PV while this warp normalises and stores
+                if constexpr (kPacked) {
+                    // normalised and packed 32 columns at a time: with all of O_t in registers
+                    // the loop over the K/V tiles spills
+                    uint4 w[D / 8];
+#pragma unroll
+                    for (int oc = 0; oc < D / 32; ++oc) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(lane_base + o_col + oc * 32, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint4& x = w[(oc * 32 + e) / 8];
+                            x.x = f32x2_to_bf16x2(__uint_as_float(o[e]) * inv_l, __uint_as_float(o[e + 1]) * inv_l);
+                            x.y = f32x2_to_bf16x2(__uint_as_float(o[e + 2]) * inv_l, __uint_as_float(o[e + 3]) * inv_l);
+                            x.z = f32x2_to_bf16x2(__uint_as_float(o[e + 4]) * inv_l, __uint_as_float(o[e + 5]) * inv_l);
+                            x.w = f32x2_to_bf16x2(__uint_as_float(o[e + 6]) * inv_l, __uint_as_float(o[e + 7]) * inv_l);
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&o_free[t]);
+                    if (row_ok) {
+#pragma unroll
+                        for (int e = 0; e < D / 8; ++e) reinterpret_cast<uint4*>(orow)[e] = w[e];
+                    }
+                } else {
                 uint32_t o[D / 32][32];
 #pragma unroll
                 for (int oc = 0; oc < D / 32; ++oc)
@@ -747,9 +822,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             *reinterpret_cast<uint4*>(orow + oc * 32 + e) = w;
                         }
                 }
-                if (row_ok && p.lse)
-                    p.lse[kPacked ? (int64_t)head * p.total_q + g.q_tok + qi
-                                  : (int64_t)bh * p.S_q + qi] = lse_v;
+                }
+                if (row_ok && p.lse) p.lse[l_off] = lse_v;
             } else {
                 // stage this warp's 32 rows (D * 2 bytes each, 16-byte slots swizzled by
                 // row) in the tile's Q buffer: every MMA that read it has completed
@@ -948,14 +1022,13 @@ int launch_packed(const PackedArgs& a, cudaStream_t st) {
     p.o_tok = a.strides[6];
     p.o_head = a.strides[7];
     p.total_q = a.total_q;
-    p.plan = varlen_plan_at(a.ws, a.B);
-    if ((rc = varlen_make_plan(p.plan, a.cu_q, a.cu_kv, a.total_q, a.total_kv, a.Hq, a.Hkv, false, st)))
-        return rc;
+    // no more CTAs than there can be items
+    const int64_t most = ((int64_t)a.total_q / BQ + a.B) * a.Hq;
+    p.plan = {a.ws, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
+    if ((rc = varlen_make_plan(p.plan, (most + 1) / 2, a.Hq, a.Hkv, false, st))) return rc;
     auto kern = k_flash_fwd<D, false, false, true, true>;
     AMPB_CHECK_CUDA(
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FaCfg<D>::SMEM));
-    // no more CTAs than there can be items
-    const int64_t most = ((int64_t)a.total_q / BQ + a.B) * a.Hq;
     AMPB_CHECK_CUDA(launch_pdl(kern, dim3((unsigned)std::min<int64_t>(most, sm_count())),
                                dim3(kThreads), FaCfg<D>::SMEM, st, tq, tk, tv, p));
     return AMP_OK;

@@ -100,26 +100,23 @@ struct BwdItem {
     int S_q, S_kv, coff;
 };
 
-// Packed mode, warp 3: draws item after item of list `which` and publishes it.
+// Packed mode, warp 3: draws item after item of its list and publishes it.  It and warp 2
+// sleep in their waits: polling would take issue slots from the element-wise warps.
 template <bool kKeys>
 __device__ __forceinline__ void draw_items(const BwdParams& p, BwdItem* items, uint64_t* it_full,
                                            uint64_t* it_empty) {
-    constexpr int which = kKeys ? 0 : 1;
     const int lane = threadIdx.x & 31;
-    const int total = p.plan.first[which][p.plan.B];
+    VarlenDraw draw(p.plan, kKeys ? 0 : 1, [&](const VarlenSeq& s) {
+        return kKeys ? varlen_tiles(s.k_len) * p.Hkv : varlen_tiles(s.q_len) * p.Hq;
+    }, p.status);
     for (int k = 0;; ++k) {
-        if (k >= 2 && !mbar_wait_warp(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) return;
-        int item = (int)blockIdx.x;
-        if (k > 0) {
-            if (lane == 0) item = (int)gridDim.x + atomicAdd(&p.plan.next[which], 1);
-            item = __shfl_sync(0xffffffffu, item, 0);
-        }
+        if (k >= 2 && !mbar_wait_warp<true>(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) return;
+        const int item = draw.next(k);
         BwdItem it = {};
-        if (item < total) {
-            const int r = varlen_find(p.plan.first[which], p.plan.B, item);
-            const VarlenSeq sq = p.plan.seqs[r];
+        if (item < draw.total) {
+            VarlenSeq sq;
+            const int w = draw.find(item, sq);   // number within its sequence
             const int n = varlen_tiles(kKeys ? sq.k_len : sq.q_len);
-            const int w = item - p.plan.first[which][r];
             it.live = 1;
             it.head = w / n;
             // under a causal mask the first keys and the last queries have the most steps
@@ -135,15 +132,16 @@ __device__ __forceinline__ void draw_items(const BwdParams& p, BwdItem* items, u
             mbar_arrive(&it_full[k & 1]);
         }
         __syncwarp();
-        if (item >= total) return;
+        if (item >= draw.total) return;
     }
 }
 
 // Reads the k-th published item; false at the end (or when a wait ran out).
+template <bool kSleep = false>
 __device__ __forceinline__ bool read_item(int k, const BwdItem* items, uint64_t* it_full,
                                           int* status, BwdItem& it) {
-    if (!mbar_wait(&it_full[k & 1], (k >> 1) & 1, status)) return false;
-    const volatile BwdItem& src = items[k & 1];
+    if (!mbar_wait<kSleep>(&it_full[k & 1], (k >> 1) & 1, status)) return false;
+    const BwdItem& src = items[k & 1];
     it.live = src.live;
     it.b = 0;
     it.head = src.head;
@@ -161,7 +159,7 @@ __device__ __forceinline__ bool read_item(int k, const BwdItem* items, uint64_t*
 __device__ __forceinline__ bool zero_tail(uint64_t* raw, uint32_t parity, uint64_t* full,
                                           uint8_t* tile0, uint8_t* tile1, int slabs, int valid,
                                           int* status) {
-    if (!mbar_wait_warp(raw, parity, status)) return false;
+    if (!mbar_wait_warp<true>(raw, parity, status)) return false;
     const int lane = threadIdx.x & 31;
     for (int i = valid * 8 + lane; i < BT * 8; i += 32)
         for (int sl = 0; sl < slabs; ++sl) {
@@ -546,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int k = 0; ok; ++k) {
             BwdItem it;
-            const bool any = __all_sync(0xffffffffu, read_item(k, items, it_full, p.status, it));
+            const bool any = __all_sync(0xffffffffu, read_item<true>(k, items, it_full, p.status, it));
             if (!any) break;
             __syncwarp();
             if (lane == 0) it_done(k);
@@ -976,7 +974,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int k = 0; ok; ++k) {
             BwdItem it;
-            const bool any = __all_sync(0xffffffffu, read_item(k, items, it_full, p.status, it));
+            const bool any = __all_sync(0xffffffffu, read_item<true>(k, items, it_full, p.status, it));
             if (!any) break;
             __syncwarp();
             if (lane == 0) it_done(k);
@@ -1219,12 +1217,14 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
     p.dk_head = s[13];
     p.dv_tok = s[14];
     p.dv_head = s[15];
-    p.plan = varlen_plan_at(a.ws, a.B);
+    p.plan = {a.ws, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
     float* delta = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) +
                                             (varlen_plan_bytes(a.B) + 15) / 16 * 16);
     p.delta = delta;
-    if ((rc = varlen_make_plan(p.plan, a.cu_q, a.cu_kv, a.total_q, a.total_kv, a.Hq, a.Hkv, true, st)))
-        return rc;
+    // no more CTAs than there can be items
+    const int64_t most_kv = ((int64_t)a.total_kv / BT + a.B) * a.Hkv;
+    const int64_t most_q = ((int64_t)a.total_q / BT + a.B) * a.Hq;
+    if ((rc = varlen_make_plan(p.plan, std::max(most_kv, most_q), a.Hq, a.Hkv, true, st))) return rc;
     const int64_t rows = (int64_t)a.total_q * a.Hq;
     if (rows > 0) {
         const int64_t per_block = 8 * (32 / (D / 8)) * kDeltaLoads;
@@ -1239,17 +1239,14 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, CF::SMEM_KV));
     AMPB_CHECK_CUDA(cudaFuncSetAttribute(k_fa_bwd_dq<D, true>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, CF::SMEM_Q));
-    // no more CTAs than there can be items
     if (a.total_kv > 0) {
-        const int64_t most = ((int64_t)a.total_kv / BT + a.B) * a.Hkv;
         AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_dkdv<D, true>,
-                                   dim3((unsigned)std::min<int64_t>(most, sm_count())),
+                                   dim3((unsigned)std::min<int64_t>(most_kv, sm_count())),
                                    dim3(kThreads), CF::SMEM_KV, st, tq, tk, tv, to, p));
     }
     if (a.total_q > 0) {
-        const int64_t most = ((int64_t)a.total_q / BT + a.B) * a.Hq;
         AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_dq<D, true>,
-                                   dim3((unsigned)std::min<int64_t>(most, sm_count())),
+                                   dim3((unsigned)std::min<int64_t>(most_q, sm_count())),
                                    dim3(kThreads), CF::SMEM_Q, st, tq, tk, tv, to, p));
     }
     return AMP_OK;

@@ -14,6 +14,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "tc_common.cuh"
+
 namespace ampb {
 
 struct VarlenSeq {
@@ -30,32 +32,41 @@ __host__ __device__ __forceinline__ int varlen_fwd_pairs(int q_len, int group) {
     return (varlen_tiles(q_len) * group + 1) / 2;
 }
 
-// The lists, in the caller's workspace.
-struct VarlenPlan {
-    int* next;            // [2] items drawn so far beyond the first of each CTA
-    VarlenSeq* seqs;      // [B] longest first
-    int* first[2];        // [B + 1] items before sequence r: list 0 (forward or dK/dV), list 1 (dQ)
-    int B;
-};
-
+// The lists in the caller's workspace:
+//   next   int [16]     items drawn beyond the first of each CTA, one count a list
+//   seqs   VarlenSeq [B], longest first
+//   first  int [B + 1]  items before sequence r, for list 0 (forward or dK/dV) and 1 (dQ)
 inline size_t varlen_plan_bytes(int B) {
     return 64 + (size_t)B * sizeof(VarlenSeq) + 2 * ((size_t)B + 1) * sizeof(int);
 }
 
-inline VarlenPlan varlen_plan_at(void* ws, int B) {
-    uint8_t* p = static_cast<uint8_t*>(ws);
-    VarlenPlan pl;
-    pl.next = reinterpret_cast<int*>(p);
-    pl.seqs = reinterpret_cast<VarlenSeq*>(p + 64);
-    pl.first[0] = reinterpret_cast<int*>(pl.seqs + B);
-    pl.first[1] = pl.first[0] + B + 1;
-    pl.B = B;
-    return pl;
-}
+struct VarlenPlan {
+    void* ws;                        // the lists, or null: no plan kernel (VarlenDraw)
+    const int *cu_q, *cu_kv;         // the offsets themselves
+    int B, total_q, total_kv;
+    __device__ int* next() const { return static_cast<int*>(ws); }
+    __device__ VarlenSeq* seqs() const {
+        return reinterpret_cast<VarlenSeq*>(static_cast<uint8_t*>(ws) + 64);
+    }
+    __device__ int* first(int list) const { return reinterpret_cast<int*>(seqs() + B) + list * (B + 1); }
 
-// Enqueues the plan kernel; `backward` selects which lists it fills.
-int varlen_make_plan(const VarlenPlan& plan, const int* cu_q, const int* cu_kv, int total_q,
-                     int total_kv, int Hq, int Hkv, bool backward, cudaStream_t st);
+    // Sequence b.  One whose bounds are not within its tensor, in order, counts as empty.
+    __device__ __forceinline__ VarlenSeq load(int b, int* status) const {
+        const int q0 = cu_q[b], q1 = cu_q[b + 1], k0 = cu_kv[b], k1 = cu_kv[b + 1];
+        const bool ok = q0 >= 0 && q1 >= q0 && q1 <= total_q && k0 >= 0 && k1 >= k0 && k1 <= total_kv;
+        if (!ok) {
+            status[kStatusBadIndexInt] = AMP_DEV_ERR_BAD_INDEX;
+            return {0, 0, 0, 0};
+        }
+        return {q0, q1 - q0, k0, k1 - k0};
+    }
+};
+
+// Enqueues the plan kernel (`backward` selects which lists it fills), or, for few items,
+// sets plan.ws to null and leaves the plan to each CTA.  most_items: the most that there
+// can be, which is all that the host knows.
+int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward,
+                     cudaStream_t st);
 
 // Warp-wide (all lanes call it): the sequence r whose items hold `item`, i.e. the
 // last r with first[r] <= item, where first[] ascends and first[0] <= item < first[B];
@@ -74,5 +85,72 @@ __device__ __forceinline__ int varlen_find(const int* first, int B, int item) {
     }
     return lo;
 }
+
+// How a CTA's drawing warp gets its items.  With a plan in the workspace: from the
+// lists, the first by the CTA's index and the rest from the counter.  Without one (few
+// items, at most 32 sequences): lane r holds the r-th longest sequence, and the items
+// are dealt out forth and back, so that a CTA whose first was long gets a short one.
+// That saves a small call the plan's launch.
+struct VarlenDraw {
+    const VarlenPlan& plan;
+    int list, total;
+    VarlenSeq mine;
+    int first;
+
+    template <typename F>
+    __device__ __forceinline__ VarlenDraw(const VarlenPlan& p, int list_, F items, int* status)
+        : plan(p), list(list_), mine{0, 0, 0, 0}, first(0) {
+        if (plan.ws) {
+            total = plan.first(list)[plan.B];
+            return;
+        }
+        const int lane = threadIdx.x & 31;
+        VarlenSeq s = {0, 0, 0, 0};
+        if (lane < plan.B) s = plan.load(lane, status);
+        const int key = s.q_len > s.k_len ? s.q_len : s.k_len;
+        int rank = 0, from = 0;
+        for (int i = 0; i < 32; ++i) {
+            const int other = __shfl_sync(0xffffffffu, key, i);
+            rank += other > key || (other == key && i < lane);
+        }
+        for (int i = 0; i < 32; ++i)
+            if (__shfl_sync(0xffffffffu, rank, i) == lane) from = i;
+        mine.q_off = __shfl_sync(0xffffffffu, s.q_off, from);
+        mine.q_len = __shfl_sync(0xffffffffu, s.q_len, from);
+        mine.k_off = __shfl_sync(0xffffffffu, s.k_off, from);
+        mine.k_len = __shfl_sync(0xffffffffu, s.k_len, from);
+        const int n = items(mine);
+        int end = n;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += t;
+        }
+        first = end - n;
+        total = __shfl_sync(0xffffffffu, end, 31);
+    }
+    // the CTA's k-th item, k = 0, 1, ...; at or past `total`: no more
+    __device__ __forceinline__ int next(int k) const {
+        const int grid = (int)gridDim.x, cta = (int)blockIdx.x;
+        if (!plan.ws) return k * grid + (k & 1 ? grid - 1 - cta : cta);
+        if (k == 0) return cta;
+        int item = 0;
+        if ((threadIdx.x & 31) == 0) item = grid + atomicAdd(plan.next() + list, 1);
+        return __shfl_sync(0xffffffffu, item, 0);
+    }
+    // the sequence of an item, and the item's number within it
+    __device__ __forceinline__ int find(int item, VarlenSeq& s) const {
+        if (plan.ws) {
+            const int r = varlen_find(plan.first(list), plan.B, item);
+            s = plan.seqs()[r];
+            return item - plan.first(list)[r];
+        }
+        const int r = __popc(__ballot_sync(0xffffffffu, first <= item)) - 1;
+        s.q_off = __shfl_sync(0xffffffffu, mine.q_off, r);
+        s.q_len = __shfl_sync(0xffffffffu, mine.q_len, r);
+        s.k_off = __shfl_sync(0xffffffffu, mine.k_off, r);
+        s.k_len = __shfl_sync(0xffffffffu, mine.k_len, r);
+        return item - __shfl_sync(0xffffffffu, first, r);
+    }
+};
 
 }  // namespace ampb

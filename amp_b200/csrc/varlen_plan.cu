@@ -27,30 +27,17 @@ __device__ __forceinline__ int length_bucket(int len) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-    k_varlen_plan(VarlenPlan pl, const int* __restrict__ cu_q, const int* __restrict__ cu_kv,
-                  int total_q, int total_kv, int Hq, int Hkv, int backward, int* status) {
+    k_varlen_plan(VarlenPlan pl, int Hq, int Hkv, int backward, int* status) {
     __shared__ int at[kBuckets];
     __shared__ int part[32];
     const int tid = threadIdx.x;
     at[tid] = 0;
     pdl_wait();
     pdl_trigger();   // the attention kernel's CTAs set up meanwhile
-    if (tid < 2) pl.next[tid] = 0;
+    if (tid < 2) pl.next()[tid] = 0;
     __syncthreads();
-    // a sequence whose bounds are not within its tensor, in order, counts as empty
-    auto load = [&](int b) {
-        VarlenSeq s;
-        const int q0 = cu_q[b], q1 = cu_q[b + 1], k0 = cu_kv[b], k1 = cu_kv[b + 1];
-        const bool ok = q0 >= 0 && q1 >= q0 && q1 <= total_q && k0 >= 0 && k1 >= k0 && k1 <= total_kv;
-        s.q_off = ok ? q0 : 0;
-        s.q_len = ok ? q1 - q0 : 0;
-        s.k_off = ok ? k0 : 0;
-        s.k_len = ok ? k1 - k0 : 0;
-        if (!ok) status[kStatusBadIndexInt] = AMP_DEV_ERR_BAD_INDEX;
-        return s;
-    };
     for (int b = tid; b < pl.B; b += kPlanThreads) {
-        const VarlenSeq s = load(b);
+        const VarlenSeq s = pl.load(b, status);
         atomicAdd(&at[length_bucket(max(s.q_len, s.k_len))], 1);
     }
     __syncthreads();
@@ -59,8 +46,8 @@ __global__ void __launch_bounds__(kPlanThreads)
     at[tid] = end - mine;
     __syncthreads();
     for (int b = tid; b < pl.B; b += kPlanThreads) {
-        const VarlenSeq s = load(b);
-        pl.seqs[atomicAdd(&at[length_bucket(max(s.q_len, s.k_len))], 1)] = s;
+        const VarlenSeq s = pl.load(b, status);
+        pl.seqs()[atomicAdd(&at[length_bucket(max(s.q_len, s.k_len))], 1)] = s;
     }
     __syncthreads();
     const int group = Hq / Hkv;
@@ -69,36 +56,43 @@ __global__ void __launch_bounds__(kPlanThreads)
         const int r = r0 + tid;
         int n0 = 0, n1 = 0;
         if (r < pl.B) {
-            const VarlenSeq s = pl.seqs[r];
+            const VarlenSeq s = pl.seqs()[r];
             n0 = backward ? varlen_tiles(s.k_len) * Hkv : varlen_fwd_pairs(s.q_len, group) * Hkv;
             n1 = backward ? varlen_tiles(s.q_len) * Hq : 0;
         }
         const int e0 = carry0 + block_scan(n0, part);
         const int last0 = part[31];
-        if (r < pl.B) pl.first[0][r] = e0 - n0;
+        if (r < pl.B) pl.first(0)[r] = e0 - n0;
         carry0 += last0;
         if (backward) {
             const int e1 = carry1 + block_scan(n1, part);
             const int last1 = part[31];
-            if (r < pl.B) pl.first[1][r] = e1 - n1;
+            if (r < pl.B) pl.first(1)[r] = e1 - n1;
             carry1 += last1;
         }
     }
     if (tid == 0) {
-        pl.first[0][pl.B] = carry0;
-        pl.first[1][pl.B] = carry1;
+        pl.first(0)[pl.B] = carry0;
+        pl.first(1)[pl.B] = carry1;
     }
 }
 
 }  // namespace
 
-int varlen_make_plan(const VarlenPlan& plan, const int* cu_q, const int* cu_kv, int total_q,
-                     int total_kv, int Hq, int Hkv, bool backward, cudaStream_t st) {
+int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward,
+                     cudaStream_t st) {
+    // 32 sequences fit a warp, and dealing four items a CTA out in turn loses less than the
+    // launch costs: forward of 8 prompts of 22 to 200 tokens 22.5 -> 20.5 us, forward and
+    // backward of 17 sequences of up to 700 tokens 84.0 -> 73.7 us.
+    if (plan.B <= 32 && most_items <= 4 * sm_count()) {
+        plan.ws = nullptr;
+        return AMP_OK;
+    }
     int* status = nullptr;
     int rc = device_status(&status);
     if (rc) return rc;
-    AMPB_CHECK_CUDA(launch_pdl(k_varlen_plan, dim3(1), dim3(kPlanThreads), 0, st, plan, cu_q, cu_kv,
-                               total_q, total_kv, Hq, Hkv, backward ? 1 : 0, status));
+    AMPB_CHECK_CUDA(launch_pdl(k_varlen_plan, dim3(1), dim3(kPlanThreads), 0, st, plan, Hq, Hkv,
+                               backward ? 1 : 0, status));
     return AMP_OK;
 }
 
