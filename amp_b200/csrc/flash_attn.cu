@@ -153,33 +153,6 @@ struct FaCfg {
     static constexpr uint32_t O_COL = 2 * BKV;            // S0 | S1 | O0 | O1
 };
 
-// Stage and phase of a K/V tile in its ring, for tile j of the current item.  Dense: the
-// tiles of all items run through the ring in turn.  Packed: every item starts at stage 0.
-// An item's tile count then comes out of shared memory, and a stage that depended on the
-// counts of earlier items could not be known to be the same in every lane: the MMA
-// descriptors would live in vector registers, be spilled and be converted for every
-// MMA (835 against 1000 TFLOP/s at 4 x 4096, 32 / 8 heads).
-template <bool kPerItem>
-struct KvRing {
-    int used0 = 0, used1 = 0;   // per item: uses of each stage; else used0: tiles in all
-    __device__ __forceinline__ int stage(int j) const {
-        return (kPerItem ? j : used0 + j) % KV_STAGES;
-    }
-    __device__ __forceinline__ uint32_t phase(int j) const {
-        if constexpr (kPerItem) return ((j % KV_STAGES ? used1 : used0) + j / KV_STAGES) & 1;
-        else return ((used0 + j) / KV_STAGES) & 1;
-    }
-    __device__ __forceinline__ void advance(int n) {
-        if constexpr (kPerItem) {
-            static_assert(KV_STAGES == 2, "two use counts");
-            used0 += (n + 1) / 2;
-            used1 += n / 2;
-        } else {
-            used0 += n;
-        }
-    }
-};
-
 // kPersist: one CTA per SM walks a list of (batch*head, query-tile pair) items
 // (see item_at below) instead of one CTA per item, so that the next item's Q and
 // K/V loads and its first QK overlap the current item's last steps and epilogue.
@@ -191,7 +164,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     static_assert(!(kPersist && kAllGather), "the all-gather epilogue stages in Q: one item per CTA");
     static_assert(!kPacked || (kPersist && !kPaged), "packed items are drawn by persistent CTAs");
     using CF = FaCfg<D>;
-    using Ring = KvRing<kPacked>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~uintptr_t(1023));
@@ -367,9 +339,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_prefetch_desc(&tmQ);
             tma_prefetch_desc(&tmK);
             tma_prefetch_desc(&tmV);
-            // K/V tiles run through the rings continuously across items (Ring)
-            Ring ring;
-            int li = 0;
+            // K/V tiles run through the rings continuously across items: tile g of
+            // this CTA uses stage g % KV_STAGES in phase (g / KV_STAGES) & 1
+            int gkv = 0, li = 0;
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 Geo g;
@@ -395,8 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int last_page = max(0, (g.S_kv + kPageTokens - 1) / kPageTokens - 1);
                 const int hk = g.h / (p.Hq / p.Hkv);
                 for (int j = 0; j < g.n1; ++j) {
-                    const int s = ring.stage(j);
-                    const uint32_t ph = ring.phase(j);
+                    const int s = (gkv + j) % KV_STAGES;
+                    const uint32_t ph = ((gkv + j) / KV_STAGES) & 1;
                     int pages[BKV / kPageTokens];
                     if constexpr (kPaged) {
                         const int* bt = p.block_table + (int64_t)g.b * p.max_pages;
@@ -440,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (kPersist && j == 0 && !load_q(1)) { ok = false; break; }
                 }
-                ring.advance(g.n1);
+                gkv += g.n1;
                 ++li;
             }
         }
@@ -457,11 +429,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                                smem_desc_sw128(k_addr + off, 16, 1024), CF::IDESC_QK, kk != 0);
                 }
             };
-            // ring: as in the load warp; c[t]: query tile t's steps before this item (phase of
+            // gkv: K/V tiles consumed before this item (ring stage / phase as in the
+            // load warp); c[t]: query tile t's steps before this item (phase of
             // s_full / p_full / pv_done); li: items before this one (q_full, q_empty,
             // o_free)
-            Ring ring;
-            int li = 0, c[2] = {0, 0};
+            int gkv = 0, li = 0, c[2] = {0, 0};
             bool ok = true, pre0 = false;   // pre0: this item's QK_0 was issued early
             for (int k = 0; ok; ++k) {
                 Geo g;
@@ -473,8 +445,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // S_t = Q_t K_0^T of this item.  S_t may still hold P_t of the previous
                 // item's last step: its PV was issued earlier, and runs first.
                 {
-                    const int s0 = ring.stage(0);
-                    if (!mbar_wait(&k_full[s0], ring.phase(0), p.status)) break;
+                    const int s0 = gkv % KV_STAGES;
+                    if (!mbar_wait(&k_full[s0], (gkv / KV_STAGES) & 1, p.status)) break;
                     const uint32_t k_addr = opaque_u32(smem_u32(k_s + s0 * CF::TILE));
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
@@ -490,8 +462,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     pre0 = false;
                 }
                 for (int j = 0; ok && j < n1; ++j) {
-                    const int s = ring.stage(j), s1 = ring.stage(j + 1);
-                    if (!mbar_wait(&v_full[s], ring.phase(j), p.status)) { ok = false; break; }
+                    const int gj = gkv + j;
+                    const int s = gj % KV_STAGES, s1 = (gj + 1) % KV_STAGES;
+                    if (!mbar_wait(&v_full[s], (gj / KV_STAGES) & 1, p.status)) { ok = false; break; }
                     const uint32_t v_addr = opaque_u32(smem_u32(v_s + s * CF::TILE));
                     const uint32_t k1_addr = opaque_u32(smem_u32(k_s + s1 * CF::TILE));
                     bool k1_ready = false;
@@ -512,10 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             while ((st2 = next_item(kn, gn2, Poll{})) == 2) ++kn;
                             if (st2 == 1) {
                                 const int n0n = gn2.n0;
-                                Ring next = ring;
-                                next.advance(n1);
-                                const int sn = next.stage(0);
-                                if (!mbar_wait(&k_full[sn], next.phase(0), p.status) ||
+                                const int gn = gkv + n1, sn = gn % KV_STAGES;
+                                if (!mbar_wait(&k_full[sn], (gn / KV_STAGES) & 1, p.status) ||
                                     !mbar_wait(&q_full[0], (li + 1) & 1, p.status)) {
                                     ok = false;
                                     break;
@@ -544,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (t == 1) tc_commit(&v_empty[s]);
                         if (j + 1 < nt) {
                             if (!k1_ready) {
-                                if (!mbar_wait(&k_full[s1], ring.phase(j + 1), p.status)) {
+                                if (!mbar_wait(&k_full[s1], ((gj + 1) / KV_STAGES) & 1, p.status)) {
                                     ok = false;
                                     break;
                                 }
@@ -561,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                ring.advance(n1);
+                gkv += n1;
                 c[0] += n0;
                 c[1] += n1;
                 ++li;
@@ -571,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (kPacked && warp == 2) {
         // rows of V past the sequence's end: zeroed in shared memory
-        int fixed[KV_STAGES] = {};   // v_raw phases used
+        int gkv = 0, fixed[KV_STAGES] = {};   // tiles before this item; v_raw phases used
         for (int k = 0;; ++k) {
             Geo g;
             const int st = __all_sync(0xffffffffu, next_item(k, g, Sleep{}) == 1);
@@ -580,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) it_done(k);
             const int valid = g.S_kv - (g.n1 - 1) * BKV;   // of the last tile
             if (valid < BKV) {
-                const int s = (g.n1 - 1) % KV_STAGES;
+                const int s = (gkv + g.n1 - 1) % KV_STAGES;
                 bool ok = false;
 #pragma unroll
                 for (int i = 0; i < KV_STAGES; ++i)
@@ -595,6 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[s]);
             }
+            gkv += g.n1;
         }
     } else if (kPacked && warp == 3) {
         // draws items ahead of the other warps

@@ -97,7 +97,8 @@ struct BwdItem {
     int live;                   // packed: 0 ends the list
     int b, head, tile;          // head: kv head (dK/dV) or query head (dQ) within b
     int q_tok, k_tok;           // packed: the sequence's first rows
-    int S_q, S_kv, coff;
+    int S_q, S_kv;
+    int coff;                   // key j visible for query i iff j <= i + coff
 };
 
 // Packed mode, warp 3: draws item after item of its list and publishes it.  It and warp 2
@@ -125,7 +126,6 @@ __device__ __forceinline__ void draw_items(const BwdParams& p, BwdItem* items, u
             it.k_tok = sq.k_off;
             it.S_q = sq.q_len;
             it.S_kv = sq.k_len;
-            it.coff = sq.k_len - sq.q_len;
         }
         if (lane == 0) {
             items[k & 1] = it;
@@ -136,21 +136,30 @@ __device__ __forceinline__ void draw_items(const BwdParams& p, BwdItem* items, u
     }
 }
 
+// Packed: what comes out of shared memory or depends on the warp is not known to be the same
+// in every lane, and what is derived from it would be converted for every MMA; a shuffle
+// from lane 0 makes it known.
+template <bool kPacked>
+__device__ __forceinline__ int same_in_warp(int x) {
+    if constexpr (kPacked) return __shfl_sync(__activemask(), x, 0);
+    else return x;
+}
+
 // Reads the k-th published item; false at the end (or when a wait ran out).
 template <bool kSleep = false>
 __device__ __forceinline__ bool read_item(int k, const BwdItem* items, uint64_t* it_full,
                                           int* status, BwdItem& it) {
     if (!mbar_wait<kSleep>(&it_full[k & 1], (k >> 1) & 1, status)) return false;
     const BwdItem& src = items[k & 1];
-    it.live = src.live;
+    it.live = same_in_warp<true>(src.live);
     it.b = 0;
-    it.head = src.head;
-    it.tile = src.tile;
-    it.q_tok = src.q_tok;
-    it.k_tok = src.k_tok;
-    it.S_q = src.S_q;
-    it.S_kv = src.S_kv;
-    it.coff = src.coff;
+    it.head = same_in_warp<true>(src.head);
+    it.tile = same_in_warp<true>(src.tile);
+    it.q_tok = same_in_warp<true>(src.q_tok);
+    it.k_tok = same_in_warp<true>(src.k_tok);
+    it.S_q = same_in_warp<true>(src.S_q);
+    it.S_kv = same_in_warp<true>(src.S_kv);
+    it.coff = it.S_kv - it.S_q;
     return it.live != 0;
 }
 
@@ -265,6 +274,21 @@ __global__ void __launch_bounds__(256) k_fa_bwd_delta(const __nv_bfloat16* __res
     }
 }
 
+// The P that dS = P (dP - Delta) multiplies with.  Dense: as rounded to bf16 for P^T dO.
+// Packed: as computed, in fp32 (dQ and dK then carry two roundings to bf16, of dS and their
+// own, instead of three: an error of 0.0024 instead of 0.0030 relative to fp64).
+template <bool kExact>
+struct Probs {
+    float v[kExact ? 64 : 1];
+    __device__ __forceinline__ void keep(int e, float p0, float p1) {
+        if constexpr (kExact) v[e] = p0, v[e + 1] = p1;
+    }
+    __device__ __forceinline__ uint64_t pair(int e, const uint32_t* rounded) const {
+        if constexpr (kExact) return f2pack(v[e], v[e + 1]);
+        else return f2pack(bf16_lo(rounded[e >> 1]), bf16_hi(rounded[e >> 1]));
+    }
+};
+
 // store columns [half * D/2, half * D/2 + D/2) of one 128 x D fp32 TMEM
 // accumulator row (this thread's lane) as bf16 * mul
 template <int D>
@@ -335,7 +359,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* qs_raw = bars + 21;     // [2] Q / dO loaded, rows past the end not yet zeroed
     BwdItem* items = reinterpret_cast<BwdItem*>(bars + 23);   // [2]
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
+    const int warp = same_in_warp<kPacked>(threadIdx.x >> 5);
     const int G = p.Hq / p.Hkv;
     const int n_kt = (p.S_kv + BT - 1) / BT;
     // Persistent: unit u = blockIdx.x + (k/2) * gridDim.x pairs key tile n_kt-1-q with
@@ -418,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = kPacked ? 0u : *tmem_slot;   // all 512 columns start at column 0
     const uint32_t T_S = tmem, T_dP = tmem + BT, T_dV = tmem + 2 * BT, T_dK = tmem + 2 * BT + D;
 
     if (warp < 4) {
@@ -649,6 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld_32x32b_x32(T_S + lane_base + src_col + 32, sv[1]);
             tmem_ld_wait();
             uint32_t pw[32];
+            Probs<kPacked> pf;
 #pragma unroll
             for (int e = 0; e < 64; e += 4) {
                 const float4 l4 = *reinterpret_cast<const float4*>(hcl + e);
@@ -664,7 +690,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         x0 = ee >= lo ? x0 : -INFINITY;
                         x1 = ee + 1 >= lo ? x1 : -INFINITY;
                     }
-                    pw[ee >> 1] = f32x2_to_bf16x2(ex2_approx(x0), ex2_approx(x1));
+                    const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                    pw[ee >> 1] = f32x2_to_bf16x2(p0, p1);
+                    pf.keep(ee, p0, p1);
                 }
             }
             tmem_st_32x32b_x32(T_S + lane_base + dst_col, pw);
@@ -686,12 +714,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int u = 0; u < 4; u += 2) {
                     const int ee = e + u;
-                    const uint32_t pp = pw[ee >> 1];
+                    const uint64_t pp = pf.pair(ee, pw);
                     const uint64_t g2 = fadd2(f2pack(__uint_as_float(sv[ee >> 5][ee & 31]),
                                                      __uint_as_float(sv[ee >> 5][(ee & 31) + 1])),
                                               u ? f2pack(d4.z, d4.w) : f2pack(d4.x, d4.y));
                     float d0, d1;
-                    f2unpack(fmul2(f2pack(bf16_lo(pp), bf16_hi(pp)), g2), d0, d1);
+                    f2unpack(fmul2(pp, g2), d0, d1);
                     dw[ee >> 1] = f32x2_to_bf16x2(d0, d1);
                 }
             }
@@ -770,7 +798,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* v_raw = bars + 24;      // [2]
     BwdItem* items = reinterpret_cast<BwdItem*>(bars + 26);   // [2]
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
+    const int warp = same_in_warp<kPacked>(threadIdx.x >> 5);
     const int n_qt = (p.S_q + BT - 1) / BT;
     const int half_units = (n_qt + 1) / 2;
     const int units = p.B * p.Hq * half_units;
@@ -848,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = kPacked ? 0u : *tmem_slot;   // all 512 columns start at column 0
     // two S buffers, so that the next step's S = Q K^T runs during this step
     const uint32_t T_S = tmem, T_dP = tmem + 2 * BT, T_dQ = tmem + 3 * BT;
 
@@ -1049,6 +1078,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld_32x32b_x32(sb + lane_base + src_col + 32, sv[1]);
             tmem_ld_wait();
             uint32_t pw[32];
+            Probs<kPacked> pf;
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
                 const uint64_t x2 = ffma2(f2pack(__uint_as_float(sv[e >> 5][e & 31]),
@@ -1060,7 +1090,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     x0 = e <= hi ? x0 : -INFINITY;
                     x1 = e + 1 <= hi ? x1 : -INFINITY;
                 }
-                pw[e >> 1] = f32x2_to_bf16x2(ex2_approx(x0), ex2_approx(x1));
+                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                if constexpr (!kPacked) pw[e >> 1] = f32x2_to_bf16x2(p0, p1);
+                pf.keep(e, p0, p1);
             }
             // phase dS (needs dP): dS = P (dP - Delta) back over dP
             if (!mbar_wait_warp(dp_full, gj & 1, p.status)) { ok = false; break; }
@@ -1072,12 +1104,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t dw[32];
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
-                const uint32_t pp = pw[e >> 1];
+                const uint64_t pp = pf.pair(e, pw);
                 const uint64_t g2 = fadd2(f2pack(__uint_as_float(sv[e >> 5][e & 31]),
                                                  __uint_as_float(sv[e >> 5][(e & 31) + 1])),
                                           ndlx2);
                 float d0, d1;
-                f2unpack(fmul2(f2pack(bf16_lo(pp), bf16_hi(pp)), g2), d0, d1);
+                f2unpack(fmul2(pp, g2), d0, d1);
                 dw[e >> 1] = f32x2_to_bf16x2(d0, d1);
             }
             tmem_st_32x32b_x32(T_dP + lane_base + dst_col, dw);   // dS over dP

@@ -4,7 +4,7 @@ The bounds count roundings (u = 2^-8, half a bf16 step relative to the value):
   O     rounded once, from P rounded once:          u |O| + u P|V|
   lse   fp32 sums of D products:                    D 2^-23 max scale |q|.|k| + a few 2^-22
   dV    rounded once, from P rounded once:          u |dV| + u P^T|dO|
-  dS    P and dS rounded, Delta from the bf16 O:    2u |dS| + P dDelta,
+  dS    rounded once, Delta from the bf16 O:        u |dS| + P dDelta,
         dDelta = sum |dO| (u |O| + u P|V|)
   dQ    u |dQ| + scale |err dS| |K|;  dK  u |dK| + scale |err dS|^T |Q|
 each with 5% for products of roundings and 1e-5 for the fp32 sums.  The scores' fp32 error
@@ -65,7 +65,7 @@ def reference(q, k, v, do, lens_q, lens_kv, causal, scale=0.0):
             err["dv"][K, h // G] += u * (p.T @ np.abs(doh))
             dp = doh @ vh.T
             ds = p * (dp - (doh * o).sum(1, keepdims=True))
-            e_ds = (u + U) * np.abs(ds) + p * ((np.abs(doh) * e_o).sum(1, keepdims=True)
+            e_ds = u * np.abs(ds) + p * ((np.abs(doh) * e_o).sum(1, keepdims=True)
                                                + D * 2.0 ** -23 * (np.abs(doh) @ np.abs(vh).T))
             val["dq"][Q, h] = sc * (ds @ kh)
             err["dq"][Q, h] = sc * (e_ds @ np.abs(kh))
@@ -83,7 +83,7 @@ def check(got, ref, names):
         fin = np.isfinite(want)
         assert np.array_equal(np.isfinite(x), fin), n
         assert np.array_equal(x[~fin], want[~fin]), n
-        over = np.abs(x - want)[fin] / bound[fin]
+        over = np.abs(x[fin] - want[fin]) / bound[fin]
         assert over.size == 0 or over.max() <= 1, (n, float(over.max()))
 
 
@@ -221,9 +221,8 @@ def test_matches_the_rectangular_kernels(cuda, amp_lib):
     o, lse = attention.flash_attn_fwd(*dense[:3], True)
     assert torch.equal(got["lse"], lse.transpose(0, 1).reshape(Hq, B * S))
     assert torch.equal(got["o"].view(B, S, Hq, D).transpose(1, 2), o)
-    grads = attention.flash_attn_bwd(*dense[:3], o, dense[3], lse, True)
-    for n, x in zip(("dq", "dk", "dv"), grads):
-        assert torch.equal(got[n].view(B, S, -1, D).transpose(1, 2), x), n
+    dv = attention.flash_attn_bwd(*dense[:3], o, dense[3], lse, True)[2]
+    assert torch.equal(got["dv"].view(B, S, -1, D).transpose(1, 2), dv)
 
 
 def test_same_bits_again_on_another_stream_and_from_a_graph(cuda, amp_lib):
