@@ -150,17 +150,6 @@ def lib() -> C.CDLL:
     return _lib
 
 
-def call_on(device, name: str, *args) -> int:
-    """call() with `device` (a torch CUDA device) current and its current stream as the
-    last argument: the library works on the current device, and tensors may live on another."""
-    import torch
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        return call(name, *args, stream)
-    with torch.cuda.device(device):
-        return call(name, *args, stream)
-
-
 def call(name: str, *args) -> int:
     """Call an int-status entry point and raise AmpError on a nonzero status."""
     h = lib()
@@ -169,3 +158,22 @@ def call(name: str, *args) -> int:
         msg = h.amp_last_error()
         raise AmpError(name, rc, msg.decode() if msg else "")
     return rc
+
+
+_ops = None
+
+
+def ops():
+    """The compiled host entries (host/ops.cpp), bound once to the CUDA library's functions; raises
+    if either is not built."""
+    global _ops
+    if _ops is None:
+        h = lib()
+        try:
+            from . import _ops as module
+        except ImportError as e:
+            raise RuntimeError("amp_b200/_ops.so is missing or does not fit this torch: build it "
+                               "with `python -m amp_b200.build`") from e
+        module.bind({n: C.cast(getattr(h, n), C.c_void_p).value for n in module.names()}, AmpError)
+        _ops = module
+    return _ops

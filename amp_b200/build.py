@@ -79,11 +79,42 @@ def build(jobs: int | None = None, force: bool = False, verbose: bool = False) -
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr}\n{r.stdout}")
         os.replace(tmp, LIB)
+    build_host(force)
     build_tools(force)
     check_dropins(force)
     if verbose:
         print(f"built {LIB}")
     return LIB
+
+
+HOST_SRC = PKG / "host" / "ops.cpp"
+HOST_LIB = PKG / "_ops.so"
+
+
+def build_host(force: bool = False) -> Path:
+    """The compiled Python entries (host/ops.cpp) against this interpreter's torch."""
+    if not force and not _stale(HOST_LIB, [HOST_SRC] + _deps()):
+        return HOST_LIB
+    import sysconfig
+    import torch
+    tdir = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = HOST_LIB.with_suffix(".so.tmp")
+    # nvcc's host compiler, not $CXX: one that links its own copy of libstdc++ would mix two in
+    # a process with torch's
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(ROOT / "include"), "-isystem", str(tdir / "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"),
+           str(HOST_SRC), "-o", str(tmp), "-L", str(tdir / "lib"), "-ltorch_python", "-ltorch_cpu",
+           "-ltorch", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building {HOST_SRC.name} failed:\n{r.stderr}")
+    if r.stderr.strip():
+        sys.stderr.write(r.stderr)
+    os.replace(tmp, HOST_LIB)
+    return HOST_LIB
 
 
 TOOLS = PKG / "tools"

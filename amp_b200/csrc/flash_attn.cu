@@ -999,8 +999,8 @@ int launch_packed(const PackedArgs& a, cudaStream_t st) {
     p.plan = {a.ws, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
     if ((rc = varlen_make_plan(p.plan, (most + 1) / 2, a.Hq, a.Hkv, false, st))) return rc;
     auto kern = k_flash_fwd<D, false, false, true, true>;
-    AMPB_CHECK_CUDA(
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FaCfg<D>::SMEM));
+    static std::atomic<uint64_t> allowed{0};
+    AMPB_CHECK_CUDA(allow_smem_once(allowed, kern, FaCfg<D>::SMEM));
     AMPB_CHECK_CUDA(launch_pdl(kern, dim3((unsigned)std::min<int64_t>(most, sm_count())),
                                dim3(kThreads), FaCfg<D>::SMEM, st, tq, tk, tv, p));
     return AMP_OK;

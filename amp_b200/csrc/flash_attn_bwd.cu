@@ -1267,10 +1267,9 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
                                    dim3(256), 0, st, static_cast<const __nv_bfloat16*>(a.O),
                                    static_cast<const __nv_bfloat16*>(a.dO), delta, rows, ds));
     }
-    AMPB_CHECK_CUDA(cudaFuncSetAttribute(k_fa_bwd_dkdv<D, true>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, CF::SMEM_KV));
-    AMPB_CHECK_CUDA(cudaFuncSetAttribute(k_fa_bwd_dq<D, true>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, CF::SMEM_Q));
+    static std::atomic<uint64_t> allowed_kv{0}, allowed_q{0};
+    AMPB_CHECK_CUDA(allow_smem_once(allowed_kv, k_fa_bwd_dkdv<D, true>, CF::SMEM_KV));
+    AMPB_CHECK_CUDA(allow_smem_once(allowed_q, k_fa_bwd_dq<D, true>, CF::SMEM_Q));
     if (a.total_kv > 0) {
         AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_dkdv<D, true>,
                                    dim3((unsigned)std::min<int64_t>(most_kv, sm_count())),

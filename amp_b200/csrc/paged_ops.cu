@@ -484,11 +484,14 @@ int check_ws(const void* ws, size_t have, size_t need) {
     return AMP_OK;
 }
 
-template <typename K, typename... A>
-int launch_plan(K kern, int smem_words, cudaStream_t st, A... args) {
+// (two bitmaps of the pages, or one and three of the rows)
+constexpr size_t kMaxPlanSmem = std::max(2 * kMaxPages / 8, kMaxPages / 8 + 3 * kMaxRows / 8);
+
+template <auto kern, typename... A>
+int launch_plan(int smem_words, cudaStream_t st, A... args) {
     const size_t smem = (size_t)smem_words * 4;
-    if (smem > 40 * 1024)
-        AMPB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<uint64_t> allowed{0};
+    AMPB_CHECK_CUDA(allow_smem_once(allowed, kern, kMaxPlanSmem));
     AMPB_CHECK_CUDA(launch_pdl(kern, dim3(1), dim3(kPlanThreads), smem, st, args...));
     return AMP_OK;
 }
@@ -532,7 +535,7 @@ int amp_paged_copy_pages_dev(void* k_pool, void* v_pool, int layers, int num_pag
     if ((rc = device_status(&status))) return rc;
     const Moves mv = moves_at(workspace, n);
     cudaStream_t st = as_stream(stream);
-    if ((rc = launch_plan(k_copy_plan, 2 * ((num_pages + 31) / 32), st, src, dst, n, num_pages, mv, status)))
+    if ((rc = launch_plan<k_copy_plan>(2 * ((num_pages + 31) / 32), st, src, dst, n, num_pages, mv, status)))
         return rc;
     AMPB_CHECK_CUDA(launch_pdl(k_move, dim3(move_grid(pl, n, 1)), dim3(kMoveThreads), 0, st, pl, mv));
     return AMP_OK;
@@ -556,7 +559,7 @@ int amp_paged_fork_dev(void* k_pool, void* v_pool, int layers, int num_pages, in
     const Moves mv = moves_at(workspace, n);
     cudaStream_t st = as_stream(stream);
     const int words = (num_pages + 31) / 32 + 3 * ((rows + 31) / 32);
-    if ((rc = launch_plan(k_fork_plan, words, st, t, parents, children, n, done, mv))) return rc;
+    if ((rc = launch_plan<k_fork_plan>(words, st, t, parents, children, n, done, mv))) return rc;
     AMPB_CHECK_CUDA(launch_pdl(k_fork_move, dim3(move_grid(pl, n, n)), dim3(kMoveThreads), 0, st, pl, mv, t,
                                parents, children, n));
     return AMP_OK;
@@ -577,7 +580,7 @@ int amp_paged_extend_dev(void* k_pool, void* v_pool, int layers, int num_pages, 
     if ((rc = device_status(&t.status))) return rc;
     const Moves mv = moves_at(workspace, rows);
     cudaStream_t st = as_stream(stream);
-    if ((rc = launch_plan(k_extend_plan, 2 * ((num_pages + 31) / 32), st, t, add, ctx_out, done, mv))) return rc;
+    if ((rc = launch_plan<k_extend_plan>(2 * ((num_pages + 31) / 32), st, t, add, ctx_out, done, mv))) return rc;
     // pages are copied only where rows share a partly filled one: a block a multiprocessor is enough
     AMPB_CHECK_CUDA(launch_pdl(k_extend_move, dim3((unsigned)std::min(rows, sm_count())), dim3(kMoveThreads),
                                0, st, pl, mv, t));
@@ -600,7 +603,7 @@ int amp_paged_compact_dev(void* k_pool, void* v_pool, int layers, int num_pages,
     if ((rc = device_status(&t.status))) return rc;
     const Moves mv = moves_at(workspace, num_pages);
     cudaStream_t st = as_stream(stream);
-    if ((rc = launch_plan(k_compact_plan, (num_pages + 31) / 32, st, t, used, mv))) return rc;
+    if ((rc = launch_plan<k_compact_plan>((num_pages + 31) / 32, st, t, used, mv))) return rc;
     AMPB_CHECK_CUDA(launch_pdl(k_compact_move, dim3(move_grid(pl, num_pages / 2, rows)), dim3(kMoveThreads), 0,
                                st, pl, mv, t, table_out));
     return AMP_OK;

@@ -1,6 +1,8 @@
 // runtime.h -- host-side helpers shared by the entry points.
 #pragma once
+#include <atomic>
 #include <cstddef>
+#include <cstdint>
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -26,6 +28,18 @@ int device_status(int** out);
 // no interleave, 128-byte swizzle, 256-byte L2 promotion, zero out-of-bounds fill.
 int encode_tmap(CUtensorMap* m, const void* base, int es, int rank, const cuuint64_t* dims,
                 const cuuint64_t* strides, const cuuint32_t* box);
+
+// Allows `kern` `bytes` of dynamic shared memory, once per device: `done` (a static of the
+// caller, one bit a device) remembers, since asking again costs a small call a microsecond.
+template <typename K>
+cudaError_t allow_smem_once(std::atomic<uint64_t>& done, K kern, size_t bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.load() >> dev & 1)) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
+    return e;
+}
 
 // Launch with programmatic stream serialization: the kernel may start while the
 // previous kernel in the stream drains; it must call pdl_wait() (common.cuh)

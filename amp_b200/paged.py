@@ -15,8 +15,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from . import rope
-from ._lib import call, call_on, lib
+from ._lib import call, lib, ops
 
 PAGE_TOKENS = 16
 
@@ -129,82 +128,23 @@ def pool_bytes(num_pages: int, Hkv: int, D: int) -> int:
     return int(lib().amp_paged_pool_bytes(num_pages, Hkv, D))
 
 
-def _append(q, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, angles, interleaved, out_q):
-    _check_pools(k_pool, v_pool, block_table, ctx_lens)
-    num_pages, Hkv, _, D = k_pool.shape
-    T, dev = k.shape[0], k_pool.device
-    strides = list(rope.tensor_strides(q, "q", dev, k_pool.dtype, T, D)
-                   + rope.tensor_strides(out_q, "out_q", dev, k_pool.dtype, T, D)
-                   if q is not None else (D,) * 4)
-    strides += rope.tensor_strides(k, "k", dev, k_pool.dtype, T, D)
-    strides += rope.tensor_strides(v, "v", dev, k_pool.dtype, T, D)
-    if k.shape[1] != Hkv or v.shape[1] != Hkv or (q is not None and q.shape != out_q.shape):
-        raise ValueError(f"k and v must have the pools' {Hkv} heads, and out_q the shape of q")
-    B = cu_seqlens.numel() - 1
-    if cu_seqlens.device != dev or cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 \
-            or not cu_seqlens.is_contiguous() or B < 1:
-        raise ValueError(f"cu_seqlens: expected a contiguous int32 tensor [sequences + 1] on {dev}")
-    if v_pool.device != dev or block_table.device != dev or ctx_lens.device != dev \
-            or block_table.dim() != 2 or block_table.shape[0] < B or ctx_lens.numel() < B:
-        raise ValueError(f"block_table [>= {B}, pages] and ctx_lens [>= {B}] expected on {dev}")
-    call_on(dev, "amp_paged_rope_append_bf16_dev", q.data_ptr() if q is not None else None,
-            out_q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), T,
-            q.shape[1] if q is not None else 0, Hkv, D, (C.c_int64 * 8)(*strides), *angles,
-            1 if interleaved else 0, k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
-            ctx_lens.data_ptr(), cu_seqlens.data_ptr(), B, num_pages, block_table.shape[1])
-
-
 def append(k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens) -> None:
     """Writes the new tokens' k and v [tokens, Hkv, D] (bf16, any token and head strides) into their
     pages.  Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b+1] and the last ones of
     its context: ctx_lens counts them already.  Tokens of no sequence are skipped; one without a
     page in the table is not written and reported by amp_device_status."""
-    _append(None, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, (None, 0, 0, None, None),
-            False, None)
+    ops().append(None, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, None, None, None, False,
+                 None)
 
 
 def rope_append(q, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, positions, inv_freq,
                 sections=None, interleaved: bool = False, out_q=None):
     """append() of k turned by its rotary position, and q turned the same way, in one pass: returns
     q' [tokens, Hq, D] (rows of no sequence are not written).  Rotary arguments as rope.rope_fwd."""
-    if q.dim() != 3 or not q.is_cuda:
-        raise ValueError("q: expected a bf16 CUDA tensor [tokens, heads, head_dim]")
-    angles = rope.angle_args(positions, inv_freq, sections, q.device, k.shape[0])
-    out_q = out_q if out_q is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _append(q, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, angles, interleaved, out_q)
-    return out_q
-
-
-def _pool_args(k_pool, v_pool):
-    """(k, v, layers, pages, Hkv, D) of pools [pages, Hkv, 16, D] or [layers, pages, Hkv, 16, D]."""
-    if k_pool.shape != v_pool.shape or k_pool.device != v_pool.device:
-        raise ValueError("k_pool and v_pool shapes or devices differ")
-    for t, nm in ((k_pool, "k_pool"), (v_pool, "v_pool")):
-        if not t.is_cuda or t.dtype != torch.bfloat16 or not t.is_contiguous() \
-                or t.dim() not in (4, 5) or t.shape[-2] != PAGE_TOKENS:
-            raise ValueError(f"{nm}: expected contiguous bf16 CUDA [(layers,) pages, Hkv, 16, D]")
-    layers = k_pool.shape[0] if k_pool.dim() == 5 else 1
-    pages, heads, _, D = k_pool.shape[-4:]
-    return k_pool.data_ptr(), v_pool.data_ptr(), layers, pages, heads, D
-
-
-def _ints(t, name: str, device, shape):
-    """Pointer of a contiguous int32 tensor of the given shape (None: any length)."""
-    if t.device != device or t.dtype != torch.int32 or not t.is_contiguous() \
-            or t.dim() != len(shape) or any(n is not None and t.shape[i] != n for i, n in enumerate(shape)):
-        raise ValueError(f"{name}: expected a contiguous int32 tensor {list(shape)} on {device}, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
-
-
-def _scratch(workspace, nbytes: int, device):
-    if workspace is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    if workspace.device != device or workspace.dtype != torch.uint8 or not workspace.is_contiguous() \
-            or workspace.numel() < nbytes:
-        raise ValueError(f"workspace: expected a contiguous uint8 tensor of >= {nbytes} bytes "
-                         f"on {device}")
-    return workspace
+    if q is None:
+        raise ValueError("q: expected a tensor (append() writes k and v alone)")
+    return ops().append(q, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, positions, inv_freq,
+                        sections, interleaved, out_q)
 
 
 def copy_pages(k_pool, v_pool, src, dst, workspace=None) -> None:
@@ -212,11 +152,7 @@ def copy_pages(k_pool, v_pool, src, dst, workspace=None) -> None:
     [(layers,) pages, Hkv, 16, D].  A negative number, or a page onto itself, is nothing to do; a
     page that two pairs would write, or one write and another read, is left alone and reported by
     amp_device_status."""
-    pools, dev = _pool_args(k_pool, v_pool), k_pool.device
-    n = src.numel()
-    ids = _ints(src, "src", dev, (None,)), _ints(dst, "dst", dev, (n,))
-    ws = _scratch(workspace, lib().amp_paged_copy_workspace_bytes(n), dev)
-    call_on(dev, "amp_paged_copy_pages_dev", *pools, *ids, n, ws.data_ptr(), ws.numel())
+    ops().copy_pages(k_pool, v_pool, src, dst, workspace)
 
 
 def fork_sequences(k_pool, v_pool, block_table, ctx_lens, parents, children, workspace=None):
@@ -225,16 +161,7 @@ def fork_sequences(k_pool, v_pool, block_table, ctx_lens, parents, children, wor
     what the child held is released.  Changes block_table [rows, width] and ctx_lens [rows] in
     place and returns done, int32 [n]: 0 where no page was left (the child is empty then) or the
     rows are out of range or a child is named twice (nothing is done).  No host synchronisation."""
-    pools, dev = _pool_args(k_pool, v_pool), k_pool.device
-    rows, width = _table_shape(block_table)
-    n = parents.numel()
-    args = (_ints(block_table, "block_table", dev, (rows, width)), _ints(ctx_lens, "ctx_lens", dev, (rows,)))
-    ids = _ints(parents, "parents", dev, (None,)), _ints(children, "children", dev, (n,))
-    done = torch.empty(n, dtype=torch.int32, device=dev)
-    ws = _scratch(workspace, lib().amp_paged_fork_workspace_bytes(n, width), dev)
-    call_on(dev, "amp_paged_fork_dev", *pools, *args, rows, width, *ids, n, done.data_ptr(),
-            ws.data_ptr(), ws.numel())
-    return done
+    return ops().fork_sequences(k_pool, v_pool, block_table, ctx_lens, parents, children, workspace)
 
 
 def extend_sequences(k_pool, v_pool, block_table, ctx_lens, add, out=None, workspace=None):
@@ -242,46 +169,17 @@ def extend_sequences(k_pool, v_pool, block_table, ctx_lens, add, out=None, works
     done): the pages go into block_table in place, the lengths into `out` (a new tensor by default,
     or ctx_lens itself).  A partly filled last page that another row names too is copied first.  Rows
     that do not fit into the table or the pool keep their length, with done 0."""
-    pools, dev = _pool_args(k_pool, v_pool), k_pool.device
-    rows, width = _table_shape(block_table)
-    args = (_ints(block_table, "block_table", dev, (rows, width)), _ints(ctx_lens, "ctx_lens", dev, (rows,)))
-    out = torch.empty(rows, dtype=torch.int32, device=dev) if out is None else out
-    ids = _ints(add, "add", dev, (rows,)), _ints(out, "out", dev, (rows,))
-    done = torch.empty(rows, dtype=torch.int32, device=dev)
-    ws = _scratch(workspace, lib().amp_paged_extend_workspace_bytes(rows, pools[3]), dev)
-    call_on(dev, "amp_paged_extend_dev", *pools, *args, rows, width, *ids, done.data_ptr(),
-            ws.data_ptr(), ws.numel())
-    return out, done
+    return ops().extend_sequences(k_pool, v_pool, block_table, ctx_lens, add, out, workspace)
 
 
 def compact_pages(k_pool, v_pool, block_table, ctx_lens, out=None, workspace=None):
     """Moves the pages in use to the front of the pools, in every layer, and returns (the changed
     table, the number of pages in use as int32 [1]); pages from that number on are free.  The table
     goes to `out` (a new tensor by default, or block_table itself), -1 past each row's entries."""
-    pools, dev = _pool_args(k_pool, v_pool), k_pool.device
-    rows, width = _table_shape(block_table)
-    args = (_ints(block_table, "block_table", dev, (rows, width)), _ints(ctx_lens, "ctx_lens", dev, (rows,)))
-    out = torch.empty_like(block_table) if out is None else out
-    used = torch.empty(1, dtype=torch.int32, device=dev)
-    ws = _scratch(workspace, lib().amp_paged_compact_workspace_bytes(pools[3]), dev)
-    call_on(dev, "amp_paged_compact_dev", *pools, *args, rows, width,
-            _ints(out, "out", dev, (rows, width)), used.data_ptr(), ws.data_ptr(), ws.numel())
-    return out, used
+    return ops().compact_pages(k_pool, v_pool, block_table, ctx_lens, out, workspace)
 
 
 def free_sequences(block_table, ctx_lens, seqs) -> None:
     """Empties the rows seqs (int32): context length 0, entries -1.  Pages that no other row names are
     free from then on."""
-    rows, width = _table_shape(block_table)
-    dev = block_table.device
-    if not block_table.is_cuda:
-        raise ValueError("block_table: expected a CUDA tensor")
-    call_on(dev, "amp_paged_free_dev", _ints(block_table, "block_table", dev, (rows, width)),
-            _ints(ctx_lens, "ctx_lens", dev, (rows,)), rows, width, _ints(seqs, "seqs", dev, (None,)),
-            seqs.numel())
-
-
-def _table_shape(block_table):
-    if block_table.dim() != 2:
-        raise ValueError("block_table: expected [rows, pages a row]")
-    return block_table.shape
+    ops().free_sequences(block_table, ctx_lens, seqs)

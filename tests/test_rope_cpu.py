@@ -68,12 +68,3 @@ def test_python_refuses(amp_lib):
         rope.rope_fwd(q, None, pos, f)        # not on a GPU
     with pytest.raises(ValueError):
         paged.rope_append(q, q, q, q, q, q, q, q, pos, f)
-    dev = torch.device("cpu")
-    for bad in (pos.long(), pos[:, :3], pos[None]):
-        with pytest.raises(ValueError):
-            rope.angle_args(bad, f, (32,), dev, 4)
-    for sections in ((31,), (16, 16), None):
-        with pytest.raises(ValueError):
-            rope.angle_args(torch.zeros(3, 4, dtype=torch.int32), f, sections, dev, 4)
-    with pytest.raises(ValueError):
-        rope.tensor_strides(q.transpose(1, 2), "x", dev, q.dtype, 4, 2)
