@@ -768,7 +768,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     k_fa_bwd_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
                 const BwdParams p) {
-    pdl_wait();
+    // Packed: nothing here needs what the dK/dV pass writes, so a CTA starts as soon as one of
+    // that pass leaves its SM, and waits for the pass to be complete (the next kernel in the
+    // stream relies on it) only at the end.  Delta is there: every dK/dV CTA waited for it
+    // before it let this kernel launch.
+    if constexpr (!kPacked) pdl_wait();
     pdl_trigger();
     using CF = BwdCfg<D>;
     extern __shared__ uint8_t smem_raw[];
@@ -1139,6 +1143,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+    if constexpr (kPacked) pdl_wait();
 }
 
 template <int D>

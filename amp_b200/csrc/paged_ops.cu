@@ -9,24 +9,29 @@
 // There is no reference count that could drift, nothing is copied to the host,
 // and every call can be captured into a graph.
 //
-// Each operation is a plan and a move.  The plan (one CTA of 1024 threads) marks
-// the pages in use in a bitmap in shared memory, turns it into a list of free
+// Each operation is a plan and a move.  The plan (a cluster of eight blocks) marks
+// the pages in use in bitmaps in shared memory; one block turns them into a list of free
 // pages, lowest first, by a scan over the bitmap's words, and hands pages out in
 // the order of the request, so the result does not depend on the scheduling of
 // any atomic.  The move copies the pages that the plan listed in every layer and
 // rewrites table rows; it is one grid, launched while the plan runs (programmatic
 // dependent launch), and is HBM-bound: a page is read and written once.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "common.cuh"
 #include "runtime.h"
 #include "tc_common.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace ampb {
 namespace {
 
 constexpr int kPage = 16;
 constexpr int kPlanThreads = 1024;
+constexpr int kCluster = 8;   // blocks that mark pages for one plan
 constexpr int kMoveThreads = 256;
 // The bitmaps take 2 bits a page, of the 227 KB that a block may have.
 constexpr int kMaxPages = 768 * 1024;
@@ -64,16 +69,22 @@ __device__ __forceinline__ void bad_index(int* status) {
     status[kStatusBadIndexInt] = AMP_DEV_ERR_BAD_INDEX;
 }
 
-// Marks the pages of the rows that `counts` accepts; `twice` (may be null) gets those that
-// are named more than once.  One warp a row, four entries a lane in flight.
+// Marks the pages of the rows that `counts` accepts in this block's bitmaps; `twice` (may be
+// null) gets those that are named more than once.  The rows are shared out among the warps of
+// the cluster, a row among several where there are fewer rows than warps; four entries a
+// lane are in flight.
 template <typename F>
 __device__ __forceinline__ void mark_used(const Table& t, unsigned* used, unsigned* twice, F counts) {
+    constexpr int kWarps = kCluster * kPlanThreads / 32;
     const int lane = threadIdx.x & 31;
-    for (int r = threadIdx.x >> 5; r < t.rows; r += kPlanThreads / 32) {
+    const int split = max(1, kWarps / t.rows);   // warps of a row
+    const int tasks = t.rows * split;
+    for (int task = blockIdx.x * (kPlanThreads / 32) + (threadIdx.x >> 5); task < tasks; task += kWarps) {
+        const int r = task / split, seg = task - r * split;
         if (!counts(r)) continue;
         const int n = named(t, t.ctx[r]);
         const int* row = t.table + (int64_t)r * t.width;
-        for (int e0 = 0; e0 < n; e0 += 128) {
+        for (int e0 = seg * 128; e0 < n; e0 += split * 128) {
             int p[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -88,6 +99,30 @@ __device__ __forceinline__ void mark_used(const Table& t, unsigned* used, unsign
             }
         }
     }
+}
+
+// Joins the cluster's bitmaps in its first block, each block taking a part of the words; true
+// for that block, which goes on alone.  (What bounds a plan is marking: a shared-memory atomic
+// takes about as many cycles as a warp has lanes, 12 thousand entries of 256 rows took one
+// block 11 us, eight blocks 3 us with the two waits of the cluster.)
+__device__ __forceinline__ bool join_marks(unsigned* used, unsigned* twice, int words) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int each = (words + kCluster - 1) / kCluster;
+    const int w0 = (int)blockIdx.x * each, w1 = min(w0 + each, words);
+    for (int w = w0 + (int)threadIdx.x; w < w1; w += kPlanThreads) {
+        unsigned once = 0, more = 0;
+#pragma unroll
+        for (int c = 0; c < kCluster; ++c) {
+            const unsigned u = *cluster.map_shared_rank(used + w, c);
+            if (twice) more |= (once & u) | *cluster.map_shared_rank(twice + w, c);
+            once |= u;
+        }
+        *cluster.map_shared_rank(used + w, 0) = once;
+        if (twice) *cluster.map_shared_rank(twice + w, 0) = more;
+    }
+    cluster.sync();
+    return blockIdx.x == 0;
 }
 
 // Writes the lowest free pages, ascending, into list[0 .. most) and returns how many pages
@@ -189,7 +224,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(Pools pl, Moves mv) {
 // (none left) or kSkip; [n] new context; [n * width] parents' rows, when a parent is a child too
 constexpr int kShare = -1, kFailed = -2, kSkip = -3;
 
-__global__ void __launch_bounds__(kPlanThreads)
+__global__ void __cluster_dims__(kCluster) __launch_bounds__(kPlanThreads)
     k_fork_plan(Table t, const int* parents, const int* children, int n, int* done, Moves mv) {
     extern __shared__ unsigned used[];
     __shared__ int part[32];
@@ -206,7 +241,7 @@ __global__ void __launch_bounds__(kPlanThreads)
         return parents[i] >= 0 && parents[i] < t.rows && children[i] >= 0 && children[i] < t.rows;
     };
     for (int i = threadIdx.x; i < n; i += kPlanThreads) {
-        if (!in_range(i)) bad_index(t.status);
+        if (!in_range(i)) bad_index(t.status);   // every block looks: row flags are the block's own
         else if (set_bit(child, children[i])) set_bit(again, children[i]);
     }
     __syncthreads();
@@ -219,7 +254,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     __syncthreads();
     auto replaced = [&](int r) { return bit(child, r) && !bit(again, r); };
     mark_used(t, used, nullptr, [&](int r) { return !replaced(r) || bit(parent, r); });
-    __syncthreads();
+    if (!join_marks(used, nullptr, words)) return;
     // the fresh pages, in dst: the k-th goes to the k-th fork that needs one
     const int free = list_free(used, t.num_pages, mv.dst, n, part);
     int carry = 0;
@@ -286,72 +321,75 @@ __global__ void __launch_bounds__(kMoveThreads)
 // ------------------------------------------------------------------ extend
 // aux: [num_pages] free pages; [rows] where a row's pages begin in that list; [rows] how many
 // (0: none, or not extended); [rows] its entries so far, less one if its last page is replaced
-__global__ void __launch_bounds__(kPlanThreads)
+__global__ void __cluster_dims__(kCluster) __launch_bounds__(kPlanThreads)
     k_extend_plan(Table t, const int* add, int* ctx_out, int* done, Moves mv) {
     extern __shared__ unsigned used[];
     __shared__ int part[32];
-    __shared__ unsigned long long total_need;
     const int words = (t.num_pages + 31) / 32;
     unsigned* twice = used + words;
     int *list = mv.aux, *first = list + t.num_pages, *count = first + t.rows, *at_entry = count + t.rows;
     pdl_wait();
     pdl_trigger();
     for (int i = threadIdx.x; i < 2 * words; i += kPlanThreads) used[i] = 0;
-    if (threadIdx.x == 0) total_need = 0;
     __syncthreads();
     mark_used(t, used, twice, [](int) { return true; });
-    __syncthreads();
+    if (!join_marks(used, twice, words)) return;
     // Pages that row r needs: new ones, and one for a partly filled last page that another
     // row names too (the next token must not be written into the other's cache).
-    auto plan_row = [&](int r, int& ctx, int& have, int& more, bool& own) {
+    auto plan_row = [&](int r, int& ctx, int& have, bool& own, bool& ok) {
         ctx = max(t.ctx[r], 0);
         have = named(t, ctx);
-        more = 0;
         own = false;
         const int n = add[r];
-        if (n <= 0 || (int64_t)ctx + n > (int64_t)t.width * kPage) return n == 0;
-        more = (int)(((int64_t)ctx + n - 1) / kPage + 1) - have;
+        ok = n >= 0 && (int64_t)ctx + n <= (int64_t)t.width * kPage;
+        if (n <= 0 || !ok) return 0;
+        int more = (int)(((int64_t)ctx + n - 1) / kPage + 1) - have;
         if (ctx % kPage != 0) {
             const int tail = t.table[(int64_t)r * t.width + have - 1];
             own = tail >= 0 && tail < t.num_pages && bit(twice, tail);
             more += own;
         }
-        more = min(more, t.num_pages + 1);   // more than there are is as bad as one too many
-        return true;
+        return min(more, t.num_pages + 1);   // more than there are is as bad as one too many
     };
-    for (int r = threadIdx.x; r < t.rows; r += kPlanThreads) {
-        int ctx, have, more;
-        bool own;
-        plan_row(r, ctx, have, more, own);
-        if (more) atomicAdd(&total_need, (unsigned long long)more);
-    }
-    __syncthreads();
-    const int most = (int)min(total_need, (unsigned long long)t.num_pages);
-    const int free = list_free(used, t.num_pages, list, most, part);
-    int carry = 0, copies = 0;
+    int carry = 0;
     for (int r0 = 0; r0 < t.rows; r0 += kPlanThreads) {
         const int r = r0 + threadIdx.x;
-        int ctx = 0, have = 0, more = 0;
-        bool own = false, ok = false;
-        if (r < t.rows) ok = plan_row(r, ctx, have, more, own);
+        int ctx, have = 0, more = 0;
+        bool own = false, ok;
+        if (r < t.rows) more = plan_row(r, ctx, have, own, ok);
         const int end = carry + block_scan(more, part);
         carry = min(carry + part[31], 1 << 30);   // far past any pool: stays below 2^31
-        // in order: once the pool cannot hold a row's pages, that row and all later ones
-        // that need any fail
-        if (more && end > free) ok = false;
-        own = own && ok;
-        const int at = copies + block_scan(own ? 1 : 0, part) - 1;
-        copies += part[31];
         if (r < t.rows) {
-            if (own) {
-                mv.src[at] = t.table[(int64_t)r * t.width + have - 1];
-                mv.dst[at] = list[end - more];
-            }
             first[r] = end - more;
-            count[r] = ok ? more : 0;
+            count[r] = more;
             at_entry[r] = have - own;
+            // for now: kept, or kept only if its pages are there
             ctx_out[r] = ok ? ctx + add[r] : t.ctx[r];
             done[r] = ok;
+        }
+    }
+    const int free = list_free(used, t.num_pages, list, min(carry, t.num_pages), part);
+    int copies = 0;
+    for (int r0 = 0; r0 < t.rows; r0 += kPlanThreads) {
+        const int r = r0 + threadIdx.x;
+        bool own = false;
+        if (r < t.rows && count[r] > 0) {
+            // in order: once the pool cannot hold a row's pages, that row and all later ones
+            // that need any fail
+            const int new_ctx = ctx_out[r], have = named(t, new_ctx - add[r]);
+            if (first[r] + count[r] > free) {
+                count[r] = 0;
+                ctx_out[r] = new_ctx - add[r];
+                done[r] = 0;
+            } else {
+                own = at_entry[r] < have;
+            }
+        }
+        const int at = copies + block_scan(own ? 1 : 0, part) - 1;
+        copies += part[31];
+        if (own) {
+            mv.src[at] = t.table[(int64_t)r * t.width + at_entry[r]];
+            mv.dst[at] = list[first[r]];
         }
     }
     if (threadIdx.x == 0) mv.count[0] = copies;
@@ -374,7 +412,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_extend_move(Pools pl, Moves mv
 // ------------------------------------------------------------------ compact
 // With L pages in use, those at L and above move to the free ones below L, both in
 // ascending order; aux[p] is where page p >= L goes.
-__global__ void __launch_bounds__(kPlanThreads) k_compact_plan(Table t, int* used_out, Moves mv) {
+__global__ void __cluster_dims__(kCluster) __launch_bounds__(kPlanThreads) k_compact_plan(Table t, int* used_out, Moves mv) {
     extern __shared__ unsigned used[];
     __shared__ int part[32];
     const int words = (t.num_pages + 31) / 32;
@@ -383,7 +421,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_compact_plan(Table t, int* use
     for (int i = threadIdx.x; i < words; i += kPlanThreads) used[i] = 0;
     __syncthreads();
     mark_used(t, used, nullptr, [](int) { return true; });
-    __syncthreads();
+    if (!join_marks(used, nullptr, words)) return;
     const int each = (words + kPlanThreads - 1) / kPlanThreads;
     const int w0 = min((int)threadIdx.x * each, words), w1 = min(w0 + each, words);
     int n = 0;
@@ -488,11 +526,11 @@ int check_ws(const void* ws, size_t have, size_t need) {
 constexpr size_t kMaxPlanSmem = std::max(2 * kMaxPages / 8, kMaxPages / 8 + 3 * kMaxRows / 8);
 
 template <auto kern, typename... A>
-int launch_plan(int smem_words, cudaStream_t st, A... args) {
+int launch_plan(int blocks, int smem_words, cudaStream_t st, A... args) {
     const size_t smem = (size_t)smem_words * 4;
     static std::atomic<uint64_t> allowed{0};
     AMPB_CHECK_CUDA(allow_smem_once(allowed, kern, kMaxPlanSmem));
-    AMPB_CHECK_CUDA(launch_pdl(kern, dim3(1), dim3(kPlanThreads), smem, st, args...));
+    AMPB_CHECK_CUDA(launch_pdl(kern, dim3(blocks), dim3(kPlanThreads), smem, st, args...));
     return AMP_OK;
 }
 
@@ -535,7 +573,7 @@ int amp_paged_copy_pages_dev(void* k_pool, void* v_pool, int layers, int num_pag
     if ((rc = device_status(&status))) return rc;
     const Moves mv = moves_at(workspace, n);
     cudaStream_t st = as_stream(stream);
-    if ((rc = launch_plan<k_copy_plan>(2 * ((num_pages + 31) / 32), st, src, dst, n, num_pages, mv, status)))
+    if ((rc = launch_plan<k_copy_plan>(1, 2 * ((num_pages + 31) / 32), st, src, dst, n, num_pages, mv, status)))
         return rc;
     AMPB_CHECK_CUDA(launch_pdl(k_move, dim3(move_grid(pl, n, 1)), dim3(kMoveThreads), 0, st, pl, mv));
     return AMP_OK;
@@ -559,7 +597,7 @@ int amp_paged_fork_dev(void* k_pool, void* v_pool, int layers, int num_pages, in
     const Moves mv = moves_at(workspace, n);
     cudaStream_t st = as_stream(stream);
     const int words = (num_pages + 31) / 32 + 3 * ((rows + 31) / 32);
-    if ((rc = launch_plan<k_fork_plan>(words, st, t, parents, children, n, done, mv))) return rc;
+    if ((rc = launch_plan<k_fork_plan>(kCluster, words, st, t, parents, children, n, done, mv))) return rc;
     AMPB_CHECK_CUDA(launch_pdl(k_fork_move, dim3(move_grid(pl, n, n)), dim3(kMoveThreads), 0, st, pl, mv, t,
                                parents, children, n));
     return AMP_OK;
@@ -580,7 +618,7 @@ int amp_paged_extend_dev(void* k_pool, void* v_pool, int layers, int num_pages, 
     if ((rc = device_status(&t.status))) return rc;
     const Moves mv = moves_at(workspace, rows);
     cudaStream_t st = as_stream(stream);
-    if ((rc = launch_plan<k_extend_plan>(2 * ((num_pages + 31) / 32), st, t, add, ctx_out, done, mv))) return rc;
+    if ((rc = launch_plan<k_extend_plan>(kCluster, 2 * ((num_pages + 31) / 32), st, t, add, ctx_out, done, mv))) return rc;
     // pages are copied only where rows share a partly filled one: a block a multiprocessor is enough
     AMPB_CHECK_CUDA(launch_pdl(k_extend_move, dim3((unsigned)std::min(rows, sm_count())), dim3(kMoveThreads),
                                0, st, pl, mv, t));
@@ -603,7 +641,7 @@ int amp_paged_compact_dev(void* k_pool, void* v_pool, int layers, int num_pages,
     if ((rc = device_status(&t.status))) return rc;
     const Moves mv = moves_at(workspace, num_pages);
     cudaStream_t st = as_stream(stream);
-    if ((rc = launch_plan<k_compact_plan>((num_pages + 31) / 32, st, t, used, mv))) return rc;
+    if ((rc = launch_plan<k_compact_plan>(kCluster, (num_pages + 31) / 32, st, t, used, mv))) return rc;
     AMPB_CHECK_CUDA(launch_pdl(k_compact_move, dim3(move_grid(pl, num_pages / 2, rows)), dim3(kMoveThreads), 0,
                                st, pl, mv, t, table_out));
     return AMP_OK;

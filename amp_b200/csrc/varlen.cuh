@@ -107,6 +107,9 @@ struct VarlenDraw {
         const int lane = threadIdx.x & 31;
         VarlenSeq s = {0, 0, 0, 0};
         if (lane < plan.B) s = plan.load(lane, status);
+        mine = s;
+        number(items(mine));
+        if (total <= (int)gridDim.x) return;   // an item a CTA: any order will do
         const int key = s.q_len > s.k_len ? s.q_len : s.k_len;
         int rank = 0, from = 0;
         for (int i = 0; i < 32; ++i) {
@@ -119,8 +122,13 @@ struct VarlenDraw {
         mine.q_len = __shfl_sync(0xffffffffu, s.q_len, from);
         mine.k_off = __shfl_sync(0xffffffffu, s.k_off, from);
         mine.k_len = __shfl_sync(0xffffffffu, s.k_len, from);
-        const int n = items(mine);
+        number(items(mine));
+    }
+    // the lanes' running numbers of items
+    __device__ __forceinline__ void number(int n) {
+        const int lane = threadIdx.x & 31;
         int end = n;
+#pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int t = __shfl_up_sync(0xffffffffu, end, o);
             if (lane >= o) end += t;
