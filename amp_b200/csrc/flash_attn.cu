@@ -996,8 +996,8 @@ int launch_packed(const PackedArgs& a, cudaStream_t st) {
     p.total_q = a.total_q;
     // no more CTAs than there can be items
     const int64_t most = ((int64_t)a.total_q / BQ + a.B) * a.Hq;
-    p.plan = {a.ws, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
-    if ((rc = varlen_make_plan(p.plan, (most + 1) / 2, a.Hq, a.Hkv, false, st))) return rc;
+    p.plan = {a.ws, false, false, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
+    if ((rc = varlen_make_plan(p.plan, (most + 1) / 2, a.Hq, a.Hkv, false, true, st))) return rc;
     auto kern = k_flash_fwd<D, false, false, true, true>;
     static std::atomic<uint64_t> allowed{0};
     AMPB_CHECK_CUDA(allow_smem_once(allowed, kern, FaCfg<D>::SMEM));

@@ -216,6 +216,7 @@ constexpr int kDeltaLoads = 4;
 struct DeltaStrides {
     int64_t o_tok, o_head, do_tok, do_head;
     int H, total;
+    int* next;   // the two passes' counters to zero, or null
 };
 template <int D, bool kPacked = false>
 __global__ void __launch_bounds__(256) k_fa_bwd_delta(const __nv_bfloat16* __restrict__ O,
@@ -224,6 +225,7 @@ __global__ void __launch_bounds__(256) k_fa_bwd_delta(const __nv_bfloat16* __res
                                                       DeltaStrides st = {}) {
     pdl_wait();
     pdl_trigger();
+    if (kPacked && st.next && blockIdx.x == 0 && threadIdx.x < 2) st.next[threadIdx.x] = 0;
     constexpr int LPR = D / 8;            // lanes per row, 8 bf16 (16 bytes) each
     constexpr int RPW = 32 / LPR;         // rows per warp-wide load
     constexpr int ROWS = RPW * kDeltaLoads;
@@ -1254,18 +1256,20 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
     p.dk_head = s[13];
     p.dv_tok = s[14];
     p.dv_head = s[15];
-    p.plan = {a.ws, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
+    p.plan = {a.ws, false, false, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
     float* delta = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) +
                                             (varlen_plan_bytes(a.B) + 15) / 16 * 16);
     p.delta = delta;
     // no more CTAs than there can be items
     const int64_t most_kv = ((int64_t)a.total_kv / BT + a.B) * a.Hkv;
     const int64_t most_q = ((int64_t)a.total_q / BT + a.B) * a.Hq;
-    if ((rc = varlen_make_plan(p.plan, std::max(most_kv, most_q), a.Hq, a.Hkv, true, st))) return rc;
     const int64_t rows = (int64_t)a.total_q * a.Hq;
+    if ((rc = varlen_make_plan(p.plan, std::max(most_kv, most_q), a.Hq, a.Hkv, true, rows == 0, st)))
+        return rc;
     if (rows > 0) {
         const int64_t per_block = 8 * (32 / (D / 8)) * kDeltaLoads;
-        const DeltaStrides ds = {s[6], s[7], s[8], s[9], a.Hq, a.total_q};
+        const DeltaStrides ds = {s[6], s[7], s[8], s[9], a.Hq, a.total_q,
+                                 p.plan.lists ? nullptr : static_cast<int*>(a.ws)};
         AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_delta<D, true>,
                                    dim3((unsigned)std::min<int64_t>((rows + per_block - 1) / per_block,
                                                                     (int64_t)sm_count() * 8)),

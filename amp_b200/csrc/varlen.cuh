@@ -41,7 +41,8 @@ inline size_t varlen_plan_bytes(int B) {
 }
 
 struct VarlenPlan {
-    void* ws;                        // the lists, or null: no plan kernel (VarlenDraw)
+    void* ws;
+    bool lists, counted;             // which of the ways of VarlenDraw
     const int *cu_q, *cu_kv;         // the offsets themselves
     int B, total_q, total_kv;
     __device__ int* next() const { return static_cast<int*>(ws); }
@@ -62,10 +63,10 @@ struct VarlenPlan {
     }
 };
 
-// Enqueues the plan kernel (`backward` selects which lists it fills), or, for few items,
-// sets plan.ws to null and leaves the plan to each CTA.  most_items: the most that there
-// can be, which is all that the host knows.
-int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward,
+// Chooses how the CTAs get their items, and enqueues what that needs: the plan kernel
+// (`backward` selects which lists it fills), or, where `zero` is true, the zeroing of the
+// counters.  most_items: the most that there can be, which is all that the host knows.
+int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward, bool zero,
                      cudaStream_t st);
 
 // Warp-wide (all lanes call it): the sequence r whose items hold `item`, i.e. the
@@ -86,11 +87,13 @@ __device__ __forceinline__ int varlen_find(const int* first, int B, int item) {
     return lo;
 }
 
-// How a CTA's drawing warp gets its items.  With a plan in the workspace: from the
-// lists, the first by the CTA's index and the rest from the counter.  Without one (few
-// items, at most 32 sequences): lane r holds the r-th longest sequence, and the items
-// are dealt out forth and back, so that a CTA whose first was long gets a short one.
-// That saves a small call the plan's launch.
+// How a CTA's drawing warp gets its items.
+//   lists    (more than 32 sequences) the sequences by length and the items before each come
+//            from the plan kernel; otherwise lane r holds the r-th longest sequence, which
+//            saves the plan's launch.
+//   counted  the first item is the CTA's index, the rest come from the counter; otherwise
+//            (few items) they are dealt out forth and back, so that a CTA whose first was
+//            long gets a short one.
 struct VarlenDraw {
     const VarlenPlan& plan;
     int list, total;
@@ -100,7 +103,7 @@ struct VarlenDraw {
     template <typename F>
     __device__ __forceinline__ VarlenDraw(const VarlenPlan& p, int list_, F items, int* status)
         : plan(p), list(list_), mine{0, 0, 0, 0}, first(0) {
-        if (plan.ws) {
+        if (plan.lists) {
             total = plan.first(list)[plan.B];
             return;
         }
@@ -139,7 +142,7 @@ struct VarlenDraw {
     // the CTA's k-th item, k = 0, 1, ...; at or past `total`: no more
     __device__ __forceinline__ int next(int k) const {
         const int grid = (int)gridDim.x, cta = (int)blockIdx.x;
-        if (!plan.ws) return k * grid + (k & 1 ? grid - 1 - cta : cta);
+        if (!plan.counted) return k * grid + (k & 1 ? grid - 1 - cta : cta);
         if (k == 0) return cta;
         int item = 0;
         if ((threadIdx.x & 31) == 0) item = grid + atomicAdd(plan.next() + list, 1);
@@ -147,7 +150,7 @@ struct VarlenDraw {
     }
     // the sequence of an item, and the item's number within it
     __device__ __forceinline__ int find(int item, VarlenSeq& s) const {
-        if (plan.ws) {
+        if (plan.lists) {
             const int r = varlen_find(plan.first(list), plan.B, item);
             s = plan.seqs()[r];
             return item - plan.first(list)[r];

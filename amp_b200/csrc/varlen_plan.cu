@@ -79,13 +79,16 @@ __global__ void __launch_bounds__(kPlanThreads)
 
 }  // namespace
 
-int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward,
+int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward, bool zero,
                      cudaStream_t st) {
-    // 32 sequences fit a warp, and dealing four items a CTA out in turn loses less than the
-    // launch costs: forward of 8 prompts of 22 to 200 tokens 22.5 -> 20.5 us, forward and
-    // backward of 17 sequences of up to 700 tokens 84.0 -> 73.7 us.
-    if (plan.B <= 32 && most_items <= 4 * sm_count()) {
-        plan.ws = nullptr;
+    // 32 sequences fit a warp.  Up to four items a CTA, dealing them out in turn loses less than
+    // the counter's zeroing and its latency cost (forward of 8 prompts of 22 to 200 tokens:
+    // 22.5 -> 20.5 us; forward and backward of 17 sequences of up to 700: 84.0 -> 73.7 us);
+    // with more, lengths decide (25 sequences of up to 16384 tokens: 9.3 ms dealt, 8.5 counted).
+    plan.lists = plan.B > 32;
+    plan.counted = plan.lists || most_items > 4 * sm_count();
+    if (!plan.lists) {
+        if (plan.counted && zero) AMPB_CHECK_CUDA(cudaMemsetAsync(plan.ws, 0, 64, st));
         return AMP_OK;
     }
     int* status = nullptr;
