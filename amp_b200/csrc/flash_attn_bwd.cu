@@ -87,7 +87,7 @@ struct BwdParams {
     int* status;
     // packed mode: rows of the whole Q (lse, delta are [Hq][total_q]), strides of the
     // gradients in elements, the work lists
-    int total_q;
+    int total_q, after_dkdv;
     int64_t dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
     VarlenPlan plan;
 };
@@ -770,11 +770,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     k_fa_bwd_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
                 const BwdParams p) {
-    // Packed: nothing here needs what the dK/dV pass writes, so a CTA starts as soon as one of
-    // that pass leaves its SM, and waits for the pass to be complete (the next kernel in the
-    // stream relies on it) only at the end.  Delta is there: every dK/dV CTA waited for it
-    // before it let this kernel launch.
-    if constexpr (!kPacked) pdl_wait();
+    // Packed, after a dK/dV pass: nothing here needs what that pass writes, so a CTA starts as
+    // soon as one of its CTAs leaves the SM, and waits for the pass to be complete (the next
+    // kernel in the stream relies on it) only at the end.  Delta and the counters are there:
+    // every dK/dV CTA waited for them before it let this kernel launch.
+    if (!kPacked || !p.after_dkdv) pdl_wait();
     pdl_trigger();
     using CF = BwdCfg<D>;
     extern __shared__ uint8_t smem_raw[];
@@ -1250,6 +1250,7 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
     p.dk = a.dK;
     p.dv = a.dV;
     p.total_q = a.total_q;
+    p.after_dkdv = a.total_kv > 0;
     p.dq_tok = s[10];
     p.dq_head = s[11];
     p.dk_tok = s[12];

@@ -136,8 +136,14 @@ int staging_get(int slot, size_t bytes, void** out) {
 }
 
 namespace {
+// status word (int 0), bad-index word (int 1), wait limit (u64 at byte 8): tc_common.cuh.  A
+// variable of the module, so that a library call may be the first of its process inside a
+// stream capture: nothing is allocated or copied for it.
+struct StatusBlock { int status[2]; unsigned long long limit_ns; };
+static_assert(offsetof(StatusBlock, limit_ns) == kStatusLimitOffsetInts * sizeof(int), "layout");
+__device__ StatusBlock g_status_block = {{AMP_DEV_OK, 0}, kWaitTimeoutNs};
 std::mutex g_status_mu;
-std::vector<int*> g_status;  // [device]
+std::vector<int*> g_status;  // its address, by device
 }  // namespace
 
 int device_status(int** out) {
@@ -146,18 +152,9 @@ int device_status(int** out) {
     std::lock_guard<std::mutex> lk(g_status_mu);
     if ((int)g_status.size() <= dev) g_status.resize(dev + 1, nullptr);
     if (!g_status[dev]) {
-        // status word (int 0), bad-index word (int 1), wait limit (u64 at byte 8): tc_common.cuh
-        struct Block { int status[2]; unsigned long long limit_ns; };
-        static_assert(offsetof(Block, limit_ns) == kStatusLimitOffsetInts * sizeof(int), "layout");
-        const Block init = {{AMP_DEV_OK, 0}, kWaitTimeoutNs};
-        int* p = nullptr;
-        AMPB_CHECK_CUDA(cudaMalloc(&p, sizeof(Block)));
-        const cudaError_t e = cudaMemcpy(p, &init, sizeof(Block), cudaMemcpyHostToDevice);
-        if (e != cudaSuccess) {
-            cudaFree(p);
-            return cuda_status(e, "cudaMemcpy(status block)");
-        }
-        g_status[dev] = p;
+        void* p = nullptr;
+        AMPB_CHECK_CUDA(cudaGetSymbolAddress(&p, g_status_block));
+        g_status[dev] = static_cast<int*>(p);
     }
     *out = g_status[dev];
     return AMP_OK;

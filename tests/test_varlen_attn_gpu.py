@@ -10,6 +10,10 @@ The bounds count roundings (u = 2^-8, half a bf16 step relative to the value):
 each with 5% for products of roundings and 1e-5 for the fp32 sums.  The scores' fp32 error
 enters P through exp: it is the lse bound, and is added to u wherever P is.
 """
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -19,6 +23,7 @@ from amp_b200._lib import lib
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -8
+ROOT = Path(__file__).resolve().parents[1]
 
 
 def make(lens_q, lens_kv, Hq, Hkv, D, seed=0, pad_q=0, pad_kv=0):
@@ -297,3 +302,38 @@ def test_offsets_outside_the_tensors_are_skipped_and_reported(offsets, cuda, amp
         ref = reference(q[:50], k[:50], v[:50], do[:50], n, n, True)["o"]
         x = out[rows].double().cpu().numpy()
         assert (np.abs(x - ref[0][rows]) <= ref[1][rows]).all()
+
+
+FIRST_IN_CAPTURE = """
+import torch
+from amp_b200 import attention, rope
+q, k = torch.randn(64, 4, 64, device="cuda").bfloat16(), torch.randn(64, 2, 64, device="cuda").bfloat16()
+cu = torch.tensor([0, 20, 64], dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    o, lse = attention.flash_attn_varlen_fwd(q, k, k, cu)
+    grads = attention.flash_attn_varlen_bwd(q, k, k, o, q, lse, cu)
+graph.replay()
+torch.cuda.synchronize()
+o2, lse2 = attention.flash_attn_varlen_fwd(q, k, k, cu)
+assert torch.equal(o, o2) and torch.equal(lse, lse2)
+for a, b in zip(grads, attention.flash_attn_varlen_bwd(q, k, k, o2, q, lse2, cu)):
+    assert torch.equal(a, b)
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured(cuda, amp_lib):
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE], cwd=ROOT, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr
+
+
+def test_no_key_anywhere_with_many_items(cuda, amp_lib):
+    """The dQ pass alone, its items drawn from the counter."""
+    lens = [700] * 20
+    q, k, v, do, cu, _ = make(lens, lens, 16, 2, 64, seed=37)
+    none = torch.zeros(21, dtype=torch.int32)
+    for _ in range(5):
+        got = run(q, k[:0], v[:0], do, cu, none, True)
+        assert not got["dq"].any() and not got["o"].any() and (got["lse"] == -np.inf).all()
