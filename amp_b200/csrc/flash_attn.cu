@@ -1001,7 +1001,7 @@ int launch_packed(const PackedArgs& a, cudaStream_t st) {
     // no more CTAs than there can be items
     const int64_t most = ((int64_t)a.total_q / BQ + a.B) * a.Hq;
     p.plan = {a.ws, false, false, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
-    if ((rc = varlen_make_plan(p.plan, (most + 1) / 2, a.Hq, a.Hkv, false, true, st))) return rc;
+    if ((rc = varlen_make_plan(p.plan, (most + 1) / 2, a.Hq, a.Hkv, false, 1, true, st))) return rc;
     auto kern = k_flash_fwd<D, false, false, true, true>;
     static std::atomic<uint64_t> allowed{0};
     AMPB_CHECK_CUDA(allow_smem_once(allowed, kern, FaCfg<D>::SMEM));
@@ -1119,6 +1119,7 @@ int varlen_check(int B, int total_q, int total_kv, int Hq, int Hkv, int D, const
                      AMP_ERR_INVALID,
                      "packed attention: stride %d (%lld elements) must be a positive multiple of 8",
                      i, (long long)strides[i]);
+    AMPB_REQUIRE(need > 0, AMP_ERR_INVALID, "packed attention: bad sizes");
     AMPB_REQUIRE(ws && aligned16(ws), AMP_ERR_INVALID, "workspace must be 16-byte aligned");
     AMPB_REQUIRE(ws_bytes >= need, AMP_ERR_INVALID, "workspace too small: %zu < %zu", ws_bytes, need);
     return AMP_OK;

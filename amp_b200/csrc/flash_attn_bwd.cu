@@ -24,6 +24,11 @@
 // (S_{j+1}, dQ_j, dP_{j+1}).
 // Each pass recomputes P from lse, so there are no atomics and no fp32 dQ
 // accumulator in global memory.
+// Packed mode, few key tiles: an item sums over the query tiles of all query heads of its kv
+// head, so a short batch with large groups leaves most CTAs idle behind a few long items
+// (one kv head for 8 query heads, 2000 tokens: 16 items of up to 128 steps).  There the query
+// heads are shared out among items of their own, which leave fp32 sums that k_fa_bwd_join
+// adds in order (no atomics; the same bits every time).
 // Packed mode (sequences of different lengths one after another, varlen.cuh): both
 // passes draw their tiles from lists of the sequences, longest first, most steps first;
 // warp 3 decodes items ahead into a two-slot ring.  A tile that runs past its sequence
@@ -89,7 +94,11 @@ struct BwdParams {
     int* status;
     // packed mode: rows of the whole Q (lse, delta are [Hq][total_q]), strides of the
     // gradients in elements, the work lists
-    int total_q, after_dkdv;
+    int total_q, total_kv, after_dkdv;
+    // the query heads of a kv head are summed in so many parts, each [total_kv][Hkv][D] of
+    // dK, then of dV, in `sums`
+    int parts;
+    float* sums;
     int64_t dq_tok, dq_head, dk_tok, dk_head, dv_tok, dv_head;
     VarlenPlan plan;
 };
@@ -98,6 +107,7 @@ struct BwdParams {
 struct BwdItem {
     int live;                   // packed: 0 ends the list
     int b, head, tile;          // head: kv head (dK/dV) or query head (dQ) within b
+    int g0, heads, part;        // dK/dV: query heads of the group that it sums, and its part
     int q_tok, k_tok;           // packed: the sequence's first rows
     int S_q, S_kv;
     int coff;                   // key j visible for query i iff j <= i + coff
@@ -110,7 +120,7 @@ __device__ __forceinline__ void draw_items(const BwdParams& p, BwdItem* items, u
                                            uint64_t* it_empty) {
     const int lane = threadIdx.x & 31;
     VarlenDraw draw(p.plan, kKeys ? 0 : 1, [&](const VarlenSeq& s) {
-        return kKeys ? varlen_tiles(s.k_len) * p.Hkv : varlen_tiles(s.q_len) * p.Hq;
+        return kKeys ? varlen_tiles(s.k_len) * p.Hkv * p.parts : varlen_tiles(s.q_len) * p.Hq;
     }, p.status);
     for (int k = 0;; ++k) {
         if (k >= 2 && !mbar_wait_warp<true>(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) return;
@@ -118,8 +128,15 @@ __device__ __forceinline__ void draw_items(const BwdParams& p, BwdItem* items, u
         BwdItem it = {};
         if (item < draw.total) {
             VarlenSeq sq;
-            const int w = draw.find(item, sq);   // number within its sequence
+            int w = draw.find(item, sq);   // number within its sequence
             const int n = varlen_tiles(kKeys ? sq.k_len : sq.q_len);
+            if constexpr (kKeys) {
+                const int group = p.Hq / p.Hkv;
+                it.part = w % p.parts;
+                w /= p.parts;
+                it.g0 = it.part * group / p.parts;
+                it.heads = (it.part + 1) * group / p.parts - it.g0;
+            }
             it.live = 1;
             it.head = w / n;
             // under a causal mask the first keys and the last queries have the most steps
@@ -157,6 +174,9 @@ __device__ __forceinline__ bool read_item(int k, const BwdItem* items, uint64_t*
     it.b = 0;
     it.head = same_in_warp<true>(src.head);
     it.tile = same_in_warp<true>(src.tile);
+    it.g0 = same_in_warp<true>(src.g0);
+    it.heads = same_in_warp<true>(src.heads);
+    it.part = same_in_warp<true>(src.part);
     it.q_tok = same_in_warp<true>(src.q_tok);
     it.k_tok = same_in_warp<true>(src.k_tok);
     it.S_q = same_in_warp<true>(src.S_q);
@@ -341,6 +361,63 @@ __device__ __forceinline__ void store_zero_row(__nv_bfloat16* row, int half) {
         *reinterpret_cast<uint4*>(row + e) = make_uint4(0u, 0u, 0u, 0u);
 }
 
+// the same as fp32, for the parts of dK and dV
+template <int D>
+__device__ __forceinline__ void store_sums(uint32_t lane_addr, float mul, float* row, bool ok, int half) {
+    __syncwarp();
+#pragma unroll
+    for (int ocl = 0; ocl < D / 64; ++ocl) {
+        const int oc = half * (D / 64) + ocl;
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(lane_addr + oc * 32, v);
+        tmem_ld_wait();
+        if (ok) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(row + oc * 32 + e) =
+                    make_float4(__uint_as_float(v[e]) * mul, __uint_as_float(v[e + 1]) * mul,
+                                __uint_as_float(v[e + 2]) * mul, __uint_as_float(v[e + 3]) * mul);
+        }
+    }
+}
+template <int D>
+__device__ __forceinline__ void store_zero_sums(float* row, int half) {
+#pragma unroll
+    for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 4)
+        *reinterpret_cast<float4*>(row + e) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+}
+
+// Adds the parts up, in order, and rounds once: a warp a token of some sequence, four
+// elements a lane (the parts of a row are total_kv rows apart).
+template <int D>
+__global__ void __launch_bounds__(256) k_fa_bwd_join(BwdParams p) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int per_row = p.Hkv * (D / 4);
+    const int64_t part = (int64_t)p.total_kv * p.Hkv * D;
+    for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < p.total_kv; t += gridDim.x * 8) {
+        const VarlenSeq sq = p.plan.load(varlen_find(p.plan.cu_kv, p.plan.B, t), p.status);
+        if (t < sq.k_off || t >= sq.k_off + sq.k_len) continue;   // a token of no sequence
+        for (int i = lane; i < 2 * per_row; i += 32) {
+            const bool v = i >= per_row;
+            const int c = v ? i - per_row : i;   // four elements c * 4 of the token's heads
+            const float* src = p.sums + (v ? p.parts * part : 0) + (int64_t)t * p.Hkv * D + c * 4;
+            float4 a = *reinterpret_cast<const float4*>(src);
+            for (int z = 1; z < p.parts; ++z) {
+                const float4 b = *reinterpret_cast<const float4*>(src + z * part);
+                a = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+            }
+            const int h = c / (D / 4), e = c % (D / 4) * 4;
+            __nv_bfloat16* dst = v ? static_cast<__nv_bfloat16*>(p.dv) + t * p.dv_tok + h * p.dv_head
+                                   : static_cast<__nv_bfloat16*>(p.dk) + t * p.dk_tok + h * p.dk_head;
+            uint2 w;
+            w.x = f32x2_to_bf16x2(a.x, a.y);
+            w.y = f32x2_to_bf16x2(a.z, a.w);
+            *reinterpret_cast<uint2*>(dst + e) = w;
+        }
+    }
+}
+
 // ---------------------------------------------------------------- dK, dV
 template <int D, bool kPacked = false>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -406,6 +483,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (st == 1) {
                 it.b = bh_kv / p.Hkv;
                 it.head = bh_kv % p.Hkv;
+                it.g0 = it.part = 0;
+                it.heads = G;
                 it.tile = jt;
                 it.q_tok = it.k_tok = 0;
                 it.S_q = p.S_q;
@@ -481,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 it_done(k);
                 const int i_lo = first_tile(it);
                 const int per_head = max(0, q_tiles(it) - i_lo);
-                const int steps = G * per_head;
+                const int steps = it.heads * per_head;
                 if (steps == 0) continue;
                 const int b = it.b, hk = it.head, bh_kv = b * p.Hkv + hk;
                 const int k_row = it.k_tok + it.tile * BT;
@@ -496,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int t = 0; t < steps; ++t, ++g) {
                     const int s = g & 1;
                     if (!mbar_wait(&qs_empty[s], ((g >> 1) & 1) ^ 1, p.status)) { ok = false; break; }
-                    const int gq = t / per_head, qt = i_lo + t % per_head;
+                    const int gq = it.g0 + t / per_head, qt = i_lo + t % per_head;
                     const int bh_q = b * p.Hq + hk * G + gq;
                     // packed: a tile past the sequence's end goes to warp 2 first
                     uint64_t* bar = kPacked && (qt + 1) * BT > it.S_q ? &qs_raw[s] : &qs_full[s];
@@ -527,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (st == 0) break;
                 if (st == 2) continue;
                 it_done(k);
-                const int steps = G * max(0, q_tiles(it) - first_tile(it));
+                const int steps = it.heads * max(0, q_tiles(it) - first_tile(it));
                 if (steps == 0) continue;
                 const uint32_t ka = opaque_u32(ka0), va = opaque_u32(va0);
                 if (!(mbar_wait(kv_full, li & 1, p.status) &&
@@ -595,14 +674,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int per_head = max(0, q_tiles(it) - first_tile(it));
             const int valid = it.S_q - (q_tiles(it) - 1) * BT;   // rows of the last tile
             if (per_head > 0 && valid < BT)
-                for (int gq = 0; ok && gq < G; ++gq) {           // the last tile of each head
+                for (int gq = 0; ok && gq < it.heads; ++gq) {    // the last tile of each head
                     const int s = (g + gq * per_head + per_head - 1) & 1;
                     ok = zero_tail(&qs_raw[s], (s ? phase1 : phase0) & 1, &qs_full[s],
                                    q_s + s * CF::TILE, o_s + s * CF::TILE, CF::SLABS, valid,
                                    p.status);
                     if (s) ++phase1; else ++phase0;
                 }
-            g += G * per_head;
+            g += it.heads * per_head;
         }
     } else if (kPacked && warp == 3) {
         draw_items<true>(p, items, it_full, it_empty);
@@ -632,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int kj = item.tile * BT + kr;
         const int i_lo = first_tile(item);
         const int per_head = max(0, q_tiles(item) - i_lo);
-        const int steps = G * per_head;
+        const int steps = item.heads * per_head;
         const bool row_ok = kj < item.S_kv;
         const int64_t dense_row = ((int64_t)bh_kv * p.S_kv + (row_ok ? kj : 0)) * D;
         const int64_t tok = item.k_tok + (row_ok ? kj : 0);
@@ -640,8 +719,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 (kPacked ? tok * p.dk_tok + hk * p.dk_head : dense_row);
         __nv_bfloat16* dv_row = static_cast<__nv_bfloat16*>(p.dv) +
                                 (kPacked ? tok * p.dv_tok + hk * p.dv_head : dense_row);
+        // packed, in parts: fp32 sums of the part's query heads
+        const bool parted = kPacked && p.parts > 1;
+        float* dk_sum = nullptr;
+        float* dv_sum = nullptr;
+        if (parted) {
+            dk_sum = p.sums + (((int64_t)item.part * p.total_kv + tok) * p.Hkv + hk) * D;
+            dv_sum = dk_sum + (int64_t)p.parts * p.total_kv * p.Hkv * D;
+        }
         if (steps == 0) {   // no query sees these keys: dK = dV = 0, no barriers
-            if (row_ok) {
+            if (row_ok && parted) {
+                store_zero_sums<D>(dk_sum, half);
+                store_zero_sums<D>(dv_sum, half);
+            } else if (row_ok) {
                 store_zero_row<D>(dk_row, half);
                 store_zero_row<D>(dv_row, half);
             }
@@ -653,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // -lse2 / -Delta of query `tid` of step t's tile (threads tid < 128)
         auto fetch = [&](int t, float& nl2, float& ndl) {
-            const int gq = t / per_head, qt = i_lo + t % per_head;
+            const int gq = item.g0 + t / per_head, qt = i_lo + t % per_head;
             const int q = qt * BT + tid;
             const int64_t row = (int64_t)(b * p.Hq + hk * G + gq) * (kPacked ? p.total_q : p.S_q) +
                                 item.q_tok + q;
@@ -753,8 +843,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && !mbar_wait_warp(dk_done, (gs + steps - 1) & 1, p.status)) ok = false;
         if (!ok) break;
         tc_fence_after();
-        store_row<D>(T_dK + lane_base, p.scale, dk_row, row_ok, half);
-        store_row<D>(T_dV + lane_base, 1.0f, dv_row, row_ok, half);
+        if (parted) {
+            store_sums<D>(T_dK + lane_base, p.scale, dk_sum, row_ok, half);
+            store_sums<D>(T_dV + lane_base, 1.0f, dv_sum, row_ok, half);
+        } else {
+            store_row<D>(T_dK + lane_base, p.scale, dk_row, row_ok, half);
+            store_row<D>(T_dV + lane_base, 1.0f, dv_row, row_ok, half);
+        }
         // both accumulators are read out of TMEM: the next item's dV / dK may run
         tc_fence_before();
         __syncwarp();
@@ -1226,6 +1321,27 @@ int launch_bwd(const void* Q, const void* K, const void* V, const void* O, const
     return AMP_OK;
 }
 
+// Parts of the dK/dV pass's sums over a group: as many as six items a CTA allow, none larger
+// than it must be.  A part costs 8 bytes an element, written and read again, and the dQ pass
+// fills idle SMs anyway, so groups under 6 are shared out only where half of the CTAs would
+// have no item, and with an item for every CTA a part keeps four steps.  Forward and backward,
+// whole -> shared out: 8 / 1 heads, 2000 tokens 326 -> 123 us, 10 sequences of up to 8000
+// tokens 1400 -> 912; 28 / 4 heads, 8192 tokens 2400 -> 2106.  What the limits leave out:
+// 32 / 8 heads, 2000 tokens 300 -> 315; 32 / 4 heads, 30 sequences of under 200 tokens 112 -> 174.
+int fa_bwd_parts(int B, int total_kv, int Hq, int Hkv) {
+    const int64_t items = ((int64_t)total_kv / BT + B) * Hkv;   // at most
+    const int64_t sms = sm_count(), group = Hq / Hkv;
+    if (group < 6 && items > sms / 2) return 1;
+    int64_t most = std::min(group, 6 * sms / items);
+    if (items > sms) most = std::min(most, group * total_kv / BT / B / 4);
+    most = std::max<int64_t>(1, most);
+    const int64_t size = (group + most - 1) / most;
+    return (int)((group + size - 1) / size);
+}
+size_t fa_bwd_sums_at(int B, int Hq, int total_q) {
+    return ((varlen_plan_bytes(B) + 15) / 16 * 16 + (size_t)Hq * total_q * 4 + 15) / 16 * 16;
+}
+
 struct PackedBwdArgs {
     const void *Q, *K, *V, *O, *dO;
     const float* lse;
@@ -1267,6 +1383,9 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
     p.dk = a.dK;
     p.dv = a.dV;
     p.total_q = a.total_q;
+    p.total_kv = a.total_kv;
+    p.parts = fa_bwd_parts(a.B, a.total_kv, a.Hq, a.Hkv);
+    p.sums = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + fa_bwd_sums_at(a.B, a.Hq, a.total_q));
     p.after_dkdv = a.total_kv > 0;
     p.dq_tok = s[10];
     p.dq_head = s[11];
@@ -1279,10 +1398,10 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
                                             (varlen_plan_bytes(a.B) + 15) / 16 * 16);
     p.delta = delta;
     // no more CTAs than there can be items
-    const int64_t most_kv = ((int64_t)a.total_kv / BT + a.B) * a.Hkv;
+    const int64_t most_kv = ((int64_t)a.total_kv / BT + a.B) * a.Hkv * p.parts;
     const int64_t most_q = ((int64_t)a.total_q / BT + a.B) * a.Hq;
     const int64_t rows = (int64_t)a.total_q * a.Hq;
-    if ((rc = varlen_make_plan(p.plan, std::max(most_kv, most_q), a.Hq, a.Hkv, true, rows == 0, st)))
+    if ((rc = varlen_make_plan(p.plan, std::max(most_kv, most_q), a.Hq, a.Hkv, true, p.parts, rows == 0, st)))
         return rc;
     if (rows > 0) {
         const int64_t per_block = 8 * (32 / (D / 8)) * kDeltaLoads;
@@ -1307,6 +1426,10 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
                                    dim3((unsigned)std::min<int64_t>(most_q, sm_count())),
                                    dim3(kThreads), CF::SMEM_Q, st, tq, tk, tv, to, p));
     }
+    if (a.total_kv > 0 && p.parts > 1)
+        AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_join<D>,
+                                   dim3((unsigned)std::min((a.total_kv + 7) / 8, sm_count() * 8)), dim3(256), 0,
+                                   st, p));
     return AMP_OK;
 }
 
@@ -1355,9 +1478,12 @@ using namespace ampb;
 
 extern "C" {
 
-size_t amp_flash_attn_varlen_bwd_workspace_bytes(int B, int Hq, int total_q) {
-    if (B <= 0 || Hq <= 0 || total_q < 0) return 0;
-    return (varlen_plan_bytes(B) + 15) / 16 * 16 + (size_t)Hq * total_q * 4;
+size_t amp_flash_attn_varlen_bwd_workspace_bytes(int B, int Hq, int Hkv, int total_q, int total_kv,
+                                                 int head_dim) {
+    if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || total_q < 0 || total_kv < 0 || head_dim <= 0) return 0;
+    const int parts = fa_bwd_parts(B, total_kv, Hq, Hkv);
+    return fa_bwd_sums_at(B, Hq, total_q) +
+           (parts > 1 ? (size_t)parts * 2 * total_kv * Hkv * head_dim * sizeof(float) : 0);
 }
 
 int amp_flash_attn_varlen_bwd_bf16_dev(const void* Q, const void* K, const void* V, const void* O,
@@ -1369,7 +1495,8 @@ int amp_flash_attn_varlen_bwd_bf16_dev(const void* Q, const void* K, const void*
                                        void* workspace, size_t workspace_bytes, void* stream) {
     int rc = varlen_check(B, total_q, total_kv, Hq, Hkv, head_dim, cu_seqlens_q, cu_seqlens_kv,
                           strides, 16, workspace, workspace_bytes,
-                          amp_flash_attn_varlen_bwd_workspace_bytes(B, Hq, total_q));
+                          amp_flash_attn_varlen_bwd_workspace_bytes(B, Hq, Hkv, total_q, total_kv,
+                                                                    head_dim));
     if (rc) return rc;
     if (total_q == 0 && total_kv == 0) return AMP_OK;
     AMPB_REQUIRE((total_q == 0 || (Q && O && dO && lse && dQ)) && (total_kv == 0 || (K && V && dK && dV)),

@@ -28,7 +28,7 @@ __host__ __device__ __forceinline__ int varlen_tiles(int len) { return (len + 12
 
 // Items of one sequence in each list.
 //   forward: pairs of (query tile, query head) of one kv head
-//   dK/dV:   key tiles of one kv head;  dQ: query tiles of one query head
+//   dK/dV:   key tiles of one kv head, times `parts`;  dQ: query tiles of one query head
 __host__ __device__ __forceinline__ int varlen_fwd_pairs(int q_len, int group) {
     return (varlen_tiles(q_len) * group + 1) / 2;
 }
@@ -67,8 +67,9 @@ struct VarlenPlan {
 // Chooses how the CTAs get their items, and enqueues what that needs: the plan kernel
 // (`backward` selects which lists it fills), or, where `zero` is true, the zeroing of the
 // counters.  most_items: the most that there can be, which is all that the host knows.
-int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward, bool zero,
-                     cudaStream_t st);
+// parts: items of a key tile of a kv head in the dK/dV list.
+int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward, int parts,
+                     bool zero, cudaStream_t st);
 
 // Warp-wide (all lanes call it): the sequence r whose items hold `item`, i.e. the
 // last r with first[r] <= item, where first[] ascends and first[0] <= item < first[B];

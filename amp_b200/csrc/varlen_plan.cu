@@ -27,7 +27,7 @@ __device__ __forceinline__ int length_bucket(int len) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-    k_varlen_plan(VarlenPlan pl, int Hq, int Hkv, int backward, int* status) {
+    k_varlen_plan(VarlenPlan pl, int Hq, int Hkv, int backward, int parts, int* status) {
     __shared__ int at[kBuckets];
     __shared__ int part[32];
     const int tid = threadIdx.x;
@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kPlanThreads)
         int n0 = 0, n1 = 0;
         if (r < pl.B) {
             const VarlenSeq s = pl.seqs()[r];
-            n0 = backward ? varlen_tiles(s.k_len) * Hkv : varlen_fwd_pairs(s.q_len, group) * Hkv;
+            n0 = backward ? varlen_tiles(s.k_len) * Hkv * parts : varlen_fwd_pairs(s.q_len, group) * Hkv;
             n1 = backward ? varlen_tiles(s.q_len) * Hq : 0;
         }
         const int e0 = carry0 + block_scan(n0, part);
@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(kPlanThreads)
 
 }  // namespace
 
-int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward, bool zero,
-                     cudaStream_t st) {
+int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward, int parts,
+                     bool zero, cudaStream_t st) {
     // 32 sequences fit a warp.  Up to four items a CTA, dealing them out in turn loses less than
     // the counter's zeroing and its latency cost (forward of 8 prompts of 22 to 200 tokens:
     // 22.5 -> 20.5 us; forward and backward of 17 sequences of up to 700: 84.0 -> 73.7 us);
@@ -95,7 +95,7 @@ int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool
     int rc = device_status(&status);
     if (rc) return rc;
     AMPB_CHECK_CUDA(launch_pdl(k_varlen_plan, dim3(1), dim3(kPlanThreads), 0, st, plan, Hq, Hkv,
-                               backward ? 1 : 0, status));
+                               backward ? 1 : 0, parts, status));
     return AMP_OK;
 }
 

@@ -256,7 +256,8 @@ PyObject* varlen_bwd(const Args& a) {
                all[i].keys ? p.Hkv : p.Hq, p.D, 8, st + 2 * i);
     const float* l = check_lse(lse, p);
     const at::Tensor ws = scratch(a.maybe(13, "workspace"),
-                                  F.amp_flash_attn_varlen_bwd_workspace_bytes(p.B, p.Hq, p.T), p.dev);
+                                  F.amp_flash_attn_varlen_bwd_workspace_bytes(p.B, p.Hq, p.Hkv, p.T, p.Tk, p.D),
+                                  p.dev);
     run(p.dev, "amp_flash_attn_varlen_bwd_bf16_dev", [&](void* stream) {
         return F.amp_flash_attn_varlen_bwd_bf16_dev(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d_o.data_ptr(), l, dq.data_ptr(),

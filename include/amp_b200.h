@@ -294,7 +294,8 @@ AMP_API int amp_flash_attn_varlen_fwd_bf16_dev(const void* Q, const void* K, con
                                                const int64_t* strides, int causal, float scale,
                                                void* workspace, size_t workspace_bytes,
                                                void* stream);
-AMP_API size_t amp_flash_attn_varlen_bwd_workspace_bytes(int B, int Hq, int total_q);
+AMP_API size_t amp_flash_attn_varlen_bwd_workspace_bytes(int B, int Hq, int Hkv, int total_q,
+                                                         int total_kv, int head_dim);
 AMP_API int amp_flash_attn_varlen_bwd_bf16_dev(const void* Q, const void* K, const void* V,
                                                const void* O, const void* dO, const float* lse,
                                                void* dQ, void* dK, void* dV,

@@ -60,8 +60,12 @@ def test_workspace_sizes(amp_lib):
     assert amp_lib.amp_flash_attn_varlen_workspace_bytes(0) == 0
     small, large = (amp_lib.amp_flash_attn_varlen_workspace_bytes(b) for b in (1, 1000))
     assert 0 < small < large
-    assert amp_lib.amp_flash_attn_varlen_bwd_workspace_bytes(1, 8, 100) >= small + 8 * 100 * 4
-    assert amp_lib.amp_flash_attn_varlen_bwd_workspace_bytes(1, 8, -1) == 0
+    bwd_bytes = amp_lib.amp_flash_attn_varlen_bwd_workspace_bytes
+    assert bwd_bytes(1, 8, 8, 100, 100, 64) >= small + 8 * 100 * 4
+    # few key tiles and a group of 8: fp32 sums of its parts, of dK and of dV
+    assert bwd_bytes(1, 8, 1, 100, 100, 64) >= small + 8 * 100 * 4 + 8 * 2 * 100 * 64 * 4
+    assert bwd_bytes(1, 8, 1, 10 ** 6, 10 ** 6, 64) < 64 + 1000 + 8 * 10 ** 6 * 4
+    assert bwd_bytes(1, 8, 8, -1, 100, 64) == 0 and bwd_bytes(1, 8, 3, 100, 100, 64) == 0
 
 
 def test_python_refuses_what_the_kernels_cannot_read(amp_lib):

@@ -140,6 +140,16 @@ def test_scale(scale, cuda, amp_lib):
           reference(q, k, v, do, lens, lens, True, scale), ALL)
 
 
+@pytest.mark.parametrize("Hq,Hkv,lens", [(8, 1, [300, 1, 0, 129]), (7, 1, [1500]), (12, 4, [900, 70]), (28, 4, [513] * 3)])
+def test_groups_summed_in_parts(Hq, Hkv, lens, cuda, amp_lib):
+    """Few key tiles: the group's query heads are shared out, in parts that need not be equal."""
+    for D in (64, 128):
+        q, k, v, do, cu, _ = make(lens, lens, Hq, Hkv, D, seed=Hq)
+        assert lib().amp_flash_attn_varlen_bwd_workspace_bytes(len(lens), Hq, Hkv, sum(lens), sum(lens), D) \
+            > 64 + 1000 + (Hq + 2 * 2 * Hkv * D) * sum(lens) * 4
+        check(run(q, k, v, do, cu, cu, True), reference(q, k, v, do, lens, lens, True), ALL)
+
+
 def test_more_sequences_than_the_plan_has_threads(cuda, amp_lib):
     lens = [int(n) for n in np.random.default_rng(5).integers(0, 4, 2100)]
     q, k, v, do, cu, _ = make(lens, lens, 2, 1, 64, seed=5)
@@ -219,7 +229,7 @@ def test_gradients_agree_with_differences(cuda, amp_lib):
 
 
 def test_matches_the_rectangular_kernels(cuda, amp_lib):
-    B, S, Hq, Hkv, D = 3, 384, 8, 2, 128
+    B, S, Hq, Hkv, D = 3, 384, 4, 4, 128    # (a group's dK and dV may be summed in parts)
     q, k, v, do, cu, _ = make([S] * B, [S] * B, Hq, Hkv, D, seed=19)
     got = run(q, k, v, do, cu, cu, True)
     dense = [x.cuda().view(B, S, -1, D).transpose(1, 2).contiguous() for x in (q, k, v, do)]
