@@ -50,7 +50,7 @@ SIGNATURES: dict[str, tuple] = {
     "amp_flash_attn_bwd_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "amp_flash_attn_bwd_bf16_dev": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32,
                                            _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
-    "amp_flash_attn_varlen_workspace_bytes": (_sz, [_i32]),
+    "amp_flash_attn_varlen_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "amp_flash_attn_varlen_fwd_bf16_dev": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32,
                                                   _i32, _i32, _i32, _i32, _vp, _i32, _f32, _vp,
                                                   _sz, _vp]),

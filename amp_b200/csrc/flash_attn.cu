@@ -48,6 +48,8 @@
 // only the end of the whole tensor, so a sequence's last K/V tile brings rows of the next
 // sequence: their scores are masked, and warp 2 zeroes those rows of V in shared memory
 // before the PV product may read them (0 * NaN of a neighbour would be NaN).
+// Split mode (few queries over many keys, fa_splits): a pair's K/V tiles are shared out among
+// several items, which leave a normalised O in fp32 and lse; k_fa_join joins them.
 // Measured: 1.04 to 1.17 PFLOP/s on 25 prompts of up to 16384 tokens (32 / 8 heads, D 128),
 // within 3 to 12% of the dense kernel's rate at equal lengths of 1024 to 16384.  What bounds
 // it is the dense kernel's chain of hand-offs per step and about 8 us per item outside the
@@ -116,6 +118,10 @@ struct FaParams {
     int64_t o_tok, o_head;
     int total_q;
     VarlenPlan plan;
+    // split mode: at most so many items of a pair; their O (normalised, fp32
+    // [splits][total_q][Hq][D]) and lse [splits][Hq][total_q]
+    int splits;
+    float *o_split, *lse_split;
 };
 
 // One item of the packed mode, as warp 3 publishes it (n1 == 0: no more items).
@@ -123,6 +129,7 @@ struct PackedItem {
     int q_tok, q_len, k_tok, k_len;   // the sequence's rows in Q and in K / V
     int row0[2], head[2];             // first query row and query head of each tile
     int kv_head, n0, n1;
+    int j0, split;                    // split mode: first K/V tile, and the split
 };
 
 // Softmax warps of the all-gather attention that have stored their rows; one
@@ -150,7 +157,7 @@ template <int D>
 struct FaCfg {
     static constexpr int SLABS = D / 64;
     static constexpr int TILE = SLABS * SLAB_BYTES;
-    // barriers and the TMEM slot take 224 bytes, the packed items two slots of 44
+    // barriers and the TMEM slot take 224 bytes, the packed items two slots of 52
     static constexpr int SMEM = 2 * TILE + KV_STAGES * 2 * TILE + 1024 + 384;
     static constexpr uint32_t IDESC_QK = make_idesc(1, 1, 0, 0, BQ, BKV);
     static constexpr uint32_t IDESC_PV = make_idesc(1, 1, 0, 1, BQ, D);
@@ -161,7 +168,9 @@ struct FaCfg {
 // (see item_at below) instead of one CTA per item, so that the next item's Q and
 // K/V loads and its first QK overlap the current item's last steps and epilogue.
 // kPacked (with kPersist): the items come from the list of packed sequences.
-template <int D, bool kPaged, bool kAllGather = false, bool kPersist = false, bool kPacked = false>
+// kSplit (with kPacked): a pair's K/V tiles are shared out among several items.
+template <int D, bool kPaged, bool kAllGather = false, bool kPersist = false, bool kPacked = false,
+          bool kSplit = false>
 __global__ void __launch_bounds__(kThreads, 1)
     k_flash_fwd(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
            const __grid_constant__ CUtensorMap tmV, const FaParams p) {
@@ -228,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int q0[2];              // first query row of each tile
         int q_tok, k_tok;       // packed: the sequence's first row in Q and in K / V
         int head[2];            // packed: query head of each tile
+        int j0;                 // split: the item's first K/V tile
     };
     auto geo = [&](int bh, int qb) {
         Geo g;
@@ -281,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             g.coff = g.S_kv - g.S_q;
             g.q_tok = same(it.q_tok);
             g.k_tok = same(it.k_tok);
+            g.j0 = kSplit ? same(it.j0) : 0;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 g.q0[t] = same(it.row0[t]);
@@ -395,12 +406,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 tma_load_4d(dst + i * kPageTokens * 128, &tmK, &k_full[s], sl * 64,
                                             0, hk, pages[i]);
                         } else {
-                            tma_load_3d(dst, &tmK, &k_full[s], sl * 64, g.k_tok + j * BKV, g.bh_kv);
+                            tma_load_3d(dst, &tmK, &k_full[s], sl * 64,
+                                        g.k_tok + (kSplit ? g.j0 + j : j) * BKV, g.bh_kv);
                         }
                     }
                     if (!mbar_wait(&v_empty[s], ph ^ 1, p.status)) { ok = false; break; }
                     // packed: a tile past the sequence's end goes to warp 2 first
-                    uint64_t* v_bar = kPacked && (j + 1) * BKV > g.S_kv ? &v_raw[s] : &v_full[s];
+                    const int key0 = (kSplit ? g.j0 + j : j) * BKV;
+                    uint64_t* v_bar = kPacked && key0 + BKV > g.S_kv ? &v_raw[s] : &v_full[s];
                     mbar_arrive_expect_tx(v_bar, CF::TILE);
 #pragma unroll
                     for (int sl = 0; sl < CF::SLABS; ++sl) {
@@ -411,7 +424,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 tma_load_4d(dst + i * kPageTokens * 128, &tmV, v_bar, sl * 64,
                                             0, hk, pages[i]);
                         } else {
-                            tma_load_3d(dst, &tmV, v_bar, sl * 64, g.k_tok + j * BKV, g.bh_kv);
+                            tma_load_3d(dst, &tmV, v_bar, sl * 64,
+                                        g.k_tok + (kSplit ? g.j0 + j : j) * BKV, g.bh_kv);
                         }
                     }
                     if (kPersist && j == 0 && !load_q(1)) { ok = false; break; }
@@ -553,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!st) break;
             __syncwarp();
             if (lane == 0) it_done(k);
-            const int valid = g.S_kv - (g.n1 - 1) * BKV;   // of the last tile
+            const int valid = g.S_kv - ((kSplit ? g.j0 : 0) + g.n1 - 1) * BKV;   // of the last tile
             if (valid < BKV) {
                 const int s = (gkv + g.n1 - 1) % KV_STAGES;
                 bool ok = false;
@@ -575,41 +589,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (kPacked && warp == 3) {
         // draws items ahead of the other warps
         const int group = p.Hq / p.Hkv;
-        VarlenDraw draw(p.plan, 0, [&](const VarlenSeq& s) { return varlen_fwd_pairs(s.q_len, group) * p.Hkv; },
-                        p.status);
+        const int splits = kSplit ? p.splits : 1;
+        VarlenDraw draw(p.plan, 0, [&](const VarlenSeq& s) {
+            return varlen_fwd_pairs(s.q_len, group) * p.Hkv * splits;
+        }, p.status);
+        int drawn = 0;
         for (int k = 0;; ++k) {
             if (k >= 2 && !mbar_wait_warp<true>(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) break;
-            const int item = draw.next(k);
-            PackedItem it = {};
-            if (item < draw.total) {
+            PackedItem it;
+            int item;
+            do {
+                it = PackedItem{};
+                item = draw.next(drawn++);
+                if (item >= draw.total) break;
                 VarlenSeq sq;
-                const int w = draw.find(item, sq);   // number within its sequence
+                int w = draw.find(item, sq);   // number within its sequence
+                int split = 0;
+                if constexpr (kSplit) {
+                    split = w % splits;
+                    w /= splits;
+                }
                 const int pairs = varlen_fwd_pairs(sq.q_len, group);
-                const int tiles = varlen_tiles(sq.q_len);
-                const int pair = pairs - 1 - w % pairs;   // most keys first
+                const VarlenPair pr = varlen_pair(sq, pairs - 1 - w % pairs, group, p.causal);   // most keys first
                 it.kv_head = w / pairs;
                 it.q_tok = sq.q_off;
                 it.q_len = sq.q_len;
                 it.k_tok = sq.k_off;
                 it.k_len = sq.k_len;
-                const int n_all = (sq.k_len + BKV - 1) / BKV;
-                int n[2];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const int sub = 2 * pair + t;
-                    const bool none = sub >= tiles * group;   // the last pair's second half
-                    it.row0[t] = none ? tiles * BQ : sub / group * BQ;
-                    it.head[t] = none ? it.head[0] : it.kv_head * group + sub % group;
-                    n[t] = n_all;
-                    if (none) n[t] = 0;
-                    else if (p.causal) {
-                        const int last = it.row0[t] + BQ - 1 + sq.k_len - sq.q_len;
-                        n[t] = min(n_all, last < 0 ? 0 : last / BKV + 1);
-                    }
+                    it.row0[t] = pr.row0[t];
+                    it.head[t] = it.kv_head * group + pr.head[t];
                 }
-                it.n0 = max(n[0], 1);
-                it.n1 = max(n[1], it.n0);
-            }
+                it.n0 = pr.n[0];
+                it.n1 = pr.n[1];
+                if constexpr (kSplit) {
+                    const int chunk = varlen_chunk(it.n1, splits);
+                    it.split = split;
+                    it.j0 = split * chunk;
+                    it.n1 = min(chunk, it.n1 - it.j0);                       // <= 0: no such split
+                    it.n0 = max(min(chunk, it.n0 - it.j0), 1);   // tile 0 may see none of these keys
+                }
+            } while (kSplit && it.n1 <= 0);
             if (lane == 0) {
                 items[k & 1] = it;
                 mbar_arrive(&it_full[k & 1]);
@@ -653,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int cch = 0; cch < BKV / 32; ++cch)
                 tmem_ld_32x32b_x32(lane_base + s_col + cch * 32, sr[cch]);
             tmem_ld_wait();
-            const int k0 = j * BKV;
+            const int k0 = (kSplit ? g.j0 + j : j) * BKV;
             if (k0 + BKV - 1 > vis_hi) {
 #pragma unroll
                 for (int cch = 0; cch < BKV / 32; ++cch)
@@ -743,6 +764,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     row_ok = row < item.q_len;
                     o_off = (int64_t)(row_ok ? tok : 0) * p.o_tok + head * p.o_head;
                     l_off = (int64_t)head * p.total_q + tok;
+                    if constexpr (kSplit) {
+                        const int64_t first = (int64_t)item.split * p.total_q;
+                        o_off = ((first + (row_ok ? tok : 0)) * p.Hq + head) * D;
+                        l_off += first * p.Hq;
+                    }
                 } else {
                     o_off = ((int64_t)bh * p.S_q + (row_ok ? qi : 0)) * D;
                     l_off = (int64_t)bh * p.S_q + qi;
@@ -751,7 +777,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 // all of O_t into registers (one wait), then O_t is free for the next
                 // item's first PV while this warp normalises and stores
-                if constexpr (kPacked) {
+                if constexpr (kSplit) {
+#pragma unroll
+                    for (int oc = 0; oc < D / 32; ++oc) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(lane_base + o_col + oc * 32, o);
+                        tmem_ld_wait();
+                        if (row_ok)
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                *reinterpret_cast<float4*>(p.o_split + o_off + oc * 32 + e) = make_float4(
+                                    __uint_as_float(o[e]) * inv_l, __uint_as_float(o[e + 1]) * inv_l,
+                                    __uint_as_float(o[e + 2]) * inv_l, __uint_as_float(o[e + 3]) * inv_l);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&o_free[t]);
+                } else if constexpr (kPacked) {
                     // normalised and packed 32 columns at a time: with all of O_t in registers
                     // the loop over the K/V tiles spills
                     uint4 w[D / 8];
@@ -799,7 +841,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                 }
                 }
-                if (row_ok && p.lse) p.lse[l_off] = lse_v;
+                if constexpr (kSplit) {
+                    if (row_ok) p.lse_split[l_off] = lse_v;
+                } else if (row_ok && p.lse) {
+                    p.lse[l_off] = lse_v;
+                }
             } else {
                 // stage this warp's 32 rows (D * 2 bytes each, 16-byte slots swizzled by
                 // row) in the tile's Q buffer: every MMA that read it has completed
@@ -964,6 +1010,60 @@ int launch_fa(const void* Q, const void* K, const void* V, void* O, float* lse, 
     return AMP_OK;
 }
 
+// Joins the splits of every row, in order: with m = max lse_z,
+//   O = sum_z 2^(lse_z - m) O_z / sum_z 2^(lse_z - m)   (lse in units of log 2)
+// A warp a (token, head) row; a row's number of splits follows from its pair, as in the kernel
+// that wrote them.
+template <int D>
+__global__ void __launch_bounds__(256) k_fa_join(const FaParams p) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int group = p.Hq / p.Hkv;
+    constexpr int E = D / 32;   // elements a lane
+    for (int t = blockIdx.x; t < p.total_q; t += gridDim.x) {
+        const VarlenSeq sq = p.plan.load(varlen_find(p.plan.cu_q, p.plan.B, t), p.status);
+        if (t < sq.q_off || t >= sq.q_off + sq.q_len) continue;   // a row of no sequence
+        const int tile = (t - sq.q_off) / BQ;
+        for (int h = threadIdx.x >> 5; h < p.Hq; h += 8) {
+            const VarlenPair pr = varlen_pair(sq, (tile * group + h % group) / 2, group, p.causal);
+            const int chunk = varlen_chunk(pr.n[1], p.splits);
+            const int n = (pr.n[1] + chunk - 1) / chunk;
+            const float* lse = p.lse_split + (int64_t)h * p.total_q + t;
+            float m = -INFINITY;
+            for (int z = 0; z < n; ++z) m = fmaxf(m, lse[(int64_t)z * p.Hq * p.total_q]);
+            float acc[E] = {}, sum = 0.0f;
+            for (int z = 0; z < n; ++z) {
+                const float l = lse[(int64_t)z * p.Hq * p.total_q];
+                const float w = l == -INFINITY ? 0.0f : exp2f((l - m) * 1.4426950408889634f);
+                const float* o = p.o_split + (((int64_t)z * p.total_q + t) * p.Hq + h) * D + lane * E;
+                sum += w;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = fmaf(w, o[e], acc[e]);
+            }
+            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.O) + t * p.o_tok + h * p.o_head + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; e += 2)
+                *reinterpret_cast<uint32_t*>(dst + e) = f32x2_to_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+            if (lane == 0 && p.lse)
+                p.lse[(int64_t)h * p.total_q + t] = sum > 0.0f ? m + logf(sum) : -INFINITY;
+        }
+    }
+}
+
+// Splits of a pair's K/V tiles: where pairs leave CTAs without an item and there are many keys
+// for a query, so many that each CTA has one item, or about two where that is under four.
+// Whole -> shared out: 16 queries, 16384 keys, 32 / 8 heads 305 -> 63 us (two items a CTA: 73);
+// one query, 65536 keys, 8 / 1 heads 1188 -> 60; 256 queries, 8192 keys 137 -> 85.  With as many
+// queries as keys the splits' fp32 rows cost what the shorter chains save (2000 tokens, 8 / 2
+// heads: 47 -> 54 us).
+int fa_splits(int B, int total_q, int total_kv, int Hq) {
+    const int64_t items = (((int64_t)total_q / BQ + B) * Hq + 1) / 2, sms = sm_count();   // at most
+    if (items >= sms || total_kv < 4 * (int64_t)total_q || (int64_t)total_kv / BKV < 6 * (int64_t)B) return 1;
+    return (int)std::min<int64_t>(32, sms / items >= 4 ? sms / items : 2 * sms / items);
+}
+size_t fa_splits_at(int B) { return (varlen_plan_bytes(B) + 15) / 16 * 16; }
+
 struct PackedArgs {
     const void *Q, *K, *V;
     void* O;
@@ -1001,12 +1101,25 @@ int launch_packed(const PackedArgs& a, cudaStream_t st) {
     // no more CTAs than there can be items
     const int64_t most = ((int64_t)a.total_q / BQ + a.B) * a.Hq;
     p.plan = {a.ws, false, false, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
-    if ((rc = varlen_make_plan(p.plan, (most + 1) / 2, a.Hq, a.Hkv, false, 1, true, st))) return rc;
+    p.splits = fa_splits(a.B, a.total_q, a.total_kv, a.Hq);
+    p.o_split = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + fa_splits_at(a.B));
+    p.lse_split = p.o_split + (size_t)p.splits * a.total_q * a.Hq * D;
+    if ((rc = varlen_make_plan(p.plan, (most + 1) / 2 * p.splits, a.Hq, a.Hkv, false, p.splits, true, st)))
+        return rc;
+    const unsigned grid = (unsigned)std::min<int64_t>(most * p.splits, sm_count());
+    if (p.splits > 1) {
+        auto kern = k_flash_fwd<D, false, false, true, true, true>;
+        static std::atomic<uint64_t> allowed{0};
+        AMPB_CHECK_CUDA(allow_smem_once(allowed, kern, FaCfg<D>::SMEM));
+        AMPB_CHECK_CUDA(launch_pdl(kern, dim3(grid), dim3(kThreads), FaCfg<D>::SMEM, st, tq, tk, tv, p));
+        AMPB_CHECK_CUDA(launch_pdl(k_fa_join<D>, dim3((unsigned)std::min(a.total_q, sm_count() * 8)), dim3(256),
+                                   0, st, p));
+        return AMP_OK;
+    }
     auto kern = k_flash_fwd<D, false, false, true, true>;
     static std::atomic<uint64_t> allowed{0};
     AMPB_CHECK_CUDA(allow_smem_once(allowed, kern, FaCfg<D>::SMEM));
-    AMPB_CHECK_CUDA(launch_pdl(kern, dim3((unsigned)std::min<int64_t>(most, sm_count())),
-                               dim3(kThreads), FaCfg<D>::SMEM, st, tq, tk, tv, p));
+    AMPB_CHECK_CUDA(launch_pdl(kern, dim3(grid), dim3(kThreads), FaCfg<D>::SMEM, st, tq, tk, tv, p));
     return AMP_OK;
 }
 
@@ -1129,8 +1242,11 @@ int varlen_check(int B, int total_q, int total_kv, int Hq, int Hkv, int D, const
 
 using namespace ampb;
 
-extern "C" size_t amp_flash_attn_varlen_workspace_bytes(int B) {
-    return B > 0 ? varlen_plan_bytes(B) : 0;
+extern "C" size_t amp_flash_attn_varlen_workspace_bytes(int B, int Hq, int Hkv, int total_q, int total_kv,
+                                                        int head_dim) {
+    if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || total_q < 0 || total_kv < 0 || head_dim <= 0) return 0;
+    const size_t splits = fa_splits(B, total_q, total_kv, Hq);
+    return fa_splits_at(B) + (splits > 1 ? splits * total_q * Hq * (head_dim + 1) * sizeof(float) : 0);
 }
 
 extern "C" int amp_flash_attn_varlen_fwd_bf16_dev(const void* Q, const void* K, const void* V,
@@ -1142,7 +1258,7 @@ extern "C" int amp_flash_attn_varlen_fwd_bf16_dev(const void* Q, const void* K, 
                                                   void* stream) {
     int rc = varlen_check(B, total_q, total_kv, Hq, Hkv, head_dim, cu_seqlens_q, cu_seqlens_kv,
                           strides, 8, workspace, workspace_bytes,
-                          amp_flash_attn_varlen_workspace_bytes(B));
+                          amp_flash_attn_varlen_workspace_bytes(B, Hq, Hkv, total_q, total_kv, head_dim));
     if (rc) return rc;
     if (total_q == 0) return AMP_OK;
     AMPB_REQUIRE(Q && O && (total_kv == 0 || (K && V)), AMP_ERR_INVALID, "NULL tensor");

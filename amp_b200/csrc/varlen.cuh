@@ -27,11 +27,40 @@ struct VarlenSeq {
 __host__ __device__ __forceinline__ int varlen_tiles(int len) { return (len + 127) / 128; }
 
 // Items of one sequence in each list.
-//   forward: pairs of (query tile, query head) of one kv head
+//   forward: pairs of (query tile, query head) of one kv head, times `splits`
 //   dK/dV:   key tiles of one kv head, times `parts`;  dQ: query tiles of one query head
 __host__ __device__ __forceinline__ int varlen_fwd_pairs(int q_len, int group) {
     return (varlen_tiles(q_len) * group + 1) / 2;
 }
+
+// A pair of the forward: its two (query tile, query head) of one kv head, `pair` counting in
+// the order tile major, then the heads; and the K/V tiles that each of them visits.
+struct VarlenPair {
+    int row0[2], head[2];   // first query row; head within the group
+    int n[2];               // n[1] >= n[0] >= 1
+};
+__device__ __forceinline__ VarlenPair varlen_pair(const VarlenSeq& s, int pair, int group, bool causal) {
+    const int tiles = varlen_tiles(s.q_len), n_all = varlen_tiles(s.k_len);
+    VarlenPair r;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int sub = 2 * pair + t;
+        const bool none = sub >= tiles * group;   // the last pair's second half
+        r.row0[t] = none ? tiles * 128 : sub / group * 128;
+        r.head[t] = none ? r.head[0] : sub % group;
+        r.n[t] = none ? 0 : n_all;
+        if (!none && causal) {
+            const int last = r.row0[t] + 127 + s.k_len - s.q_len;
+            r.n[t] = last < 0 ? 0 : min(n_all, last / 128 + 1);
+        }
+    }
+    r.n[0] = max(r.n[0], 1);
+    r.n[1] = max(r.n[1], r.n[0]);
+    return r;
+}
+// K/V tiles of one split of n, where a pair's tiles are shared out among at most `splits`
+// items: an item outside its steps takes as long as four of them.
+__device__ __forceinline__ int varlen_chunk(int n, int splits) { return max((n + splits - 1) / splits, 4); }
 
 // The lists in the caller's workspace:
 //   next   int [16]     items drawn beyond the first of each CTA, one count a list
@@ -67,7 +96,7 @@ struct VarlenPlan {
 // Chooses how the CTAs get their items, and enqueues what that needs: the plan kernel
 // (`backward` selects which lists it fills), or, where `zero` is true, the zeroing of the
 // counters.  most_items: the most that there can be, which is all that the host knows.
-// parts: items of a key tile of a kv head in the dK/dV list.
+// parts: items of a key tile of a kv head in the dK/dV list, or of a pair in the forward's.
 int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward, int parts,
                      bool zero, cudaStream_t st);
 

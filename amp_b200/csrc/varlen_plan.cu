@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kPlanThreads)
         int n0 = 0, n1 = 0;
         if (r < pl.B) {
             const VarlenSeq s = pl.seqs()[r];
-            n0 = backward ? varlen_tiles(s.k_len) * Hkv * parts : varlen_fwd_pairs(s.q_len, group) * Hkv;
+            n0 = (backward ? varlen_tiles(s.k_len) : varlen_fwd_pairs(s.q_len, group)) * Hkv * parts;
             n1 = backward ? varlen_tiles(s.q_len) * Hq : 0;
         }
         const int e0 = carry0 + block_scan(n0, part);

@@ -227,7 +227,8 @@ PyObject* varlen_fwd(const Args& a) {
     packed(out, "out", p.dev, at::kBFloat16, p.T, p.Hq, p.D, 8, st + 6);
     if (!lse.defined()) lse = empty({p.Hq, p.T}, at::kFloat, p.dev);
     float* l = check_lse(lse, p);
-    const at::Tensor ws = scratch(a.maybe(9, "workspace"), F.amp_flash_attn_varlen_workspace_bytes(p.B), p.dev);
+    const at::Tensor ws = scratch(a.maybe(9, "workspace"),
+                                  F.amp_flash_attn_varlen_workspace_bytes(p.B, p.Hq, p.Hkv, p.T, p.Tk, p.D), p.dev);
     run(p.dev, "amp_flash_attn_varlen_fwd_bf16_dev", [&](void* stream) {
         return F.amp_flash_attn_varlen_fwd_bf16_dev(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), l,
                                                     p.cu, p.cu_kv, p.B, p.T, p.Tk, p.Hq, p.Hkv, p.D, st, causal,

@@ -286,7 +286,8 @@ AMP_API int amp_flash_attn_bwd_bf16_dev(const void* Q, const void* K, const void
  * are out of order or outside the tensors is skipped and reported by
  * amp_device_status (AMP_ERR_INVALID).
  * The workspace must not be shared by calls that may overlap. */
-AMP_API size_t amp_flash_attn_varlen_workspace_bytes(int B);
+AMP_API size_t amp_flash_attn_varlen_workspace_bytes(int B, int Hq, int Hkv, int total_q,
+                                                     int total_kv, int head_dim);
 AMP_API int amp_flash_attn_varlen_fwd_bf16_dev(const void* Q, const void* K, const void* V,
                                                void* O, float* lse, const int32_t* cu_seqlens_q,
                                                const int32_t* cu_seqlens_kv, int B, int total_q,

@@ -57,9 +57,13 @@ def test_no_tokens_is_no_work(amp_lib):
 
 
 def test_workspace_sizes(amp_lib):
-    assert amp_lib.amp_flash_attn_varlen_workspace_bytes(0) == 0
-    small, large = (amp_lib.amp_flash_attn_varlen_workspace_bytes(b) for b in (1, 1000))
+    fwd_bytes = amp_lib.amp_flash_attn_varlen_workspace_bytes
+    assert fwd_bytes(0, 8, 8, 100, 100, 64) == 0
+    small, large = (fwd_bytes(b, 8, 8, 100, 100, 64) for b in (1, 1000))
     assert 0 < small < large
+    # few queries over many keys: O and lse of the splits
+    assert fwd_bytes(1, 8, 8, 16, 10000, 64) > small + 2 * 16 * 8 * 65 * 4
+    assert fwd_bytes(1, 8, 8, 10 ** 5, 10 ** 5, 64) <= small + 16
     bwd_bytes = amp_lib.amp_flash_attn_varlen_bwd_workspace_bytes
     assert bwd_bytes(1, 8, 8, 100, 100, 64) >= small + 8 * 100 * 4
     # few key tiles and a group of 8: fp32 sums of its parts, of dK and of dV

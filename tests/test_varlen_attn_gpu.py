@@ -150,6 +150,36 @@ def test_groups_summed_in_parts(Hq, Hkv, lens, cuda, amp_lib):
         check(run(q, k, v, do, cu, cu, True), reference(q, k, v, do, lens, lens, True), ALL)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (3, 1, 128), (4, 4, 64)])
+@pytest.mark.parametrize("pairs", [[(1, 4000)], [(5, 3000), (200, 2500), (0, 700)], [(257, 1100)],
+                                   [(40, 5000), (1, 0), (300, 10)]], ids=str)
+def test_keys_shared_out_where_queries_are_few(pairs, Hq, Hkv, D, causal, cuda, amp_lib):
+    lq, lk = zip(*pairs)
+    assert lib().amp_flash_attn_varlen_workspace_bytes(len(lq), Hq, Hkv, sum(lq), sum(lk), D) > sum(lq) * Hq * D * 8
+    q, k, v, do, cu_q, cu_kv = make(lq, lk, Hq, Hkv, D, seed=41, pad_q=30, pad_kv=30)
+    n, m = sum(lq), sum(lk)
+    want = reference(q[:n], k[:m], v[:m], do[:n], lq, lk, causal)
+    for x, y in ((q, n), (k, m), (v, m), (do, n)):
+        x[y:] = float("nan")
+    check(run(q, k, v, do, cu_q, cu_kv, causal), want, ALL)
+
+
+def test_shared_out_keys_repeat_and_replay(cuda, amp_lib):
+    q, k, v, do, cu_q, cu_kv = (x.cuda() for x in make([3, 200], [3000, 2000], 8, 2, 128, seed=43))
+    one = attention.flash_attn_varlen_fwd(q, k, v, cu_q, cu_kv)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        two = attention.flash_attn_varlen_fwd(q, k, v, cu_q, cu_kv)
+    two[0].fill_(7.0)
+    for _ in range(3):
+        graph.replay()
+        three = attention.flash_attn_varlen_fwd(q, k, v, cu_q, cu_kv)
+        for a, b, c in zip(one, two, three):
+            assert torch.equal(a, b) and torch.equal(a, c)
+
+
 def test_more_sequences_than_the_plan_has_threads(cuda, amp_lib):
     lens = [int(n) for n in np.random.default_rng(5).integers(0, 4, 2100)]
     q, k, v, do, cu, _ = make(lens, lens, 2, 1, 64, seed=5)
