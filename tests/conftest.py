@@ -38,3 +38,16 @@ def cuda():
     if not torch.cuda.is_available():
         pytest.fail("GPU test collected on a machine without CUDA (run with -m 'not gpu')")
     return torch.device("cuda:0")
+
+
+def pytest_collection_modifyitems(items):
+    """test_amp_check_gpu.py validates a library that is built from AMP's sources (oracle/_ref).  Where
+    neither the sources nor an earlier build of them is there, it is skipped with that reason, as its
+    CPU counterpart is; where the sources are there and nothing is built, it fails as it says."""
+    sources = Path(os.environ.get("AMP_REF", "/root/reference")) / "include" / "fp8.hpp"
+    built = [ROOT / "oracle" / "_ref" / n for n in ("amp_validate_kernel", "libamp_check_cuda.so")]
+    if sources.exists() or all(p.exists() for p in built):
+        return
+    for item in items:
+        if item.path.name == "test_amp_check_gpu.py":
+            item.add_marker(pytest.mark.skip(reason="AMP sources absent, oracle/_ref not built"))
