@@ -138,9 +138,6 @@ __device__ unsigned g_fa_allgather_done;
 
 constexpr int kPageTokens = 16;
 
-using Poll = std::false_type;    // how a warp waits for the packed mode's next item
-using Sleep = std::true_type;
-
 __device__ __forceinline__ float lg2_approx(float x) {
     float y;
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -208,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // known, and all 512 columns can only start at column 0 (4 x 4096, 32 / 8 heads: 830
     // -> 903 TFLOP/s).
     const int lane = threadIdx.x & 31;
-    const int warp = kPacked ? __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0) : threadIdx.x >> 5;
+    const int warp = kPacked ? same_in<WholeWarp<false>>(threadIdx.x >> 5) : threadIdx.x >> 5;
     const int n_qb = (p.S_q + 2 * BQ - 1) / (2 * BQ);
     // Items of this CTA, k = 0, 1, ...: 0 = no more, 1 = item (bh, qb), 2 = empty slot.
     // Persistent: unit u = blockIdx.x + (k/2) * gridDim.x pairs query-tile pair
@@ -271,15 +268,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // k-th item of this CTA into g: 0 = no more (or a wait ran out), 1 = an item, 2 = an
     // empty slot.  Packed: read from the ring; the reader releases its slot with it_done.
-    // kSleep: for warps 2 and 3, which have nothing to do for most of an item -- polling,
-    // they took issue slots from the softmax warps of their sub-partitions (a fifth of the
-    // kernel's rate).
-    auto next_item = [&](int k, Geo& g, auto sleep) -> int {
+    // who: the calling lane or warp.  Warps 2 and 3 sleep: they have nothing to do for most of
+    // an item, and polling they took issue slots from the softmax warps of their
+    // sub-partitions (799 against 836 TFLOP/s at 4 x 4096, 32 / 8 heads).
+    auto next_item = [&](int k, Geo& g, auto who) -> int {
+        using Who = decltype(who);
         if constexpr (kPacked) {
-            if (!mbar_wait<decltype(sleep)::value>(&it_full[k & 1], (k >> 1) & 1, p.status)) return 0;
+            if (!Who::wait(&it_full[k & 1], (k >> 1) & 1, p.status)) return 0;
             const PackedItem& it = items[k & 1];
-            const unsigned lanes = __activemask();   // lane 0, or the whole warp
-            auto same = [&](int x) { return __shfl_sync(lanes, x, 0); };
+            auto same = [&](int x) { return same_in<Who>(x); };
             g.n1 = same(it.n1);
             if (g.n1 == 0) return 0;
             g.n0 = same(it.n0);
@@ -360,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 Geo g;
-                const int st = next_item(k, g, Poll{});
+                const int st = next_item(k, g, OneLane{});
                 if (st == 0) break;
                 if (st == 2) continue;
                 it_done(k);
@@ -455,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true, pre0 = false;   // pre0: this item's QK_0 was issued early
             for (int k = 0; ok; ++k) {
                 Geo g;
-                const int st = next_item(k, g, Poll{});
+                const int st = next_item(k, g, OneLane{});
                 if (st == 0) break;
                 if (st == 2) continue;
                 it_done(k);
@@ -500,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             // item's last tile-0 step, whose PV was issued before).
                             Geo gn2;
                             int kn = k + 1, st2;
-                            while ((st2 = next_item(kn, gn2, Poll{})) == 2) ++kn;
+                            while ((st2 = next_item(kn, gn2, OneLane{})) == 2) ++kn;
                             if (st2 == 1) {
                                 const int n0n = gn2.n0;
                                 const int gn = gkv + n1, sn = gn % KV_STAGES;
@@ -563,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int gkv = 0, fixed[KV_STAGES] = {};   // tiles before this item; v_raw phases used
         for (int k = 0;; ++k) {
             Geo g;
-            const int st = __all_sync(0xffffffffu, next_item(k, g, Sleep{}) == 1);
+            const int st = next_item(k, g, WholeWarp<true>{});
             if (!st) break;
             __syncwarp();
             if (lane == 0) it_done(k);
@@ -653,8 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int it = 0; ok; ++it) {
         Geo g;
-        int st_item = next_item(it, g, Poll{});
-        if constexpr (kPacked) st_item = __all_sync(0xffffffffu, st_item == 1);
+        const int st_item = next_item(it, g, WholeWarp<false>{});
         if (st_item == 0) break;
         if (st_item == 2) continue;
         const int bh = g.bh, S_kv = g.S_kv, coff = g.coff;

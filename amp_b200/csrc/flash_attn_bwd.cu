@@ -155,32 +155,25 @@ __device__ __forceinline__ void draw_items(const BwdParams& p, BwdItem* items, u
     }
 }
 
-// Packed: what comes out of shared memory or depends on the warp is not known to be the same
-// in every lane, and what is derived from it would be converted for every MMA; a shuffle
-// from lane 0 makes it known.
-template <bool kPacked>
-__device__ __forceinline__ int same_in_warp(int x) {
-    if constexpr (kPacked) return __shfl_sync(__activemask(), x, 0);
-    else return x;
-}
-
-// Reads the k-th published item; false at the end (or when a wait ran out).
-template <bool kSleep = false>
+// Reads the k-th published item; false at the end (or when a wait ran out).  What comes out of
+// shared memory is not known to be the same in every lane, and what is derived from it would be
+// converted for every MMA; a shuffle from lane 0 makes it known.
+template <typename Who>
 __device__ __forceinline__ bool read_item(int k, const BwdItem* items, uint64_t* it_full,
                                           int* status, BwdItem& it) {
-    if (!mbar_wait<kSleep>(&it_full[k & 1], (k >> 1) & 1, status)) return false;
+    if (!Who::wait(&it_full[k & 1], (k >> 1) & 1, status)) return false;
     const BwdItem& src = items[k & 1];
-    it.live = same_in_warp<true>(src.live);
+    it.live = same_in<Who>(src.live);
     it.b = 0;
-    it.head = same_in_warp<true>(src.head);
-    it.tile = same_in_warp<true>(src.tile);
-    it.g0 = same_in_warp<true>(src.g0);
-    it.heads = same_in_warp<true>(src.heads);
-    it.part = same_in_warp<true>(src.part);
-    it.q_tok = same_in_warp<true>(src.q_tok);
-    it.k_tok = same_in_warp<true>(src.k_tok);
-    it.S_q = same_in_warp<true>(src.S_q);
-    it.S_kv = same_in_warp<true>(src.S_kv);
+    it.head = same_in<Who>(src.head);
+    it.tile = same_in<Who>(src.tile);
+    it.g0 = same_in<Who>(src.g0);
+    it.heads = same_in<Who>(src.heads);
+    it.part = same_in<Who>(src.part);
+    it.q_tok = same_in<Who>(src.q_tok);
+    it.k_tok = same_in<Who>(src.k_tok);
+    it.S_q = same_in<Who>(src.S_q);
+    it.S_kv = same_in<Who>(src.S_kv);
     it.coff = it.S_kv - it.S_q;
     return it.live != 0;
 }
@@ -456,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     BwdItem* items = reinterpret_cast<BwdItem*>(bars + 23);   // [2]
 
     const int lane = threadIdx.x & 31;
-    const int warp = same_in_warp<kPacked>(threadIdx.x >> 5);
+    const int warp = kPacked ? same_in<WholeWarp<false>>(threadIdx.x >> 5) : threadIdx.x >> 5;
     const int G = p.Hq / p.Hkv;
     const int n_kt = (p.S_kv + BT - 1) / BT;
     // Persistent: unit u = blockIdx.x + (k/2) * gridDim.x pairs key tile n_kt-1-q with
@@ -474,9 +467,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         return ((k & 1) && q == n_kt - 1 - q) ? 2 : 1;
     };
     // the same with the item's geometry; packed: from the ring, released with it_done
-    auto next_item = [&](int k, BwdItem& it) -> int {
+    auto next_item = [&](int k, BwdItem& it, auto who) -> int {
         if constexpr (kPacked) {
-            return read_item(k, items, it_full, p.status, it) ? 1 : 0;
+            return read_item<decltype(who)>(k, items, it_full, p.status, it) ? 1 : 0;
         } else {
             int bh_kv, jt;
             const int st = item_at(k, bh_kv, jt);
@@ -554,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 BwdItem it;
-                const int st = next_item(k, it);
+                const int st = next_item(k, it, OneLane{});
                 if (st == 0) break;
                 if (st == 2) continue;
                 it_done(k);
@@ -602,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 BwdItem it;
-                const int st = next_item(k, it);
+                const int st = next_item(k, it, OneLane{});
                 if (st == 0) break;
                 if (st == 2) continue;
                 it_done(k);
@@ -667,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int k = 0; ok; ++k) {
             BwdItem it;
-            const bool any = __all_sync(0xffffffffu, read_item<true>(k, items, it_full, p.status, it));
+            const bool any = read_item<WholeWarp<true>>(k, items, it_full, p.status, it);
             if (!any) break;
             __syncwarp();
             if (lane == 0) it_done(k);
@@ -703,8 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int k = 0; ok; ++k) {
         BwdItem item;
-        int st = next_item(k, item);
-        if constexpr (kPacked) st = __all_sync(0xffffffffu, st == 1);
+        const int st = next_item(k, item, WholeWarp<false>{});
         if (st == 0) break;
         if (st == 2) continue;
         const int b = item.b, hk = item.head, bh_kv = b * p.Hkv + hk;
@@ -917,7 +909,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     BwdItem* items = reinterpret_cast<BwdItem*>(bars + 26);   // [2]
 
     const int lane = threadIdx.x & 31;
-    const int warp = same_in_warp<kPacked>(threadIdx.x >> 5);
+    const int warp = kPacked ? same_in<WholeWarp<false>>(threadIdx.x >> 5) : threadIdx.x >> 5;
     const int n_qt = (p.S_q + BT - 1) / BT;
     const int half_units = (n_qt + 1) / 2;
     const int units = p.B * p.Hq * half_units;
@@ -931,9 +923,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         return ((k & 1) && q == n_qt - 1 - q) ? 2 : 1;
     };
     // the same with the item's geometry; packed: from the ring, released with it_done
-    auto next_item = [&](int k, BwdItem& it) -> int {
+    auto next_item = [&](int k, BwdItem& it, auto who) -> int {
         if constexpr (kPacked) {
-            return read_item(k, items, it_full, p.status, it) ? 1 : 0;
+            return read_item<decltype(who)>(k, items, it_full, p.status, it) ? 1 : 0;
         } else {
             int bh, tile;
             const int st = item_at(k, bh, tile);
@@ -1009,7 +1001,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 BwdItem it;
-                const int st = next_item(k, it);
+                const int st = next_item(k, it, OneLane{});
                 if (st == 0) break;
                 if (st == 1) it_done(k);
                 const int n_kv = st == 1 ? kv_tiles(it) : 0;
@@ -1057,7 +1049,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 BwdItem it;
-                const int st = next_item(k, it);
+                const int st = next_item(k, it, OneLane{});
                 if (st == 0) break;
                 if (st == 1) it_done(k);
                 const int n_kv = st == 1 ? kv_tiles(it) : 0;
@@ -1121,7 +1113,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int k = 0; ok; ++k) {
             BwdItem it;
-            const bool any = __all_sync(0xffffffffu, read_item<true>(k, items, it_full, p.status, it));
+            const bool any = read_item<WholeWarp<true>>(k, items, it_full, p.status, it);
             if (!any) break;
             __syncwarp();
             if (lane == 0) it_done(k);
@@ -1155,8 +1147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int k = 0; ok; ++k) {
         BwdItem item;
-        int st = next_item(k, item);
-        if constexpr (kPacked) st = __all_sync(0xffffffffu, st == 1);
+        const int st = next_item(k, item, WholeWarp<false>{});
         if (st == 0) break;
         if (st == 2) continue;
         const int bh = item.b * p.Hq + item.head;

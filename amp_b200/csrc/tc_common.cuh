@@ -147,6 +147,24 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
     return __all_sync(0xffffffffu, ok);
 }
 
+// Who calls: one lane (lane 0), or every lane of the warp -- and then whether its wait sleeps.
+struct OneLane {
+    static constexpr unsigned lanes = 1u;
+    static __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status) {
+        return mbar_wait(bar, parity, status);
+    }
+};
+template <bool kSleep>
+struct WholeWarp {
+    static constexpr unsigned lanes = 0xffffffffu;
+    static __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status) {
+        return mbar_wait_warp<kSleep>(bar, parity, status);
+    }
+};
+// x as lane 0 has it, known to be the same in every calling lane.
+template <typename Who>
+__device__ __forceinline__ int same_in(int x) { return __shfl_sync(Who::lanes, x, 0); }
+
 // ----------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
