@@ -100,6 +100,21 @@ def test_copy_of_pages_named_twice_is_skipped_and_reported(cuda, amp_lib):
     c.copy([8, 8, 9], [8, 25, 9])              # onto itself: still a source
 
 
+def test_pages_past_32_bits(cuda, amp_lib):
+    Hkv, D = 8, 128
+    pages = (1 << 32) // (Hkv * 16 * D) + 64          # the last pages start past 2^32 elements
+    k, v = (torch.zeros(pages, Hkv, 16, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    last = pages - 1
+    k[last], v[last] = 1.0, 2.0
+    paged.copy_pages(k, v, ints([last, 0]), ints([last - 7, last - 9]))
+    assert (k[last - 7] == 1.0).all() and (v[last - 7] == 2.0).all() and not k[last - 9].any()
+    table, ctx = ints([[last, last - 7, -1], [3, -1, -1]]), ints([20, 5])
+    assert paged.fork_sequences(k, v, table, ctx, ints([0]), ints([1])).all()
+    assert table.tolist() == [[last, last - 7, -1], [last, 0, -1]] and (k[0] == 1.0).all()
+    new, used = paged.compact_pages(k, v, table, ctx)
+    assert new.tolist() == [[2, 1, -1], [2, 0, -1]] and used.item() == 3 and (v[:3] == 2.0).all()
+
+
 @pytest.mark.parametrize("n", [300, 1024, 1025, 3000])
 def test_copy_of_many_pages(n, cuda, amp_lib):
     """Few pairs are compared by the copying blocks, many by a plan: the same pages are left alone."""

@@ -220,6 +220,23 @@ def test_rows_of_no_sequence_are_not_read_nor_written(cuda, amp_lib):
         check({"o": o, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, ref, ALL)
 
 
+@pytest.mark.parametrize("pairs,Hq,Hkv", [([(60, 60), (130, 130)], 4, 2), ([(5, 3000)], 8, 1)], ids=str)
+def test_rows_before_the_first_sequence_are_left_alone(pairs, Hq, Hkv, cuda, amp_lib):
+    lq, lk = zip(*pairs)
+    q, k, v, do, cu_q, cu_kv = make(lq, lk, Hq, Hkv, 64, seed=12, pad_q=9, pad_kv=13)
+    ref = reference(q[9:], k[13:], v[13:], do[9:], lq, lk, True)
+    for x, n in ((q, 9), (do, 9), (k, 13), (v, 13)):
+        x[:n] = float("nan")
+    q, k, v, do, cu_q, cu_kv = (x.cuda() for x in (q, k, v, do, cu_q + 9, cu_kv + 13))
+    o, dq = (torch.full_like(q, 7.0) for _ in range(2))
+    dk, dv = (torch.full_like(k, 7.0) for _ in range(2))
+    lse = torch.full((Hq, len(q)), 7.0, device="cuda")
+    attention.flash_attn_varlen_fwd(q, k, v, cu_q, cu_kv, out=o, lse=lse)
+    attention.flash_attn_varlen_bwd(q, k, v, o, do, lse, cu_q, cu_kv, dq=dq, dk=dk, dv=dv)
+    assert (lse[:, :9] == 7.0).all() and all((x[:n] == 7.0).all() for x, n in ((o, 9), (dq, 9), (dk, 13), (dv, 13)))
+    check({"o": o[9:], "lse": lse[:, 9:], "dq": dq[9:], "dk": dk[13:], "dv": dv[13:]}, ref, ALL)
+
+
 def test_a_sequence_of_nan_leaves_its_neighbours_alone(cuda, amp_lib):
     lens, Hq, Hkv, D = [60, 33, 200, 7], 4, 2, 64
     q, k, v, do, cu, _ = make(lens, lens, Hq, Hkv, D, seed=13)
@@ -342,6 +359,28 @@ def test_offsets_outside_the_tensors_are_skipped_and_reported(offsets, cuda, amp
         ref = reference(q[:50], k[:50], v[:50], do[:50], n, n, True)["o"]
         x = out[rows].double().cpu().numpy()
         assert (np.abs(x - ref[0][rows]) <= ref[1][rows]).all()
+
+
+def test_offsets_past_32_bits(cuda, amp_lib):
+    """Tokens 2^30 elements apart, all tensors side by side in one allocation."""
+    Hq, Hkv, D, T = 4, 2, 64, 6
+    lens = [4, 2]
+    far = torch.zeros((T - 1 << 30) + 8192, dtype=torch.bfloat16, device="cuda")
+    at = 0
+
+    def view(heads, x=None):
+        nonlocal at
+        v = far.as_strided((T, heads, D), (1 << 30, D, 1), at)
+        at += heads * D
+        return v.copy_(x) if x is not None else v
+
+    q, k, v, do, cu, _ = make(lens, lens, Hq, Hkv, D, seed=47)
+    ref = reference(q, k, v, do, lens, lens, True)
+    qv, kv, vv, dov, o = view(Hq, q), view(Hkv, k), view(Hkv, v), view(Hq, do), view(Hq)
+    grads = view(Hq), view(Hkv), view(Hkv)
+    _, lse = attention.flash_attn_varlen_fwd(qv, kv, vv, cu.cuda(), out=o)
+    attention.flash_attn_varlen_bwd(qv, kv, vv, o, dov, lse, cu.cuda(), dq=grads[0], dk=grads[1], dv=grads[2])
+    check(dict(zip(ALL, (o, lse, *grads))), ref, ALL)
 
 
 FIRST_IN_CAPTURE = """
