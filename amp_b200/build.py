@@ -107,7 +107,7 @@ def build_host(force: bool = False) -> Path:
            "-I", str(ROOT / "include"), "-isystem", str(tdir / "include"),
            "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"),
            str(HOST_SRC), "-o", str(tmp), "-L", str(tdir / "lib"), "-ltorch_python", "-ltorch_cpu",
-           "-ltorch", "-lc10", "-lc10_cuda"]
+           "-ltorch_cuda", "-ltorch", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {HOST_SRC.name} failed:\n{r.stderr}")

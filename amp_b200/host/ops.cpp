@@ -15,6 +15,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -128,8 +129,9 @@ int narrow(int64_t x, const char* name) {
     return (int)x;
 }
 
+// Straight from the caching allocator (dev's current stream), without the dispatcher.
 at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev) {
-    return at::empty(sizes, at::TensorOptions().dtype(type).device(dev));
+    return at::detail::empty_cuda(sizes, type, dev, std::nullopt);
 }
 
 at::Tensor scratch(at::Tensor ws, size_t bytes, const at::Device& dev) {
