@@ -275,7 +275,7 @@ int set_angles(RopeParams& p, const int32_t* positions, int64_t pos_stride, int 
     for (int a = std::max(n_axes - 1, 0); a < kMaxAxes - 1; ++a) p.axis_end[a] = INT32_MAX;
     AMPB_REQUIRE(2 * pairs <= p.D, AMP_ERR_INVALID, "rope: sections name %lld pairs, head_dim is %d",
                  (long long)pairs, p.D);
-    AMPB_REQUIRE(n_axes <= 1 || pos_stride >= p.T, AMP_ERR_INVALID,
+    AMPB_REQUIRE(n_axes <= 1 || pos_stride >= p.T || pos_stride == 0, AMP_ERR_INVALID,
                  "rope: the axes' positions overlap (stride %lld < %d tokens)", (long long)pos_stride,
                  p.T);
     p.pairs = (int)pairs;

@@ -4,7 +4,7 @@
 //
 // A decode step makes these calls on a few kilobytes, where the kernels take 2 to 10 us.
 // Checked and called through ctypes, a call cost 18 to 28 us of host time (20 to 25
-// converted arguments, four attribute reads a tensor); here it costs 5 to 8.  The rest of
+// converted arguments, four attribute reads a tensor); here it costs 4 to 8.  The rest of
 // the package calls the C ABI through ctypes (_lib.py); both use the same library: bind()
 // receives the addresses of its functions.
 //
@@ -142,7 +142,13 @@ at::Tensor scratch(at::Tensor ws, size_t bytes, const at::Device& dev) {
     return ws;
 }
 
-// Runs `call(stream)`, which must not raise, with the tensors' device current and its current stream, without the
+// Without the interpreter lock while it lives; an exception passes with the lock held again.
+struct Unlocked {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
+// Runs `call(stream)`, which calls no Python, with the tensors' device current and its current stream, without the
 // interpreter lock, and raises AmpError for a nonzero status.
 template <typename C>
 void run(const at::Device& dev, const char* name, C call) {
@@ -152,10 +158,9 @@ void run(const at::Device& dev, const char* name, C call) {
         c10::cuda::OptionalCUDAGuard guard;
         if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
         void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-        Py_BEGIN_ALLOW_THREADS
+        const Unlocked unlocked;
         rc = call(stream);
         if (rc) message = F.amp_last_error();
-        Py_END_ALLOW_THREADS
     }
     if (rc == 0) return;
     PyObject* e = PyObject_CallFunction(g_amp_error, "sis", name, rc, message.c_str());

@@ -314,7 +314,8 @@ AMP_API int amp_flash_attn_varlen_bwd_bf16_dev(const void* Q, const void* K, con
  * of every head is turned by pos[axis(i)][t] * inv_freq[i]; backward != 0 turns
  * back (the gradient).  Pairs are elements (i, i + pairs), or (2i, 2i + 1) when
  * interleaved != 0; elements from 2 * pairs on pass through.
- *   positions  device int32 [n_axes][pos_stride], the first T of each row used
+ *   positions  device int32 [n_axes][pos_stride], the first T of each row used;
+ *              pos_stride 0: one row for every axis
  *   sections   HOST int32 [n_axes], pairs that follow each axis; n_axes <= 4
  *   inv_freq   device float [pairs]
  *   strides    HOST array: token and head stride in elements of q, q_out, k, k_out

@@ -100,6 +100,26 @@ def test_strides_in_place_and_one_position_row(cuda, amp_lib):
     assert torch.equal(rope.rope_fwd(head_major, None, pos, f)[0], want_q)
 
 
+def test_one_row_of_positions_for_every_axis(cuda, amp_lib):
+    q, k, pos, f = inputs(40, 4, 2, 128, (64,), torch.bfloat16, seed=6)
+    want, got = rope.rope_fwd(q, k, pos, f), rope.rope_fwd(q, k, pos.expand(3, 40), f, (16, 24, 24))
+    assert all(map(torch.equal, got, want))
+
+
+def test_a_tensor_without_storage_is_an_error(cuda, amp_lib):
+    """It has a CUDA device, a type and sizes, so only the address is missing."""
+    class Bare(torch.Tensor):
+        @classmethod
+        def __torch_dispatch__(cls, *args):
+            raise NotImplementedError
+
+    q, _, pos, f = inputs(4, 2, 1, 64, (32,), torch.bfloat16)
+    bare = torch.Tensor._make_wrapper_subclass(Bare, (4, 2, 64), dtype=q.dtype, device=q.device)
+    with pytest.raises(RuntimeError, match="NULL|storage"):
+        rope.rope_fwd(bare, None, pos, f)
+    assert torch.equal(rope.rope_fwd(q, None, pos, f)[0], rope.rope_fwd(q.clone(), None, pos, f)[0])
+
+
 def cache(ctx, Hkv, D, seed=0, spare=3):
     rng = np.random.default_rng(seed)
     need = [-(-c // 16) for c in ctx]
