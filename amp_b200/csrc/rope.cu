@@ -263,8 +263,7 @@ int set_angles(RopeParams& p, const int32_t* positions, int64_t pos_stride, int 
                const int32_t* sections, const float* inv_freq) {
     AMPB_REQUIRE(n_axes >= 0 && n_axes <= kMaxAxes, AMP_ERR_UNSUPPORTED,
                  "rope: %d axes not supported (at most %d)", n_axes, kMaxAxes);
-    AMPB_REQUIRE(n_axes == 0 || (positions && sections && inv_freq), AMP_ERR_INVALID,
-                 "rope: NULL positions, sections or inv_freq");
+    AMPB_REQUIRE(n_axes == 0 || sections, AMP_ERR_INVALID, "rope: NULL sections");
     int64_t pairs = 0;
     for (int a = 0; a < n_axes; ++a) {
         AMPB_REQUIRE(sections[a] >= 0, AMP_ERR_INVALID, "rope: section %d is negative", a);
@@ -273,6 +272,9 @@ int set_angles(RopeParams& p, const int32_t* positions, int64_t pos_stride, int 
     }
     // pairs past the last axis do not exist: later ends are never reached
     for (int a = std::max(n_axes - 1, 0); a < kMaxAxes - 1; ++a) p.axis_end[a] = INT32_MAX;
+    // an empty tensor's address is NULL: no tokens have no positions, no pairs no frequencies
+    AMPB_REQUIRE((n_axes == 0 || p.T == 0 || positions) && (pairs == 0 || inv_freq), AMP_ERR_INVALID,
+                 "rope: NULL positions or inv_freq");
     AMPB_REQUIRE(2 * pairs <= p.D, AMP_ERR_INVALID, "rope: sections name %lld pairs, head_dim is %d",
                  (long long)pairs, p.D);
     AMPB_REQUIRE(n_axes <= 1 || pos_stride >= p.T || pos_stride == 0, AMP_ERR_INVALID,

@@ -319,6 +319,7 @@ AMP_API int amp_flash_attn_varlen_bwd_bf16_dev(const void* Q, const void* K, con
  *   sections   HOST int32 [n_axes], pairs that follow each axis; n_axes <= 4
  *   inv_freq   device float [pairs]
  *   strides    HOST array: token and head stride in elements of q, q_out, k, k_out
+ * T may be 0 (tensors and positions may be NULL then), and so may the pairs (inv_freq may).
  * dtype BF16 or F32; head_dim even, at most 1024.  An output may be its input
  * (same strides); no other overlap.  The angle is reduced in 64 bits.
  * ---------------------------------------------------------------------- */

@@ -68,3 +68,16 @@ def test_python_refuses(amp_lib):
         rope.rope_fwd(q, None, pos, f)        # not on a GPU
     with pytest.raises(ValueError):
         paged.rope_append(q, q, q, q, q, q, q, q, pos, f)
+
+
+@pytest.mark.parametrize("call_of", [rope_call, append_call])
+def test_an_empty_tensor_has_no_address(call_of, amp_lib):
+    """What a caller holds for no tokens: positions, q, k and v at address 0; for no pairs, inv_freq too."""
+    none = dict(T=0, q=None, k=None, qo=None, pos=None)
+    call_of(**none)
+    call_of(**none, sections=(0,), f=None)
+    call_of(**none, sections=(16, 16), axes=2, stride=0)
+    with pytest.raises(AmpError):
+        call_of(**none, f=None)       # pairs without frequencies are refused, however many tokens
+    with pytest.raises(AmpError):
+        call_of(**none, sections=None)

@@ -240,3 +240,36 @@ def test_graph_and_other_stream(cuda, amp_lib):
     torch.cuda.synchronize()
     assert torch.equal(first, second) and torch.equal(first, third)
     assert torch.equal(pools[0][table[0, 2].item(), :, 7], rope.rope_fwd(k, None, pos, f)[0][0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_no_tokens(dtype, cuda, amp_lib):
+    for sections in ((32,), (8, 12, 12)):
+        q, k, pos, f = inputs(0, 4, 2, 64, sections, dtype)
+        for call in (rope.rope_fwd, rope.rope_bwd):
+            a, b = call(q, k, pos, f, sections)
+            assert a.shape == q.shape and b.shape == k.shape
+            assert call(q, None, pos, f, sections)[0].shape == q.shape
+        if dtype == torch.bfloat16:
+            pools, table, ctx = cache([5, 17], 2, 64)
+            cu = torch.zeros(3, dtype=torch.int32, device="cuda")
+            assert paged.rope_append(q, k, k, *pools, table, ctx, cu, pos, f, sections).shape == q.shape
+            paged.append(k, k, *pools, table, ctx, cu)
+            assert all((p == 7.0).all() for p in pools)
+    assert rope.rope_fwd(q, k, pos[0], f)[0].shape == q.shape
+    torch.cuda.synchronize()
+    assert lib().amp_device_status(1) == 0
+
+
+def test_no_pairs_is_a_copy(cuda, amp_lib):
+    q, k, pos, f = inputs(37, 3, 2, 80, (0,), torch.bfloat16)
+    assert f.numel() == 0
+    for sections in (None, (0,)):
+        a, b = rope.rope_fwd(q, k, pos, f, sections)
+        assert torch.equal(a, q) and torch.equal(b, k)
+    pools, table, ctx = cache([37], 2, 80)
+    cu = torch.tensor([0, 37], dtype=torch.int32, device="cuda")
+    assert torch.equal(paged.rope_append(q, k, k, *pools, table, ctx, cu, pos, f), q)
+    fresh, _, _ = cache([37], 2, 80)
+    paged.append(k, k, *fresh, table, ctx, cu)
+    assert all(map(torch.equal, pools, fresh))
