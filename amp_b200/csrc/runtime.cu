@@ -171,8 +171,9 @@ int amp_device_status(int clear) {
     int words[2] = {0, 0};
     AMPB_CHECK_CUDA(cudaDeviceSynchronize());
     AMPB_CHECK_CUDA(cudaMemcpy(words, p, sizeof(words), cudaMemcpyDeviceToHost));
-    const int v = words[0] ? words[0] : words[ampb::kStatusBadIndexInt];
-    if (v && clear) AMPB_CHECK_CUDA(cudaMemset(p, 0, sizeof(words)));
+    // one report a call: with both words set the other one is left for the next
+    const int word = words[0] ? 0 : ampb::kStatusBadIndexInt, v = words[word];
+    if (v && clear) AMPB_CHECK_CUDA(cudaMemset(p + word, 0, sizeof(int)));
     if (v == 2) {
         ampb::set_error(AMP_ERR_INVALID, "a kernel met a page id outside the KV pool "
                         "(device status 2); the affected pages were skipped");

@@ -57,7 +57,9 @@ AMP_API int amp_abi_version(void);
 /* Synchronises the current device and reports whether any kernel's bounded
  * wait expired since the last clear (AMP_ERR_TIMEOUT) -- the device-side
  * failure path of the pipelined tensor-core kernels, which end instead of
- * hanging.  clear != 0 resets the flag. */
+ * hanging -- or a kernel skipped a page, row or offset outside its tensor
+ * (AMP_ERR_INVALID).  clear != 0 resets what this call reports; with a skipped
+ * offset or row beside another report, the next call reports it. */
 AMP_API int amp_device_status(int clear);
 /* The amp_user_* entry points stage their host data in per-device device
  * buffers that grow as needed and are kept across calls, so repeated calls do
