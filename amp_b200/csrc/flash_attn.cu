@@ -1017,8 +1017,8 @@ __global__ void __launch_bounds__(256) k_fa_join(const FaParams p) {
     const int group = p.Hq / p.Hkv;
     constexpr int E = D / 32;   // elements a lane
     for (int t = blockIdx.x; t < p.total_q; t += gridDim.x) {
-        const VarlenSeq sq = p.plan.load(varlen_find(p.plan.cu_q, p.plan.B, t), p.status);
-        if (t < sq.q_off || t >= sq.q_off + sq.q_len) continue;   // a row of no sequence
+        const VarlenSeq sq = varlen_owner<false>(p.plan, t, p.status);
+        if (sq.q_len == 0) continue;   // a row of no sequence
         const int tile = (t - sq.q_off) / BQ;
         for (int h = threadIdx.x >> 5; h < p.Hq; h += 8) {
             const VarlenPair pr = varlen_pair(sq, (tile * group + h % group) / 2, group, p.causal);

@@ -389,8 +389,7 @@ __global__ void __launch_bounds__(256) k_fa_bwd_join(BwdParams p) {
     const int per_row = p.Hkv * (D / 4);
     const int64_t part = (int64_t)p.total_kv * p.Hkv * D;
     for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < p.total_kv; t += gridDim.x * 8) {
-        const VarlenSeq sq = p.plan.load(varlen_find(p.plan.cu_kv, p.plan.B, t), p.status);
-        if (t < sq.k_off || t >= sq.k_off + sq.k_len) continue;   // a token of no sequence
+        if (varlen_owner<true>(p.plan, t, p.status).k_len == 0) continue;   // a token of no sequence
         for (int i = lane; i < 2 * per_row; i += 32) {
             const bool v = i >= per_row;
             const int c = v ? i - per_row : i;   // four elements c * 4 of the token's heads

@@ -118,6 +118,25 @@ __device__ __forceinline__ int varlen_find(const int* first, int B, int item) {
     return lo;
 }
 
+// Warp-wide (all lanes call it, with one t): the sequence that row t of q (kKeys: of k and v)
+// belongs to, or an empty one.  Ascending offsets are searched; where that finds no sequence with
+// the row, it is a row of none or the offsets are out of order, and every sequence is looked at.
+template <bool kKeys>
+__device__ __forceinline__ VarlenSeq varlen_owner(const VarlenPlan& plan, int t, int* status) {
+    auto holds = [&](const VarlenSeq& s) {
+        return t >= (kKeys ? s.k_off : s.q_off) && t < (kKeys ? s.k_off + s.k_len : s.q_off + s.q_len);
+    };
+    const VarlenSeq found = plan.load(varlen_find(kKeys ? plan.cu_kv : plan.cu_q, plan.B, t), status);
+    if (holds(found)) return found;
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < plan.B; b0 += 32) {
+        const bool mine = b0 + lane < plan.B && holds(plan.load(b0 + lane, status));
+        const unsigned who = __ballot_sync(0xffffffffu, mine);
+        if (who) return plan.load(b0 + __ffs(who) - 1, status);
+    }
+    return {0, 0, 0, 0};
+}
+
 // How a CTA's drawing warp gets its items.
 //   lists    (more than 32 sequences) the sequences by length and the items before each come
 //            from the plan kernel; otherwise lane r holds the r-th longest sequence, which

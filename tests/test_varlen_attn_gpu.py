@@ -416,3 +416,33 @@ def test_no_key_anywhere_with_many_items(cuda, amp_lib):
     for _ in range(5):
         got = run(q, k[:0], v[:0], do, cu, none, True)
         assert not got["dq"].any() and not got["o"].any() and (got["lse"] == -np.inf).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,cu_q,cu_kv,Tk", [
+    (4, 2, [0, 200, 50, 100], [0, 3000, 500, 2000], 2600),     # keys and heads shared out
+    (8, 1, [0, 200, 50, 100], [0, 200, 50, 100], 100),         # heads shared out in the backward
+    (8, 1, [0, 200, 50, 100], [0, 3000, 500, 2000], 2600),
+    (8, 1, [70, 20, 101, 50, 60], [1900, 100, 4001, 300, 800], 4000),
+], ids=str)
+def test_a_sequence_after_bad_offsets_is_whole(Hq, Hkv, cu_q, cu_kv, Tk, cuda, amp_lib):
+    """Offsets that do not ascend: the last sequence is the only one within its tensors."""
+    T, D, B = 100, 64, len(cu_q) - 1
+    assert (amp_lib.amp_flash_attn_varlen_workspace_bytes(B, Hq, Hkv, T, Tk, D) > T * Hq * D * 8) == (Tk > 100)
+    assert amp_lib.amp_flash_attn_varlen_bwd_workspace_bytes(B, Hq, Hkv, T, Tk, D) \
+        > 64 + 1000 + (Hq * T + 2 * Hkv * D * Tk) * 4
+    q, k, v, do, _, _ = make([T], [Tk], Hq, Hkv, D, seed=53)
+    Q, K = slice(*cu_q[-2:]), slice(*cu_kv[-2:])
+    lq, lk = Q.stop - Q.start, K.stop - K.start
+    ref = reference(q[Q], k[K], v[K], do[Q], [lq], [lk], True)
+    q, k, v, do = (x.cuda() for x in (q, k, v, do))
+    cu, cukv = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (cu_q, cu_kv))
+    o, dq = (torch.full_like(q, 7.0) for _ in range(2))
+    dk, dv = (torch.full_like(k, 7.0) for _ in range(2))
+    lse = torch.full((Hq, T), 7.0, device="cuda")
+    attention.flash_attn_varlen_fwd(q, k, v, cu, cukv, out=o, lse=lse)
+    attention.flash_attn_varlen_bwd(q, k, v, o, do, lse, cu, cukv, dq=dq, dk=dk, dv=dv)
+    assert amp_lib.amp_device_status(1) == -1 and amp_lib.amp_device_status(1) == 0
+    check({"o": o[Q], "lse": lse[:, Q], "dq": dq[Q], "dk": dk[K], "dv": dv[K]}, ref, ALL)
+    for x, rows in ((o, Q), (dq, Q), (dk, K), (dv, K), (lse.T, Q)):
+        x[rows] = 7.0
+        assert (x == 7.0).all()                                # nothing else was written
