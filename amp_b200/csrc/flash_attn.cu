@@ -1047,16 +1047,21 @@ __global__ void __launch_bounds__(256) k_fa_join(const FaParams p) {
     }
 }
 
-// Splits of a pair's K/V tiles: where pairs leave CTAs without an item and there are many keys
-// for a query, so many that each CTA has one item, or about two where that is under four.
-// Whole -> shared out: 16 queries, 16384 keys, 32 / 8 heads 305 -> 63 us (two items a CTA: 73);
-// one query, 65536 keys, 8 / 1 heads 1188 -> 60; 256 queries, 8192 keys 137 -> 85.  With as many
-// queries as keys the splits' fp32 rows cost what the shorter chains save (2000 tokens, 8 / 2
-// heads: 47 -> 54 us).
-int fa_splits(int B, int total_q, int total_kv, int Hq) {
-    const int64_t items = (((int64_t)total_q / BQ + B) * Hq + 1) / 2, sms = sm_count();   // at most
-    if (items >= sms || total_kv < 4 * (int64_t)total_q || (int64_t)total_kv / BKV < 6 * (int64_t)B) return 1;
-    return (int)std::min<int64_t>(32, sms / items >= 4 ? sms / items : 2 * sms / items);
+// Splits of a pair's K/V tiles: where pairs leave CTAs without an item, or half a round of them
+// without a second one, and there are many keys for a query; so many that each CTA has one item, or
+// about two where that is under four.  The number of items is that of equally long sequences, the
+// host knows no more.
+// Whole -> shared out (inside a graph): 16 queries, 16384 keys, 32 / 8 heads 305 -> 56 us (two
+// items a CTA: 73); one query, 65536 keys, 8 / 1 heads 1188 -> 55; 256 queries, 8192 keys, 32 / 8 heads
+// 137 -> 52; at the limit, one query and 4096 keys a sequence, 32 / 32 heads: 6 sequences (192 items)
+// 164 -> 139, 8 sequences (256 items) 165 -> 180.  With as many queries as keys the splits' fp32 rows
+// cost what the shorter chains save (2000 tokens, 8 / 2 heads: 47 -> 54 us).
+int fa_splits(int B, int total_q, int total_kv, int Hq, int Hkv) {
+    // items, if the sequences are equally long
+    const int64_t len = std::max(1, (int)(((int64_t)total_q + B - 1) / B)), sms = sm_count();
+    const int64_t items = (int64_t)B * Hkv * varlen_fwd_pairs((int)len, Hq / Hkv);
+    if (items >= sms * 3 / 2 || total_kv < 4 * (int64_t)total_q || (int64_t)total_kv / BKV < 6 * (int64_t)B) return 1;
+    return (int)std::min<int64_t>(32, sms / items >= 4 ? sms / items : std::max<int64_t>(2, 2 * sms / items));
 }
 size_t fa_splits_at(int B) { return (varlen_plan_bytes(B) + 15) / 16 * 16; }
 
@@ -1094,15 +1099,13 @@ int launch_packed(const PackedArgs& a, cudaStream_t st) {
     p.o_tok = a.strides[6];
     p.o_head = a.strides[7];
     p.total_q = a.total_q;
-    // no more CTAs than there can be items
-    const int64_t most = ((int64_t)a.total_q / BQ + a.B) * a.Hq;
     p.plan = {a.ws, false, false, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
-    p.splits = fa_splits(a.B, a.total_q, a.total_kv, a.Hq);
+    p.splits = fa_splits(a.B, a.total_q, a.total_kv, a.Hq, a.Hkv);
     p.o_split = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + fa_splits_at(a.B));
     p.lse_split = p.o_split + (size_t)p.splits * a.total_q * a.Hq * D;
-    if ((rc = varlen_make_plan(p.plan, (most + 1) / 2 * p.splits, a.Hq, a.Hkv, false, p.splits, true, st)))
-        return rc;
-    const unsigned grid = (unsigned)std::min<int64_t>(most * p.splits, sm_count());
+    const int64_t most = varlen_most_pairs(a.B, a.total_q, a.Hq, a.Hkv) * p.splits;
+    if ((rc = varlen_make_plan(p.plan, most, a.Hq, a.Hkv, false, p.splits, true, st))) return rc;
+    const unsigned grid = (unsigned)std::min<int64_t>(most, sm_count());   // no more CTAs than items
     if (p.splits > 1) {
         auto kern = k_flash_fwd<D, false, false, true, true, true>;
         static std::atomic<uint64_t> allowed{0};
@@ -1241,7 +1244,7 @@ using namespace ampb;
 extern "C" size_t amp_flash_attn_varlen_workspace_bytes(int B, int Hq, int Hkv, int total_q, int total_kv,
                                                         int head_dim) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || total_q < 0 || total_kv < 0 || head_dim <= 0) return 0;
-    const size_t splits = fa_splits(B, total_q, total_kv, Hq);
+    const size_t splits = fa_splits(B, total_q, total_kv, Hq, Hkv);
     return fa_splits_at(B) + (splits > 1 ? splits * total_q * Hq * (head_dim + 1) * sizeof(float) : 0);
 }
 

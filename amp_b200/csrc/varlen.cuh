@@ -33,6 +33,13 @@ __host__ __device__ __forceinline__ int varlen_fwd_pairs(int q_len, int group) {
     return (varlen_tiles(q_len) * group + 1) / 2;
 }
 
+// The most pairs that B sequences of total_q tokens in all can have: a sequence has at most one
+// tile more than its tokens fill, and with an odd group half a pair more for a kv head.
+inline int64_t varlen_most_pairs(int B, int total_q, int Hq, int Hkv) {
+    const int64_t tiles = (int64_t)total_q / 128 + B, group = Hq / Hkv;
+    return Hkv * ((tiles * group + (group % 2 ? B : 0)) / 2);
+}
+
 // A pair of the forward: its two (query tile, query head) of one kv head, `pair` counting in
 // the order tile major, then the heads; and the K/V tiles that each of them visits.
 struct VarlenPair {

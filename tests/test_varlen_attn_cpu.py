@@ -79,3 +79,16 @@ def test_python_refuses_what_the_kernels_cannot_read(amp_lib):
         attention.flash_attn_varlen_fwd(q, q, q, cu)          # not on a GPU
     with pytest.raises(ValueError):
         attention.flash_attn_varlen_fwd(q[0], q, q, cu)       # not packed
+
+
+def test_keys_are_shared_out_only_where_ctas_are_idle(amp_lib):
+    """One query tile a sequence: with a group of 1 a kv head is an item of its own, with an odd group
+    half of one more than its heads fill."""
+    size = amp_lib.amp_flash_attn_varlen_workspace_bytes
+
+    def shared(B, Hq, Hkv, lq=1, lk=4096):
+        return size(B, Hq, Hkv, B * lq, B * lk, 128) > size(B, Hq, Hkv, B * lq, B, 128)
+
+    assert shared(4, 64, 8) and shared(1, 64, 64) and shared(2, 64, 64)     # 128, 64, 128 items
+    assert not shared(4, 64, 64) and not shared(40, 12, 4)                  # 256, 320
+    assert shared(4, 28, 4) and not shared(40, 28, 4)                       # 64, 640
