@@ -129,14 +129,19 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Inclusive scan over a block of 1024 threads (`part`: 32 ints of shared memory; the
-// block's total is left in part[31]).
+// Sum of two counts (>= 0), 2^31 - 1 where it is larger.
+__device__ __forceinline__ int add_counts(int a, int b) {
+    return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu);
+}
+
+// Inclusive scan of counts over a block of 1024 threads (`part`: 32 ints of shared memory; the
+// block's total is left in part[31]); sums end at 2^31 - 1.
 __device__ __forceinline__ int block_scan(int v, int* part) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int t = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += t;
+        if (lane >= o) v = add_counts(v, t);
     }
     __syncthreads();   // `part` may still be read from the call before
     if (lane == 31) part[warp] = v;
@@ -146,12 +151,12 @@ __device__ __forceinline__ int block_scan(int v, int* part) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int t = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += t;
+            if (lane >= o) w = add_counts(w, t);
         }
         part[lane] = w;
     }
     __syncthreads();
-    return v + (warp ? part[warp - 1] : 0);
+    return add_counts(v, warp ? part[warp - 1] : 0);
 }
 
 }  // namespace ampb

@@ -1099,12 +1099,12 @@ int launch_packed(const PackedArgs& a, cudaStream_t st) {
     p.o_tok = a.strides[6];
     p.o_head = a.strides[7];
     p.total_q = a.total_q;
-    p.plan = {a.ws, false, false, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
+    p.plan = {a.ws, false, false, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv, {}};
     p.splits = fa_splits(a.B, a.total_q, a.total_kv, a.Hq, a.Hkv);
     p.o_split = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + fa_splits_at(a.B));
     p.lse_split = p.o_split + (size_t)p.splits * a.total_q * a.Hq * D;
     const int64_t most = varlen_most_pairs(a.B, a.total_q, a.Hq, a.Hkv) * p.splits;
-    if ((rc = varlen_make_plan(p.plan, most, a.Hq, a.Hkv, false, p.splits, true, st))) return rc;
+    if ((rc = varlen_make_plan(p.plan, most, 0, a.Hq, a.Hkv, false, p.splits, true, st))) return rc;
     const unsigned grid = (unsigned)std::min<int64_t>(most, sm_count());   // no more CTAs than items
     if (p.splits > 1) {
         auto kern = k_flash_fwd<D, false, false, true, true, true>;

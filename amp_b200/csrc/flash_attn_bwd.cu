@@ -1383,7 +1383,7 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
     p.dk_head = s[13];
     p.dv_tok = s[14];
     p.dv_head = s[15];
-    p.plan = {a.ws, false, false, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv};
+    p.plan = {a.ws, false, false, a.cu_q, a.cu_kv, a.B, a.total_q, a.total_kv, {}};
     float* delta = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) +
                                             (varlen_plan_bytes(a.B) + 15) / 16 * 16);
     p.delta = delta;
@@ -1391,7 +1391,7 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
     const int64_t most_kv = ((int64_t)a.total_kv / BT + a.B) * a.Hkv * p.parts;
     const int64_t most_q = ((int64_t)a.total_q / BT + a.B) * a.Hq;
     const int64_t rows = (int64_t)a.total_q * a.Hq;
-    if ((rc = varlen_make_plan(p.plan, std::max(most_kv, most_q), a.Hq, a.Hkv, true, p.parts, rows == 0, st)))
+    if ((rc = varlen_make_plan(p.plan, most_kv, most_q, a.Hq, a.Hkv, true, p.parts, rows == 0, st)))
         return rc;
     if (rows > 0) {
         const int64_t per_block = 8 * (32 / (D / 8)) * kDeltaLoads;

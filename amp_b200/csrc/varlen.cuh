@@ -15,6 +15,7 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "common.cuh"
 #include "tc_common.cuh"
 
 namespace ampb {
@@ -82,6 +83,7 @@ struct VarlenPlan {
     bool lists, counted;             // which of the ways of VarlenDraw
     const int *cu_q, *cu_kv;         // the offsets themselves
     int B, total_q, total_kv;
+    int most[2];                     // items that each list can have while no two sequences overlap
     __device__ int* next() const { return static_cast<int*>(ws); }
     __device__ VarlenSeq* seqs() const {
         return reinterpret_cast<VarlenSeq*>(static_cast<uint8_t*>(ws) + 64);
@@ -102,10 +104,11 @@ struct VarlenPlan {
 
 // Chooses how the CTAs get their items, and enqueues what that needs: the plan kernel
 // (`backward` selects which lists it fills), or, where `zero` is true, the zeroing of the
-// counters.  most_items: the most that there can be, which is all that the host knows.
+// counters.  most0, most1: the most items of list 0 and 1, which is all that the host knows; offsets
+// that name more (sequences that overlap) get none, so that a call's work is bounded by its sizes.
 // parts: items of a key tile of a kv head in the dK/dV list, or of a pair in the forward's.
-int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward, int parts,
-                     bool zero, cudaStream_t st);
+int varlen_make_plan(VarlenPlan& plan, int64_t most0, int64_t most1, int Hq, int Hkv, bool backward,
+                     int parts, bool zero, cudaStream_t st);
 
 // Warp-wide (all lanes call it): the sequence r whose items hold `item`, i.e. the
 // last r with first[r] <= item, where first[] ascends and first[0] <= item < first[B];
@@ -169,6 +172,10 @@ struct VarlenDraw {
         if (lane < plan.B) s = plan.load(lane, status);
         mine = s;
         number(items(mine));
+        if (total > plan.most[list]) {   // sequences overlap
+            status[kStatusBadIndexInt] = AMP_DEV_ERR_BAD_INDEX;
+            total = 0;
+        }
         if (total <= (int)gridDim.x) return;   // an item a CTA: any order will do
         const int key = s.q_len > s.k_len ? s.q_len : s.k_len;
         int rank = 0, from = 0;
@@ -191,7 +198,7 @@ struct VarlenDraw {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int t = __shfl_up_sync(0xffffffffu, end, o);
-            if (lane >= o) end += t;
+            if (lane >= o) end = add_counts(end, t);
         }
         first = end - n;
         total = __shfl_sync(0xffffffffu, end, 31);

@@ -60,33 +60,39 @@ __global__ void __launch_bounds__(kPlanThreads)
             n0 = (backward ? varlen_tiles(s.k_len) : varlen_fwd_pairs(s.q_len, group)) * Hkv * parts;
             n1 = backward ? varlen_tiles(s.q_len) * Hq : 0;
         }
-        const int e0 = carry0 + block_scan(n0, part);
+        const int e0 = add_counts(carry0, block_scan(n0, part));
         const int last0 = part[31];
         if (r < pl.B) pl.first(0)[r] = e0 - n0;
-        carry0 += last0;
+        carry0 = add_counts(carry0, last0);
         if (backward) {
-            const int e1 = carry1 + block_scan(n1, part);
+            const int e1 = add_counts(carry1, block_scan(n1, part));
             const int last1 = part[31];
             if (r < pl.B) pl.first(1)[r] = e1 - n1;
-            carry1 += last1;
+            carry1 = add_counts(carry1, last1);
         }
     }
     if (tid == 0) {
-        pl.first(0)[pl.B] = carry0;
-        pl.first(1)[pl.B] = carry1;
+        const bool over = carry0 > pl.most[0] || carry1 > pl.most[1];   // sequences overlap: no items
+        if (over) status[kStatusBadIndexInt] = AMP_DEV_ERR_BAD_INDEX;
+        pl.first(0)[pl.B] = over ? 0 : carry0;
+        pl.first(1)[pl.B] = over ? 0 : carry1;
     }
 }
 
 }  // namespace
 
-int varlen_make_plan(VarlenPlan& plan, int64_t most_items, int Hq, int Hkv, bool backward, int parts,
-                     bool zero, cudaStream_t st) {
+int varlen_make_plan(VarlenPlan& plan, int64_t most0, int64_t most1, int Hq, int Hkv, bool backward,
+                     int parts, bool zero, cudaStream_t st) {
+    AMPB_REQUIRE(most0 <= INT32_MAX / 2 && most1 <= INT32_MAX / 2, AMP_ERR_UNSUPPORTED,
+                 "packed attention too large");
+    plan.most[0] = (int)most0;
+    plan.most[1] = (int)most1;
     // 32 sequences fit a warp.  Up to four items a CTA, dealing them out in turn loses less than
     // the counter's zeroing and its latency cost (forward of 8 prompts of 22 to 200 tokens:
     // 22.5 -> 20.5 us; forward and backward of 17 sequences of up to 700: 84.0 -> 73.7 us);
     // with more, lengths decide (25 sequences of up to 16384 tokens: 9.3 ms dealt, 8.5 counted).
     plan.lists = plan.B > 32;
-    plan.counted = plan.lists || most_items > 4 * sm_count();
+    plan.counted = plan.lists || std::max(most0, most1) > 4 * sm_count();
     if (!plan.lists) {
         if (plan.counted && zero) AMPB_CHECK_CUDA(cudaMemsetAsync(plan.ws, 0, 64, st));
         return AMP_OK;

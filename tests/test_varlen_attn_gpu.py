@@ -446,3 +446,29 @@ def test_a_sequence_after_bad_offsets_is_whole(Hq, Hkv, cu_q, cu_kv, Tk, cuda, a
     for x, rows in ((o, Q), (dq, Q), (dk, K), (dv, K), (lse.T, Q)):
         x[rows] = 7.0
         assert (x == 7.0).all()                                # nothing else was written
+
+
+@pytest.mark.parametrize("times", [16, 51])
+def test_overlapping_sequences_get_no_work(times, cuda, amp_lib):
+    """The same rows again and again (up to 32 sequences, and more): more tiles than the tensors have."""
+    T, Hq, Hkv, D = 1000, 2, 2, 64
+    q, k, v, do, _, _ = (x.cuda() for x in make([T], [T], Hq, Hkv, D, seed=59))
+    cu = torch.tensor([0, T] * times, dtype=torch.int32, device="cuda")
+    o, dq = (torch.full_like(q, 7.0) for _ in range(2))
+    dk, dv = (torch.full_like(k, 7.0) for _ in range(2))
+    lse = torch.full((Hq, T), 7.0, device="cuda")
+    attention.flash_attn_varlen_fwd(q, k, v, cu, out=o, lse=lse)
+    assert amp_lib.amp_device_status(1) == -1 and amp_lib.amp_device_status(1) == 0
+    attention.flash_attn_varlen_bwd(q, k, v, o, do, lse, cu, dq=dq, dk=dk, dv=dv)
+    assert amp_lib.amp_device_status(1) == -1 and amp_lib.amp_device_status(1) == 0
+    assert all((x == 7.0).all() for x in (o, lse, dq, dk, dv))
+
+
+def test_overlapping_sequences_of_more_items_than_32_bits_count(cuda, amp_lib):
+    T, Hq, Hkv, D, B = 8192, 64, 1, 64, 1 << 22        # 2^21 times 2048 items
+    q, k, v, _, _, _ = (x.cuda() for x in make([T], [T], Hq, Hkv, D, seed=61))
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda").repeat(B // 2 + 1)[:B + 1]
+    o, lse = torch.full_like(q, 7.0), torch.full((Hq, T), 7.0, device="cuda")
+    attention.flash_attn_varlen_fwd(q, k, v, cu, out=o, lse=lse)
+    assert amp_lib.amp_device_status(1) == -1 and amp_lib.amp_device_status(1) == 0
+    assert (o == 7.0).all() and (lse == 7.0).all()
