@@ -747,9 +747,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && !mbar_wait_warp(&pv_done[t], (c_t + nt - 1) & 1, p.status)) ok = false;
         if (ok) {
             tc_fence_after();
-            const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+            // l_run is 0 where no key is visible, and NaN where a score is NaN or +inf
+            const float inv_l = l_run == 0.0f ? 0.0f : 1.0f / l_run;
             const float lse_v =
-                l_run > 0.0f ? (m_run + lg2_approx(l_run)) * 0.69314718055994531f : -INFINITY;
+                l_run == 0.0f ? -INFINITY : (m_run + lg2_approx(l_run)) * 0.69314718055994531f;
             if constexpr (!kAllGather) {
                 // packed: where the row goes is read here, not kept over the K/V tiles -- their
                 // loop has no register to spare
@@ -1036,13 +1037,13 @@ __global__ void __launch_bounds__(256) k_fa_join(const FaParams p) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] = fmaf(w, o[e], acc[e]);
             }
-            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.O) + t * p.o_tok + h * p.o_head + lane * E;
 #pragma unroll
             for (int e = 0; e < E; e += 2)
                 *reinterpret_cast<uint32_t*>(dst + e) = f32x2_to_bf16x2(acc[e] * inv, acc[e + 1] * inv);
             if (lane == 0 && p.lse)
-                p.lse[(int64_t)h * p.total_q + t] = sum > 0.0f ? m + logf(sum) : -INFINITY;
+                p.lse[(int64_t)h * p.total_q + t] = sum == 0.0f ? -INFINITY : m + logf(sum);
         }
     }
 }

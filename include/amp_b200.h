@@ -277,7 +277,8 @@ AMP_API int amp_flash_attn_bwd_bf16_dev(const void* Q, const void* K, const void
  * twice for self-attention).  Lengths may differ and may be 0.  causal != 0:
  * query i sees key j iff j <= i + (keys - queries), i.e. aligned at the end, as
  * paged prefill; a query that sees no key gets O = 0, lse = -inf and zero
- * gradients.  lse [Hq, total_q] fp32 (natural log; may be NULL forward).
+ * gradients, one with a NaN or +inf score NaN in both.  lse [Hq, total_q] fp32
+ * (natural log; may be NULL forward).
  * strides: HOST array of the token and the head stride, in elements, of
  * Q, K, V, O (forward) and of Q, K, V, O, dO, dQ, dK, dV (backward); each a
  * positive multiple of 8, the head dimension contiguous.  scale <= 0 selects

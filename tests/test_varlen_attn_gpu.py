@@ -472,3 +472,21 @@ def test_overlapping_sequences_of_more_items_than_32_bits_count(cuda, amp_lib):
     attention.flash_attn_varlen_fwd(q, k, v, cu, out=o, lse=lse)
     assert amp_lib.amp_device_status(1) == -1 and amp_lib.amp_device_status(1) == 0
     assert (o == 7.0).all() and (lse == 7.0).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("lq,lk,Hq,Hkv,D", [(40, 40, 4, 2, 128), (300, 300, 3, 3, 64), (5, 3000, 8, 2, 128)])
+def test_a_query_that_is_not_finite_has_no_finite_lse(lq, lk, Hq, Hkv, D, bad, cuda, amp_lib):
+    """-inf is the lse of a row that sees nothing; this one sees keys.  Every other row keeps its bits."""
+    q, k, v, _, cu, cukv = (x.cuda() for x in make([lq], [lk], Hq, Hkv, D, seed=67))
+    k[:, :, 0] = k[:, :, 0].abs() + 1                     # a query's inf is in every score as +inf
+    want = attention.flash_attn_varlen_fwd(q, k, v, cu, cukv)
+    q[3, 1, 0] = bad
+    got = attention.flash_attn_varlen_fwd(q, k, v, cu, cukv)
+    assert got[0][3, 1].isnan().all() and got[1][1, 3].isnan()
+    got[0][3, 1], got[1][1, 3] = want[0][3, 1], want[1][1, 3]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    if lq == lk:
+        dense = [x.transpose(0, 1)[None].contiguous() for x in (q, k, v)]
+        o, lse = attention.flash_attn_fwd(*dense, True)
+        assert o[0, 1, 3].isnan().all() and lse[0, 1, 3].isnan() and lse.isnan().sum() == 1
