@@ -163,9 +163,19 @@ def call(name: str, *args) -> int:
 _ops = None
 
 
+def host_abi() -> str:
+    """What host/ops.cpp is compiled against: the interpreter's ABI and torch's build, whose C++
+    layouts it uses.  Compiled into the file, which fits no other."""
+    import sysconfig
+
+    import torch
+    return f"amp_b200 host entries for {sysconfig.get_config_var('SOABI')}, torch {torch.__version__} " \
+           f"({torch.version.git_version})"
+
+
 def ops():
     """The compiled host entries (host/ops.cpp), bound once to the CUDA library's functions; raises
-    if either is not built."""
+    if either is not built, or built for another interpreter or torch."""
     global _ops
     if _ops is None:
         h = lib()
@@ -174,6 +184,9 @@ def ops():
         except ImportError as e:
             raise RuntimeError("amp_b200/_ops.so is missing or does not fit this torch: build it "
                                "with `python -m amp_b200.build`") from e
+        if module.built_for() != host_abi():
+            raise RuntimeError(f"amp_b200/_ops.so is built as {module.built_for()}, this is {host_abi()}: "
+                               "build it with `python -m amp_b200.build`")
         module.bind({n: C.cast(getattr(h, n), C.c_void_p).value for n in module.names()}, AmpError)
         _ops = module
     return _ops

@@ -92,11 +92,14 @@ HOST_LIB = PKG / "_ops.so"
 
 
 def build_host(force: bool = False) -> Path:
-    """The compiled Python entries (host/ops.cpp) against this interpreter's torch."""
-    if not force and not _stale(HOST_LIB, [HOST_SRC] + _deps()):
-        return HOST_LIB
+    """The compiled Python entries (host/ops.cpp) against this interpreter's torch: built again when
+    the sources are newer, or when the file is for another interpreter or torch."""
     import sysconfig
     import torch
+    from ._lib import host_abi
+    if not force and not _stale(HOST_LIB, [HOST_SRC] + _deps()) and \
+            host_abi().encode() in HOST_LIB.read_bytes():
+        return HOST_LIB
     tdir = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parents[1]
     tmp = HOST_LIB.with_suffix(".so.tmp")
@@ -104,6 +107,7 @@ def build_host(force: bool = False) -> Path:
     # a process with torch's
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DAMP_HOST_ABI="{host_abi()}"',
            "-I", str(ROOT / "include"), "-isystem", str(tdir / "include"),
            "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"),
            str(HOST_SRC), "-o", str(tmp), "-L", str(tdir / "lib"), "-ltorch_python", "-ltorch_cpu",

@@ -582,11 +582,15 @@ PyObject* names(PyObject*, PyObject*) {
     return out;
 }
 
+// what this file was compiled against (_lib.host_abi)
+PyObject* built_for(PyObject*, PyObject*) { return PyUnicode_FromString(AMP_HOST_ABI); }
+
 #define ENTRY(name, count) \
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, count>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&bind)), METH_FASTCALL, nullptr},
     {"names", names, METH_NOARGS, nullptr},
+    {"built_for", built_for, METH_NOARGS, nullptr},
     ENTRY(varlen_fwd, 10),
     ENTRY(varlen_bwd, 14),
     ENTRY(rope, 9),

@@ -60,3 +60,32 @@ def test_what_is_no_cuda_tensor_is_refused(i, first, built):
 def test_a_flag_that_has_no_truth_value_is_an_error(built):
     with pytest.raises(ValueError):
         attention.flash_attn_varlen_fwd(X, X, X, I, scale="x")   # the tensors are looked at first
+
+
+def test_a_file_for_another_torch_is_built_again(built, tmp_path, monkeypatch):
+    from amp_b200 import _lib, build
+    copy = tmp_path / "_ops.so"
+    copy.write_bytes(SO.read_bytes())
+    monkeypatch.setattr(build, "HOST_LIB", copy)
+    compiled = []
+
+    def run(cmd, **kw):
+        compiled.append(cmd)
+        Path(cmd[cmd.index("-o") + 1]).write_bytes(b"")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    assert build.build_host() == copy and not compiled           # this torch's, newer than its source
+    monkeypatch.setattr(_lib, "host_abi", lambda: "amp_b200 host entries for another torch")
+    assert build.build_host() == copy and len(compiled) == 1
+    assert any("another torch" in a for a in compiled[0])
+
+
+def test_a_file_for_another_torch_is_not_used(built, monkeypatch):
+    from amp_b200 import _lib
+    assert built.built_for() == _lib.host_abi() and torch.__version__ in built.built_for()
+    monkeypatch.setattr(_lib, "_ops", None)
+    monkeypatch.setattr(torch, "__version__", "0.0")
+    with pytest.raises(RuntimeError, match="torch 0.0.*amp_b200.build"):
+        _lib.ops()
+    assert _lib._ops is None
