@@ -652,6 +652,9 @@ int amp_paged_extend_dev(void* k_pool, void* v_pool, int layers, int num_pages, 
     if ((rc = make_table(t, block_table, const_cast<int32_t*>(ctx_lens), rows, max_pages_per_seq, num_pages)))
         return rc;
     AMPB_REQUIRE(add && ctx_out && done, AMP_ERR_INVALID, "extend: NULL counts or result");
+    // the plan reads add again after it has written lengths and done
+    AMPB_REQUIRE(add != ctx_out && add != done && ctx_out != done && ctx_lens != done, AMP_ERR_INVALID,
+                 "extend: the results may share memory with ctx_lens only, and done with nothing");
     if ((rc = check_ws(workspace, workspace_bytes, amp_paged_extend_workspace_bytes(rows, num_pages)))) return rc;
     if ((rc = device_status(&t.status))) return rc;
     const Moves mv = moves_at(workspace, rows);

@@ -167,8 +167,8 @@ def fork_sequences(k_pool, v_pool, block_table, ctx_lens, parents, children, wor
 def extend_sequences(k_pool, v_pool, block_table, ctx_lens, add, out=None, workspace=None):
     """Gives every row pages for add[b] more tokens (int32 [rows]) and returns (new context lengths,
     done): the pages go into block_table in place, the lengths into `out` (a new tensor by default,
-    or ctx_lens itself).  A partly filled last page that another row names too is copied first.  Rows
-    that do not fit into the table or the pool keep their length, with done 0."""
+    or ctx_lens itself, not add).  A partly filled last page that another row names too is copied
+    first.  Rows that do not fit into the table or the pool keep their length, with done 0."""
     return ops().extend_sequences(k_pool, v_pool, block_table, ctx_lens, add, out, workspace)
 
 

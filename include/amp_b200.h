@@ -419,7 +419,8 @@ AMP_API int amp_paged_fork_dev(void* k_pool, void* v_pool, int layers, int num_p
  * ctx_lens[b] + add[b], done[b] = 1.  A partly filled last page that another row
  * names too is copied first.  A row that would not fit into the table, whose
  * add is negative, or that the pool cannot hold stays as it is, done[b] = 0; once
- * the pool cannot hold one, no later row gets pages.  ctx_out may be ctx_lens. */
+ * the pool cannot hold one, no later row gets pages.  ctx_out may be ctx_lens, not
+ * add. */
 AMP_API size_t amp_paged_extend_workspace_bytes(int rows, int num_pages);
 AMP_API int amp_paged_extend_dev(void* k_pool, void* v_pool, int layers, int num_pages, int Hkv,
                                  int head_dim, int32_t* block_table, const int32_t* ctx_lens,

@@ -81,3 +81,11 @@ def test_workspace_sizes(amp_lib):
     assert amp_lib.amp_paged_compact_workspace_bytes(100) >= 800
     assert amp_lib.amp_paged_copy_workspace_bytes(-1) == 0
     assert amp_lib.amp_paged_fork_workspace_bytes(1, 0) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(add=P + 16, out=P + 16, done=P), dict(add=P + 16, done=P + 16, out=P),
+                                dict(out=P + 16, done=P + 16), dict(ctx=P + 16, done=P + 16, out=P + 32)], ids=str)
+def test_extend_refuses_results_in_each_others_place(kw, amp_lib):
+    with pytest.raises(AmpError, match="share memory") as e:
+        extend(**kw)
+    assert e.value.code == -1

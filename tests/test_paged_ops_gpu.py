@@ -305,3 +305,17 @@ def test_python_refuses(cuda, amp_lib):
                  lambda: paged.free_sequences(c.table.cpu(), c.ctx.cpu(), one.cpu())):
         with pytest.raises(ValueError):
             call()
+
+
+def test_extend_does_not_write_lengths_over_what_it_adds(cuda, amp_lib):
+    """Two rows share a partly filled page, so each has to get a copy: with the lengths in add's place
+    the plan saw rows without tokens."""
+    pool = torch.zeros(8, 1, 16, 64, dtype=torch.bfloat16, device="cuda")
+    table = torch.tensor([[3, -1], [3, -1]], dtype=torch.int32, device="cuda")
+    ctx, add = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([5, 5], [1, 2]))
+    before = table.clone()
+    with pytest.raises(RuntimeError, match="share memory"):
+        paged.extend_sequences(pool, pool.clone(), table, ctx, add, out=add)
+    assert torch.equal(table, before) and add.tolist() == [1, 2]
+    new, done = paged.extend_sequences(pool, pool.clone(), table, ctx, add, out=ctx)
+    assert new.tolist() == [6, 7] and done.tolist() == [1, 1] and table[:, 0].tolist() == [0, 1]
