@@ -88,8 +88,9 @@ def flash_attn_varlen_fwd(q, k, v, cu_seqlens, cu_seqlens_kv=None, causal: bool 
     Sequence b is rows cu_seqlens[b] .. cu_seqlens[b+1] of q, and of k and v by cu_seqlens_kv
     (int32 CUDA tensors; cu_seqlens when None).  Under the causal mask the last query sees every
     key of its sequence.  A query that sees none gets O = 0 and lse = -inf.  Rows that belong to
-    no sequence are not written: in outputs allocated here they are unspecified.  A workspace
-    (uint8, amp_flash_attn_varlen_workspace_bytes) must not be shared by calls that may overlap."""
+    no sequence are not written: in outputs allocated here they are unspecified.  out may be q, and
+    shares no memory with k or v.  A workspace (uint8, amp_flash_attn_varlen_workspace_bytes) must
+    not be shared by calls that may overlap."""
     return ops().varlen_fwd(q, k, v, cu_seqlens, cu_seqlens_kv, causal, scale, out, lse, workspace)
 
 
@@ -98,6 +99,7 @@ def flash_attn_varlen_bwd(q, k, v, o, do, lse, cu_seqlens, cu_seqlens_kv=None, c
     """Backward of flash_attn_varlen_fwd: returns (dQ, dK, dV) shaped like q, k, v, from its
     inputs, its o and lse and the upstream gradient do.  A kv head's dK and dV sum over the query
     heads that share it; the same inputs give the same bits.  dq, dk, dv may be given (parts of a
-    fused projection's gradient, for example); rows of no sequence are not written."""
+    fused projection's gradient, for example) and share no memory with the inputs; rows of no
+    sequence are not written."""
     return ops().varlen_bwd(q, k, v, o, do, lse, cu_seqlens, cu_seqlens_kv, causal, scale, dq, dk, dv,
                             workspace)

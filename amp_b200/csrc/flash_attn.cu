@@ -1264,6 +1264,9 @@ extern "C" int amp_flash_attn_varlen_fwd_bf16_dev(const void* Q, const void* K, 
     AMPB_REQUIRE(Q && O && (total_kv == 0 || (K && V)), AMP_ERR_INVALID, "NULL tensor");
     AMPB_REQUIRE(aligned16(Q) && aligned16(K) && aligned16(V) && aligned16(O), AMP_ERR_INVALID,
                  "Q, K, V, O must be 16-byte aligned");
+    // O in Q's place: an item reads its rows of Q before it writes them, and no other item's
+    AMPB_REQUIRE(O != K && O != V && (O != Q || (strides[0] == strides[6] && strides[1] == strides[7])),
+                 AMP_ERR_INVALID, "packed attention: O shares memory with K or V, or with Q at other strides");
     if (!(scale > 0.0f)) scale = 1.0f / sqrtf((float)head_dim);
     const PackedArgs a = {Q,  K,       V,        O,  lse, cu_seqlens_q, cu_seqlens_kv, B, total_q,
                           total_kv, Hq, Hkv, causal, strides, scale, workspace};

@@ -1494,6 +1494,15 @@ int amp_flash_attn_varlen_bwd_bf16_dev(const void* Q, const void* K, const void*
     AMPB_REQUIRE(aligned16(Q) && aligned16(K) && aligned16(V) && aligned16(O) && aligned16(dO) &&
                      aligned16(dQ) && aligned16(dK) && aligned16(dV),
                  AMP_ERR_INVALID, "tensors must be 16-byte aligned");
+    // the passes overlap: what one has written the other may still have to read
+    const void *grads[3] = {dQ, dK, dV}, *inputs[5] = {Q, K, V, O, dO};
+    for (int i = 0; i < 3; ++i) {
+        for (const void* x : inputs)
+            AMPB_REQUIRE(!grads[i] || grads[i] != x, AMP_ERR_INVALID,
+                         "packed attention: a gradient shares memory with an input");
+        AMPB_REQUIRE(!grads[i] || grads[i] != grads[(i + 1) % 3], AMP_ERR_INVALID,
+                     "packed attention: two gradients share memory");
+    }
     if (!(scale > 0.0f)) scale = 1.0f / sqrtf((float)head_dim);
     const PackedBwdArgs a = {Q,  K,  V,       O,        dO, lse, dQ,     dK,      dV,   cu_seqlens_q,
                              cu_seqlens_kv, B, total_q, total_kv, Hq, Hkv, causal, strides, scale,

@@ -290,6 +290,7 @@ AMP_API int amp_flash_attn_bwd_bf16_dev(const void* Q, const void* K, const void
  * amp_device_status (AMP_ERR_INVALID).  Rows that several sequences name are left
  * unspecified; sequences that overlap so much that they have more tiles than the
  * tensors are reported too, and nothing is computed (every row is unspecified).
+ * O may be Q (same strides); outputs share no memory with other tensors.
  * The workspace must not be shared by calls that may overlap. */
 AMP_API size_t amp_flash_attn_varlen_workspace_bytes(int B, int Hq, int Hkv, int total_q,
                                                      int total_kv, int head_dim);

@@ -92,3 +92,37 @@ def test_keys_are_shared_out_only_where_ctas_are_idle(amp_lib):
     assert shared(4, 64, 8) and shared(1, 64, 64) and shared(2, 64, 64)     # 128, 64, 128 items
     assert not shared(4, 64, 64) and not shared(40, 12, 4)                  # 256, 320
     assert shared(4, 28, 4) and not shared(40, 28, 4)                       # 64, 640
+
+
+def apart(names, **kw):
+    """Addresses of their own for tensors that stay unread."""
+    return {n: P + (i << 12) for i, n in enumerate(names)} | kw
+
+
+FWD_TENSORS, BWD_TENSORS = ("q", "k", "v", "o"), ("q", "k", "v", "o", "do", "dq", "dk", "dv")
+
+
+@pytest.mark.parametrize("other", ["k", "v"])
+def test_forward_refuses_o_in_the_place_of_keys(other, amp_lib):
+    at = apart(FWD_TENSORS)
+    with pytest.raises(AmpError, match="shares memory") as e:
+        fwd(**at | {"o": at[other]})
+    assert e.value.code == -1
+
+
+def test_forward_refuses_o_over_q_at_other_strides(amp_lib):
+    at = apart(FWD_TENSORS)
+    for strides in ((256, 64, 128, 64, 128, 64, 512, 64), (256, 64, 128, 64, 128, 64, 256, 128)):
+        with pytest.raises(AmpError, match="shares memory"):
+            fwd(**at | {"o": at["q"]}, strides=strides)
+
+
+@pytest.mark.parametrize("grad", ["dq", "dk", "dv"])
+@pytest.mark.parametrize("other", BWD_TENSORS)
+def test_backward_refuses_a_gradient_in_another_tensors_place(grad, other, amp_lib):
+    if grad == other:
+        return
+    at = apart(BWD_TENSORS)
+    with pytest.raises(AmpError, match="share") as e:
+        bwd(**at | {grad: at[other]})
+    assert e.value.code == -1

@@ -490,3 +490,21 @@ def test_a_query_that_is_not_finite_has_no_finite_lse(lq, lk, Hq, Hkv, D, bad, c
         dense = [x.transpose(0, 1)[None].contiguous() for x in (q, k, v)]
         o, lse = attention.flash_attn_fwd(*dense, True)
         assert o[0, 1, 3].isnan().all() and lse[0, 1, 3].isnan() and lse.isnan().sum() == 1
+
+
+@pytest.mark.parametrize("pairs", [[(300, 300), (7, 7), (0, 0), (129, 129)], [(5, 3000), (60, 2500)],
+                                   [(700, 700)] * 40], ids=lambda p: str(p[:3]))
+def test_output_in_the_place_of_the_queries(pairs, cuda, amp_lib):
+    Hq, Hkv, D = 8, 2, 64
+    lq, lk = zip(*pairs)
+    q, k, v, _, cu, cukv = (x.cuda() for x in make(lq, lk, Hq, Hkv, D, seed=71, pad_q=9))
+    want, lse = attention.flash_attn_varlen_fwd(q, k, v, cu, cukv)
+    room = torch.cat([q, q], 1)                             # and as part of a larger tensor
+    for place in (q, room[:, :Hq]):
+        before = place.clone()
+        out, lse2 = attention.flash_attn_varlen_fwd(place, k, v, cu, cukv, out=place)
+        n = sum(lq)
+        assert out is place and torch.equal(place[:n], want[:n]) and torch.equal(lse2[:, :n], lse[:, :n])
+        assert torch.equal(place[n:], before[n:])
+    with pytest.raises(RuntimeError, match="shares memory"):
+        attention.flash_attn_varlen_fwd(q[:n, :Hkv], k[:n], v[:n], cu, out=k[:n])
