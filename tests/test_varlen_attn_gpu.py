@@ -508,3 +508,43 @@ def test_output_in_the_place_of_the_queries(pairs, cuda, amp_lib):
         assert torch.equal(place[n:], before[n:])
     with pytest.raises(RuntimeError, match="shares memory"):
         attention.flash_attn_varlen_fwd(q[:n, :Hkv], k[:n], v[:n], cu, out=k[:n])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_keys_of_many_sequences_shared_out(causal, cuda, amp_lib):
+    """More sequences than a warp has lanes (the plan kernel's lists), keys shared out and joined."""
+    Hq, Hkv, D = 4, 1, 128
+    rng = np.random.default_rng(73)
+    lq = [int(x) for x in rng.integers(0, 4, 40)]
+    lk = [int(x) for x in rng.integers(800, 1300, 40)]
+    lk[3] = lq[5] = lq[6] = lk[39] = 0
+    n, m = sum(lq), sum(lk)
+    assert amp_lib.amp_flash_attn_varlen_workspace_bytes(40, Hq, Hkv, n + 30, m + 50, D) > 2 * (n + 30) * Hq * D * 4
+    q, k, v, do, cu_q, cu_kv = make(lq, lk, Hq, Hkv, D, seed=73, pad_q=30, pad_kv=50)
+    want = reference(q[:n], k[:m], v[:m], do[:n], lq, lk, causal)
+    for x, y in ((q, n), (k, m), (v, m), (do, n)):
+        x[y:] = float("nan")
+    got = run(q, k, v, do, cu_q, cu_kv, causal)
+    check(got, want, ALL)
+    again = run(q, k, v, do, cu_q, cu_kv, causal)
+    assert torch.equal(got["o"][:n], again["o"][:n]) and torch.equal(got["lse"][:, :n], again["lse"][:, :n])
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(8, 1), (7, 1)])
+def test_heads_of_many_sequences_summed_in_parts(Hq, Hkv, cuda, amp_lib):
+    D = 64
+    rng = np.random.default_rng(79)
+    lens = [int(x) for x in rng.integers(1, 200, 70)]
+    lens[0] = lens[33] = lens[69] = 0
+    lens[50] = 700
+    n = sum(lens)
+    assert amp_lib.amp_flash_attn_varlen_bwd_workspace_bytes(70, Hq, Hkv, n + 20, n + 20, D) \
+        > 64 + 70 * 24 + (Hq + 2 * 2 * Hkv * D) * (n + 20) * 4
+    q, k, v, do, cu, _ = make(lens, lens, Hq, Hkv, D, seed=79, pad_q=20, pad_kv=20)
+    want = reference(q[:n], k[:n], v[:n], do[:n], lens, lens, True)
+    for x in (q, k, v, do):
+        x[n:] = float("nan")
+    got = run(q, k, v, do, cu, cu, True)
+    check(got, want, ALL)
+    again = run(q, k, v, do, cu, cu, True)
+    assert all(torch.equal(got[x][:n], again[x][:n]) for x in ("dq", "dk", "dv"))
