@@ -197,16 +197,23 @@ __device__ __forceinline__ void move_pages(const Pools& pl, const Moves& mv, int
 }
 
 // ------------------------------------------------------------------ copy
-// A page named twice as a target, or as a source and a target of different pairs, would make
-// the result depend on the order: those pairs are skipped and reported.  A negative number
+// Pairs with one target, or a pair whose source another one writes, would make the result
+// depend on the order: they are skipped and reported.  A negative number
 // and a page onto itself are nothing to do.
 __device__ __forceinline__ bool real_pair(int s, int d, int num_pages) {
     return s >= 0 && d >= 0 && s != d && s < num_pages && d < num_pages;
 }
 
-// Up to kDirectPairs pairs: each block compares its pair with all others itself, which saves
-// the plan's launch (38 pages of 64 KB: 6.9 -> 4.6 us a call).
+// Up to kDirectPairs pairs each block compares its pair with all others itself, for every piece that
+// it copies, which saves the plan's launch (inside a graph, planned -> direct: 38 pairs of 32 KB pages,
+// one layer 3.5 -> 2.5 us, 32 layers 30.0 -> 28.8; 1024 pairs 24.2 -> 24.0 and 741 -> 726).  With pages of
+// less than half a piece the comparisons outweigh the copying once there are more than about 1024
+// pieces a pool (2 KB pages, one layer: 512 pairs 4.1 -> 3.4; 32 layers: 38 pairs 5.5 -> 5.6, 256 pairs
+// 21.8 -> 32.0, 1024 pairs 93.7 -> 157; 8 KB pages, 32 layers: 1024 pairs 188 -> 173).
 constexpr int kDirectPairs = 1024;
+bool copies_direct(const Pools& pl, int n) {
+    return n <= kDirectPairs && (pl.page16 >= kMoveThreads * 2 || (int64_t)n * pl.layers <= 1024);
+}
 __global__ void __launch_bounds__(kMoveThreads)
     k_copy_direct(Pools pl, const int* src, const int* dst, int n, int* status) {
     pdl_wait();
@@ -605,7 +612,7 @@ int amp_paged_copy_pages_dev(void* k_pool, void* v_pool, int layers, int num_pag
     int* status = nullptr;
     if ((rc = device_status(&status))) return rc;
     cudaStream_t st = as_stream(stream);
-    if (n <= kDirectPairs) {
+    if (copies_direct(pl, n)) {
         AMPB_CHECK_CUDA(launch_pdl(k_copy_direct, dim3(move_grid(pl, n, 1)), dim3(kMoveThreads), 0, st, pl, src,
                                    dst, n, status));
         return AMP_OK;

@@ -149,9 +149,9 @@ def rope_append(q, k, v, k_pool, v_pool, block_table, ctx_lens, cu_seqlens, posi
 
 def copy_pages(k_pool, v_pool, src, dst, workspace=None) -> None:
     """Copies page src[i] onto page dst[i] (int32 CUDA tensors) in every layer of the pools
-    [(layers,) pages, Hkv, 16, D].  A negative number, or a page onto itself, is nothing to do; a
-    page that two pairs would write, or one write and another read, is left alone and reported by
-    amp_device_status."""
+    [(layers,) pages, Hkv, 16, D].  A negative number, or a page onto itself, is nothing to do.
+    A page that two pairs would write is left alone, and a pair whose source another pair writes is
+    skipped; amp_device_status reports both."""
     ops().copy_pages(k_pool, v_pool, src, dst, workspace)
 
 

@@ -397,9 +397,9 @@ AMP_API int amp_paged_rope_append_bf16_dev(
  * be shared by calls that may overlap.  Row and page numbers outside their
  * arrays are skipped and reported by amp_device_status (AMP_ERR_INVALID). */
 /* Copies page src[i] onto page dst[i] (device int32 [n]) in every layer.  A negative
- * number, or a page onto itself, is nothing to do.  A page named twice as a
- * target, or as a source and as another pair's target, has no defined order:
- * those pairs are skipped and reported. */
+ * number, or a page onto itself, is nothing to do.  Pairs that name one page as
+ * their target, and a pair whose source is another pair's target, have no defined
+ * order: they are skipped and reported. */
 AMP_API size_t amp_paged_copy_workspace_bytes(int n);
 AMP_API int amp_paged_copy_pages_dev(void* k_pool, void* v_pool, int layers, int num_pages, int Hkv,
                                      int head_dim, const int32_t* src, const int32_t* dst, int n,

@@ -319,3 +319,29 @@ def test_extend_does_not_write_lengths_over_what_it_adds(cuda, amp_lib):
     assert torch.equal(table, before) and add.tolist() == [1, 2]
     new, done = paged.extend_sequences(pool, pool.clone(), table, ctx, add, out=ctx)
     assert new.tolist() == [6, 7] and done.tolist() == [1, 1] and table[:, 0].tolist() == [0, 1]
+
+
+@pytest.mark.parametrize("n,layers,Hkv,D", [(300, 4, 1, 64), (300, 3, 1, 64), (300, 4, 2, 128), (1025, 1, 1, 64)])
+def test_copy_of_many_pairs_by_either_way(n, layers, Hkv, D, cuda, amp_lib):
+    """Around the limits between comparing pairs in place and planning them, with pairs that clash."""
+    pages = 4 * n
+    g = torch.Generator("cuda").manual_seed(n + layers)
+    pools = [torch.randn(layers, pages, Hkv, 16, D, device="cuda", generator=g).bfloat16() for _ in range(2)]
+    perm = torch.randperm(pages, device="cuda", generator=g).int()
+    src, dst = perm[:n].clone(), perm[n:2 * n].clone()
+    src[1], dst[2], src[3] = -1, -5, dst[3]                # nothing to do
+    want = [p.clone() for p in pools]
+    real = [0] + list(range(4, n))
+    for w in want:
+        w[:, dst[real].long()] = w[:, src[real].long()]
+    paged.copy_pages(*pools, src, dst)
+    assert all(map(torch.equal, pools, want)) and lib().amp_device_status(1) == 0
+    dst[7], src[9] = dst[6], dst[8]                        # two onto one page; one from a page that is written
+    dst[10] = pages
+    keep = [0, 4, 5, 8] + list(range(11, n))
+    want = [p.clone() for p in pools]
+    for w in want:
+        w[:, dst[keep].long()] = w[:, src[keep].long()]
+    paged.copy_pages(*pools, src, dst)
+    assert all(map(torch.equal, pools, want))
+    assert lib().amp_device_status(1) == -1 and lib().amp_device_status(1) == 0
