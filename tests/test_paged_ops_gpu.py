@@ -345,3 +345,22 @@ def test_copy_of_many_pairs_by_either_way(n, layers, Hkv, D, cuda, amp_lib):
     paged.copy_pages(*pools, src, dst)
     assert all(map(torch.equal, pools, want))
     assert lib().amp_device_status(1) == -1 and lib().amp_device_status(1) == 0
+
+
+@pytest.mark.parametrize("rows,layers", [(2, 32), (3, 5), (40, 7)])
+def test_extend_copies_shared_pages_in_every_layer(rows, layers, cuda, amp_lib):
+    """More blocks copy than there are rows: each row gets its own copy, whatever the layer."""
+    g = torch.Generator("cuda").manual_seed(rows)
+    pools = [torch.randn(layers, 2 * rows, 8, 16, 128, device="cuda", generator=g).bfloat16() for _ in range(2)]
+    before = [p.clone() for p in pools]
+    last = 2 * rows - 1
+    table, ctx, add = (torch.full((rows, 2), -1), torch.full((rows,), 9), torch.ones(rows))
+    table[:, 0] = last
+    table, ctx, add = (x.int().cuda() for x in (table, ctx, add))
+    new, done = paged.extend_sequences(*pools, table, ctx, add)
+    assert new.tolist() == [10] * rows and done.tolist() == [1] * rows
+    assert table[:, 0].tolist() == list(range(rows))
+    for p, b in zip(pools, before):
+        assert torch.equal(p[:, :rows], b[:, last:].expand(-1, rows, -1, -1, -1))
+        assert torch.equal(p[:, rows:], b[:, rows:])
+    assert lib().amp_device_status(1) == 0
