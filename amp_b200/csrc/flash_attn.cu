@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bool ok = false;
 #pragma unroll
                 for (int i = 0; i < KV_STAGES; ++i)
-                    if (i == s) ok = mbar_wait_warp<true>(&v_raw[i], fixed[i]++ & 1, p.status);
+                    if (i == s) ok = mbar_wait_warp<true, kItemLimits>(&v_raw[i], fixed[i]++ & 1, p.status);
                 if (!ok) break;
                 for (int i = max(valid, 0) * 8 + lane; i < BKV * 8; i += 32)
 #pragma unroll
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }, p.status);
         int drawn = 0;
         for (int k = 0;; ++k) {
-            if (k >= 2 && !mbar_wait_warp<true>(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) break;
+            if (k >= 2 && !mbar_wait_warp<true, kItemLimits>(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) break;
             PackedItem it;
             int item;
             do {

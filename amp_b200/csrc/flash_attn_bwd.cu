@@ -123,7 +123,7 @@ __device__ __forceinline__ void draw_items(const BwdParams& p, BwdItem* items, u
         return kKeys ? varlen_tiles(s.k_len) * p.Hkv * p.parts : varlen_tiles(s.q_len) * p.Hq;
     }, p.status);
     for (int k = 0;; ++k) {
-        if (k >= 2 && !mbar_wait_warp<true>(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) return;
+        if (k >= 2 && !mbar_wait_warp<true, kItemLimits>(&it_empty[k & 1], ((k >> 1) & 1) ^ 1, p.status)) return;
         const int item = draw.next(k);
         BwdItem it = {};
         if (item < draw.total) {
@@ -183,7 +183,7 @@ __device__ __forceinline__ bool read_item(int k, const BwdItem* items, uint64_t*
 __device__ __forceinline__ bool zero_tail(uint64_t* raw, uint32_t parity, uint64_t* full,
                                           uint8_t* tile0, uint8_t* tile1, int slabs, int valid,
                                           int* status) {
-    if (!mbar_wait_warp<true>(raw, parity, status)) return false;
+    if (!mbar_wait_warp<true, kItemLimits>(raw, parity, status)) return false;
     const int lane = threadIdx.x & 31;
     for (int i = valid * 8 + lane; i < BT * 8; i += 32)
         for (int sl = 0; sl < slabs; ++sl) {

@@ -117,8 +117,12 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 }
 
 // Bounded wait for the phase with the given parity to complete.  Returns
-// false (and records a timeout in *status) if it does not within the limit.
-template <bool kSleep = false>
+// false (and records a timeout in *status) if it does not within kLimits limits.
+// A role that waits for whole work items (seconds, at millions of tokens) takes
+// kItemLimits: the roles that do the work wait a step at a time, and where one of
+// them stops, another's limit ends this wait too.
+constexpr int kItemLimits = 64;
+template <bool kSleep = false, int kLimits = 1>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* status) {
     if (mbar_try_wait<kSleep>(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
@@ -128,7 +132,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
     while (true) {
         if (mbar_try_wait<kSleep>(bar, parity)) return true;
         if ((++n & kCheckMask) == 0) {
-            if (wait_expired(globaltimer_ns() - t0, status)) {
+            if (wait_expired((globaltimer_ns() - t0) / kLimits, status)) {
                 atomicExch(status, AMP_DEV_ERR_TIMEOUT);
                 return false;
             }
@@ -141,13 +145,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
 // Warp-uniform form for warps that go on to warp-collective tcgen05.ld/st:
 // every lane waits (each needs the acquire), then the warp agrees, so a lane
 // that gave up never leaves the others stuck at a collective.
-template <bool kSleep = false>
+template <bool kSleep = false, int kLimits = 1>
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status) {
-    const bool ok = mbar_wait<kSleep>(bar, parity, status);
+    const bool ok = mbar_wait<kSleep, kLimits>(bar, parity, status);
     return __all_sync(0xffffffffu, ok);
 }
 
-// Who calls: one lane (lane 0), or every lane of the warp -- and then whether its wait sleeps.
+// Who calls: one lane (lane 0), or every lane of the warp -- and then whether its wait sleeps,
+// as those do that wait for whole items.
 struct OneLane {
     static constexpr unsigned lanes = 1u;
     static __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status) {
@@ -158,7 +163,7 @@ template <bool kSleep>
 struct WholeWarp {
     static constexpr unsigned lanes = 0xffffffffu;
     static __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status) {
-        return mbar_wait_warp<kSleep>(bar, parity, status);
+        return mbar_wait_warp<kSleep, kSleep ? kItemLimits : 1>(bar, parity, status);
     }
 };
 // x as lane 0 has it, known to be the same in every calling lane.

@@ -548,3 +548,22 @@ def test_heads_of_many_sequences_summed_in_parts(Hq, Hkv, cuda, amp_lib):
     check(got, want, ALL)
     again = run(q, k, v, do, cu, cu, True)
     assert all(torch.equal(got[x][:n], again[x][:n]) for x in ("dq", "dk", "dv"))
+
+
+def test_a_short_wait_limit_holds_for_steps_not_for_whole_items(cuda, amp_lib):
+    """Items of several milliseconds under a limit of one: the roles that wait for whole items go on."""
+    q, k, v, do, cu, cukv = (x.cuda() for x in make([130000], [519000], 1, 1, 64, seed=83))
+
+    def step():
+        o, lse = attention.flash_attn_varlen_fwd(q, k, v, cu, cukv, causal=False)
+        return (o, lse, *attention.flash_attn_varlen_bwd(q, k, v, o, do, lse, cu, cukv, causal=False))
+
+    want = step()
+    torch.cuda.synchronize()
+    try:
+        assert amp_lib.amp_set_wait_timeout_ns(1_000_000) == 0
+        got = step()
+        assert amp_lib.amp_device_status(1) == 0, amp_lib.amp_last_error()
+    finally:
+        amp_lib.amp_set_wait_timeout_ns(0)
+    assert all(map(torch.equal, want, got))
