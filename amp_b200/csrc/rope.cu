@@ -302,6 +302,12 @@ int set_tensor(RopeParams& p, int i, const void* in, void* out, int heads, const
     return AMP_OK;
 }
 
+// An output may be its own input, not another tensor's place (NULL: no tensor).
+int check_apart(const void* out, const void* other) {
+    AMPB_REQUIRE(!out || out != other, AMP_ERR_INVALID, "rope: an output shares memory with another tensor");
+    return AMP_OK;
+}
+
 int check_sizes(int T, int Hq, int Hk, int D) {
     AMPB_REQUIRE(T >= 0 && Hq >= 0 && Hk >= 0 && D > 0, AMP_ERR_INVALID, "rope: negative size");
     AMPB_REQUIRE(D % 2 == 0 && D <= 1024 && Hq <= 4096 && Hk <= 4096, AMP_ERR_UNSUPPORTED,
@@ -334,6 +340,9 @@ extern "C" int amp_rope_dev(const void* q, void* q_out, const void* k, void* k_o
     if (T == 0 || p.H == 0) return AMP_OK;
     if ((rc = set_tensor(p, 0, q, q_out, Hq, strides, strides + 2, true))) return rc;
     if ((rc = set_tensor(p, 1, k, k_out, Hk, strides + 4, strides + 6, true))) return rc;
+    if (Hq > 0 && Hk > 0 &&
+        ((rc = check_apart(q_out, k)) || (rc = check_apart(k_out, q)) || (rc = check_apart(q_out, k_out))))
+        return rc;
     return dtype == AMP_DTYPE_BF16
                ? launch_rope<__nv_bfloat16, false>(p, interleaved != 0, as_stream(stream))
                : launch_rope<float, false>(p, interleaved != 0, as_stream(stream));
@@ -362,6 +371,7 @@ extern "C" int amp_paged_rope_append_bf16_dev(
     if ((rc = set_tensor(p, 0, q, q_out, Hq, strides, strides + 2, true))) return rc;
     if ((rc = set_tensor(p, 1, k, nullptr, Hkv, strides + 4, nullptr, false))) return rc;
     if ((rc = set_tensor(p, 2, v, nullptr, Hkv, strides + 6, nullptr, false))) return rc;
+    if (Hq > 0 && ((rc = check_apart(q_out, k)) || (rc = check_apart(q_out, v)))) return rc;
     p.k_pool = k_pool;
     p.v_pool = v_pool;
     p.block_table = block_table;

@@ -14,7 +14,8 @@ def rope_fwd(q, k, positions, inv_freq, sections=None, interleaved: bool = False
              out_k=None):
     """Turns q [tokens, Hq, D] and k [tokens, Hk, D] (bf16 or fp32, any token and head strides; k
     may be None) and returns (q', k').  positions int32 [axes, tokens] (an expanded row is taken
-    as it is) or [tokens], inv_freq fp32 [pairs], sections the pairs of each axis (with one axis: None).  An output may be its input."""
+    as it is) or [tokens], contiguous along the tokens; inv_freq fp32 [pairs], sections the pairs of
+    each axis (with one axis: None).  An output may be its input, and shares no memory with others."""
     return ops().rope(q, k, positions, inv_freq, sections, interleaved, out_q, out_k, False)
 
 

@@ -81,3 +81,15 @@ def test_an_empty_tensor_has_no_address(call_of, amp_lib):
         call_of(**none, f=None)       # pairs without frequencies are refused, however many tokens
     with pytest.raises(AmpError):
         call_of(**none, sections=None)
+
+
+def test_refuses_an_output_in_another_tensors_place(amp_lib):
+    q, qo, k, ko = (P + (i << 12) for i in range(4))
+    for kw in (dict(qo=k), dict(ko=q), dict(qo=ko), dict(qo=q, ko=q)):
+        with pytest.raises(AmpError, match="shares memory") as e:
+            rope_call(**(dict(q=q, qo=qo, k=k, ko=ko) | kw))
+        assert e.value.code == -1
+    for kw in (dict(qo=k), dict(qo=ko)):
+        with pytest.raises(AmpError, match="shares memory") as e:
+            append_call(**(dict(q=q, qo=qo, k=k, v=ko) | kw))
+        assert e.value.code == -1
