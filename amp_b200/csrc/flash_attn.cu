@@ -33,7 +33,11 @@
 //              row per thread: tcgen05.ld the S row, mask, online max in the
 //              log2 domain (scale * log2(e) folded into one packed f32x2 FMA
 //              per two scores), ex2, row sum in fp32 (independent accumulator
-//              chains), P packed to bf16 and tcgen05.st back over S.  O is
+//              chains), P packed to bf16 and tcgen05.st back over S: the tensor
+//              core multiplies 16-bit operands.  That rounding of P (the row sum
+//              takes it unrounded) takes O's error against fp64 from the 0.0016 of
+//              its own rounding to 0.0020; ex2 and lg2 are the hardware's
+//              approximations (2 ulp), far below either.  O is
 //              rescaled (tcgen05.ld/st) only when a row maximum grows by more
 //              than 2^8; otherwise the stale maximum is kept.
 //              Epilogue: O / l to bf16, lse = (m + log2 l) * ln 2.
@@ -50,9 +54,9 @@
 // before the PV product may read them (0 * NaN of a neighbour would be NaN).
 // Split mode (few queries over many keys, fa_splits): a pair's K/V tiles are shared out among
 // several items, which leave a normalised O in fp32 and lse; k_fa_join joins them.
-// Measured: 1.04 to 1.17 PFLOP/s on 25 prompts of up to 16384 tokens (32 / 8 heads, D 128),
-// within 3 to 12% of the dense kernel's rate at equal lengths of 1024 to 16384.  What bounds
-// it is the dense kernel's chain of hand-offs per step and about 8 us per item outside the
+// Measured: 1.04 PFLOP/s on 25 prompts of up to 16384 tokens (32 / 8 heads, D 128); at equal
+// lengths 0.90 to 1.01 of the dense kernel's rate (32 x 1024: 705 and 695 TFLOP/s, 8 x 4096: 978 to
+// 1023 and 1090, 2 x 16384: 1090 and 1130).  What bounds it is the dense kernel's chain of hand-offs per step and about 8 us per item outside the
 // steps, which is most of the time for sequences under 256 tokens.
 //
 // All-gather mode ((batch*head)-sharded attention on the GPUs of one node: the
@@ -1052,9 +1056,8 @@ __global__ void __launch_bounds__(256) k_fa_join(const FaParams p) {
 // without a second one, and there are many keys for a query; so many that each CTA has one item, or
 // about two where that is under four.  The number of items is that of equally long sequences, the
 // host knows no more.
-// Whole -> shared out (inside a graph): 16 queries, 16384 keys, 32 / 8 heads 305 -> 56 us (two
-// items a CTA: 73); one query, 65536 keys, 8 / 1 heads 1188 -> 55; 256 queries, 8192 keys, 32 / 8 heads
-// 137 -> 52; at the limit, one query and 4096 keys a sequence, 32 / 32 heads: 6 sequences (192 items)
+// Whole -> shared out (inside a graph): 16 queries, 16384 keys, 32 / 8 heads 300 -> 56 us; one
+// query, 65536 keys, 8 / 1 heads 1174 -> 56; 256 queries, 8192 keys, 32 / 8 heads 127 -> 52; at the limit, one query and 4096 keys a sequence, 32 / 32 heads: 6 sequences (192 items)
 // 164 -> 139, 8 sequences (256 items) 165 -> 180.  With as many queries as keys the splits' fp32 rows
 // cost what the shorter chains save (2000 tokens, 8 / 2 heads: 47 -> 54 us).
 int fa_splits(int B, int total_q, int total_kv, int Hq, int Hkv) {

@@ -36,7 +36,7 @@
 // dK/dV pass, K and V in the dQ pass) warp 2 zeroes them in shared memory before the
 // MMAs may read them; where they are rows of the output they are just not stored.
 // Measured: 20 documents of up to 8192 tokens (46763 in all, 32 / 8 heads, D 128), forward and
-// backward, 8.5 to 8.9 ms = 725 to 760 TFLOP/s, the dense passes' rate.
+// backward, 8.7 ms = 741 TFLOP/s, the dense passes' rate.
 // Both kernels: 384 threads; warp 0 TMA, warp 1
 // TMEM + MMA issue (warps 2-3 only lend their registers, setmaxnreg 72 / 216);
 // warps 4-11 the element-wise work, two warps per TMEM lane quadrant (one row
@@ -308,7 +308,10 @@ __global__ void __launch_bounds__(256) k_fa_bwd_delta(const __nv_bfloat16* __res
 
 // The P that dS = P (dP - Delta) multiplies with.  Dense: as rounded to bf16 for P^T dO.
 // Packed: as computed, in fp32 (dQ and dK then carry two roundings to bf16, of dS and their
-// own, instead of three: an error of 0.0024 instead of 0.0030 relative to fp64).
+// own, instead of three: an error of 0.0024 instead of 0.0030 relative to fp64; the outputs'
+// rounding alone is 0.0017).  dS is rounded because the tensor core multiplies 16-bit operands.
+// Delta is formed from O as the forward rounded it, the only O there is; in rows of few keys,
+// where one P is near 1, that rounding is felt most (0.0026).
 template <bool kExact>
 struct Probs {
     float v[kExact ? 64 : 1];
@@ -1315,8 +1318,8 @@ int launch_bwd(const void* Q, const void* K, const void* V, const void* O, const
 // than it must be.  A part costs 8 bytes an element, written and read again, and the dQ pass
 // fills idle SMs anyway, so groups under 6 are shared out only where half of the CTAs would
 // have no item, and with an item for every CTA a part keeps four steps.  Forward and backward,
-// whole -> shared out: 8 / 1 heads, 2000 tokens 326 -> 123 us, 10 sequences of up to 8000
-// tokens 1400 -> 912; 28 / 4 heads, 8192 tokens 2400 -> 2106.  What the limits leave out:
+// whole -> shared out: 8 / 1 heads, 2000 tokens 311 -> 114 us, 10 sequences of 200 to 8000
+// tokens 1396 -> 1006; 28 / 4 heads, 8192 tokens 2325 -> 2175.  What the limits leave out:
 // 32 / 8 heads, 2000 tokens 300 -> 315; 32 / 4 heads, 30 sequences of under 200 tokens 112 -> 174.
 int fa_bwd_parts(int B, int total_kv, int Hq, int Hkv) {
     const int64_t items = ((int64_t)total_kv / BT + B) * Hkv;   // at most

@@ -89,8 +89,9 @@ int varlen_make_plan(VarlenPlan& plan, int64_t most0, int64_t most1, int Hq, int
     plan.most[1] = (int)most1;
     // 32 sequences fit a warp.  Up to four items a CTA, dealing them out in turn loses less than
     // the counter's zeroing and its latency cost (forward of 8 prompts of 22 to 200 tokens:
-    // 22.5 -> 20.5 us; forward and backward of 17 sequences of up to 700: 84.0 -> 73.7 us);
-    // with more, lengths decide (25 sequences of up to 16384 tokens: 9.3 ms dealt, 8.5 counted).
+    // 16.4 -> 12.4 us; forward and backward of 17 sequences of up to 700: 65.4 -> 61.7 us); with
+    // more, lengths decide (25 sequences of up to 16384 tokens: 9.4 ms dealt, 8.8 counted; 20
+    // documents of up to 8192, forward and backward: 10.0 ms dealt, 8.7 counted).
     plan.lists = plan.B > 32;
     plan.counted = plan.lists || std::max(most0, most1) > 4 * sm_count();
     if (!plan.lists) {

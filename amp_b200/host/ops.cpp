@@ -4,8 +4,8 @@
 //
 // A decode step makes these calls on a few kilobytes, where the kernels take 2 to 10 us.
 // Checked and called through ctypes, a call cost 18 to 28 us of host time (20 to 25
-// converted arguments, four attribute reads a tensor); here it costs 4 to 8.  The rest of
-// the package calls the C ABI through ctypes (_lib.py); both use the same library: bind()
+// converted arguments, four attribute reads a tensor); here it costs 2.5 to 7, and 13 for the
+// backward's three results and four kernels.  The rest of the package calls the C ABI through ctypes (_lib.py); both use the same library: bind()
 // receives the addresses of its functions.
 //
 // Every entry takes its arguments by position -- the keywords, defaults and documentation
