@@ -4,6 +4,7 @@
 // the backward pass" (kernels/flash_attn.cuh:48).  Given Q, K, V, O, dO and the
 // forward's lse (natural log):
 //   Delta = rowsum(dO * O)                                   k_fa_bwd_delta
+//     (packed, rows of few keys: rowsum(P * dP)              k_fa_bwd_few)
 //   P = exp(scale Q K^T - lse),  dP = dO V^T,  dS = P * (dP - Delta)
 //   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K
 // in two passes shaped like the forward, so every product is one of its MMA
@@ -306,12 +307,154 @@ __global__ void __launch_bounds__(256) k_fa_bwd_delta(const __nv_bfloat16* __res
     }
 }
 
+// ------------------------------------------------------- Delta of rows of few keys
+// Queries of a sequence that see few keys (1 to kFewKeys): row0 .. row0 + n.  O is rounded to
+// bf16, and in a row of n keys that moves Delta by about 1 / sqrt(n) of what rounding dS does, all
+// entries of the row together; beyond 32 keys there is little left to gain.  Error
+// of dQ and dK against fp64, with Delta from O -> with these rows' Delta from the unrounded
+// P and dP (both passes' sum of P dP): sequences of 8 tokens 0.0034 -> 0.0023, of 20 0.0030 -> 0.0024,
+// of up to 700 0.0026 -> 0.0024; outputs and dS rounded alone: 0.0024.
+constexpr int kFewKeys = 32;
+struct FewRows {
+    int row0, n;
+};
+__device__ __forceinline__ FewRows few_rows(const VarlenSeq& s, int causal) {
+    if (!causal) return {0, s.k_len >= 1 && s.k_len <= kFewKeys ? s.q_len : 0};
+    // query i sees i + 1 + (k_len - q_len) keys
+    const int first = max(0, s.q_len - s.k_len);
+    const int64_t end = (int64_t)kFewKeys + s.q_len - s.k_len;
+    return {first, (int)max((int64_t)0, min((int64_t)s.q_len, end) - first)};
+}
+
+struct Frag4 { uint32_t x[4]; };
+struct Frag2 { uint32_t x[2]; };
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], const Frag4& a, const Frag2& b) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                 "{%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a.x[0]), "r"(a.x[1]), "r"(a.x[2]), "r"(a.x[3]), "r"(b.x[0]), "r"(b.x[1]));
+}
+
+struct FewParams {
+    const __nv_bfloat16 *q, *k, *v, *d_o;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, do_tok, do_head;
+    const float* lse;
+    float* delta;
+    int Hq, Hkv, causal, strips;   // strips: warps of a (sequence, head)
+    float scale_log2;
+    int* status;
+    VarlenPlan plan;
+};
+
+// Delta of 16 such rows (from row0 on, below row_end) of one head by one warp: the scores and dP
+// of up to 32 keys are 16 x 8 tiles of mma.sync, whose few products end before operands for tcgen05
+// would be staged.  A lane loads 16 bytes of a row, 8 neighbouring elements, and gives them to the
+// MMA as the columns that it has to bring in two steps: a dot product may be summed in any order,
+// as long as both operands keep one.
+// Measured, whole backward without -> with these rows: 17 sequences of up to 700 tokens (8 heads, D 64)
+// 46 -> 46 us, 20 documents of up to 8192 unchanged; 200 sequences of 30 tokens 80 -> 87; 1000 of 30
+// (32 / 8 heads, D 128) 1464 -> 1640, where nearly all rows see few keys and what it adds is
+// reading q, k, v and dO once more.  (4-byte loads in the MMA's own order: 2080; all 32 keys at once
+// in 160 registers: 1708; 80 registers: 1678; in the Delta kernel's own blocks, whose rows then have
+// to be looked up: 1686.)
+template <int D>
+__device__ __forceinline__ float2 few_tile(const FewParams& st, const VarlenSeq& s, int row0, int row_end, int h) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = (lane & 3) * 8;
+    // (a row or key past the end is read as the last one: MMA rows and columns do not mix)
+    const __nv_bfloat16 *qp[2], *op[2];
+    // as the passes take it; a row that sees no key, or is none, takes no part
+    int seen[2];
+    float nl2[2], acc[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = row0 + g + i * 8;
+        const int64_t tok = s.q_off + min(row, row_end - 1);
+        qp[i] = st.q + tok * st.q_tok + h * st.q_head + c;
+        op[i] = st.d_o + tok * st.do_tok + h * st.do_head + c;
+        seen[i] = row >= row_end ? 0 : st.causal ? row + 1 + s.k_len - s.q_len : s.k_len;
+        const float lse = seen[i] > 0 ? st.lse[(int64_t)h * st.plan.total_q + tok] : -INFINITY;
+        nl2[i] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+    }
+    const int keys = st.causal ? min(row0 + 16, row_end) + s.k_len - s.q_len : s.k_len;   // seen by the last row
+    const int hk = h / (st.Hq / st.Hkv);
+    auto eight = [](const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); };
+    constexpr int kTiles = 2;   // of 8 keys at a time
+#pragma unroll 1
+    for (int n0 = 0; n0 < keys; n0 += kTiles * 8) {
+        const __nv_bfloat16 *kp[kTiles], *vp[kTiles];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+            const int64_t tok = s.k_off + min(n0 + n * 8 + g, keys - 1);
+            kp[n] = st.k + tok * st.k_tok + hk * st.k_head + c;
+            vp[n] = st.v + tok * st.v_tok + hk * st.v_head + c;
+        }
+        float sc[kTiles][4] = {}, dp[kTiles][4] = {};
+#pragma unroll 1
+        for (int e = 0; e < D; e += 32) {
+            const uint4 q0 = eight(qp[0] + e), q1 = eight(qp[1] + e), o0 = eight(op[0] + e), o1 = eight(op[1] + e);
+            uint4 kv[kTiles], vv[kTiles];
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) kv[n] = eight(kp[n] + e), vv[n] = eight(vp[n] + e);
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+                mma_16x8x16(sc[n], {q0.x, q1.x, q0.y, q1.y}, {kv[n].x, kv[n].y});
+                mma_16x8x16(dp[n], {o0.x, o1.x, o0.y, o1.y}, {vv[n].x, vv[n].y});
+                mma_16x8x16(sc[n], {q0.z, q1.z, q0.w, q1.w}, {kv[n].z, kv[n].w});
+                mma_16x8x16(dp[n], {o0.z, o1.z, o0.w, o1.w}, {vv[n].z, vv[n].w});
+            }
+        }
+        const int col = n0 + (lane & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + n * 8 + (i & 1) < seen[i >> 1])
+                    acc[i >> 1] = fmaf(ex2_approx(fmaf(sc[n][i], st.scale_log2, nl2[i >> 1])), dp[n][i], acc[i >> 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);
+        acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 2);
+    }
+    return make_float2(acc[0], acc[1]);   // of rows g and g + 8, in every lane of four
+}
+
+// A warp takes a (sequence, head)'s tiles of 16 rows: one of at most two under a causal mask, every
+// strips-th of all rows of a sequence with few keys under a full one.  Runs beside k_fa_bwd_delta,
+// which forms Delta of every row: only the store has to wait for that kernel's end.  What this one
+// reads is there before: each of that kernel's blocks waited for it before it let this one launch.
+template <int D>
+__global__ void __launch_bounds__(256, 2) k_fa_bwd_few(const __grid_constant__ FewParams p) {
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    bool waited = false;
+    // (B * Hq is below 2^30: varlen_check)
+    const unsigned total = (unsigned)p.plan.B * p.Hq * p.strips;
+    for (unsigned w = blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += gridDim.x * 8) {
+        // heads first: the warps of a block share keys
+        const unsigned bs = w / (unsigned)p.Hq;
+        const int h = (int)(w - bs * p.Hq), strip = (int)(bs % (unsigned)p.strips);
+        const VarlenSeq s = p.plan.load((int)(bs / (unsigned)p.strips), p.status);
+        const FewRows rows = few_rows(s, p.causal);
+        for (int r = strip * 16; r < rows.n; r += p.strips * 16) {
+            const int row0 = rows.row0 + r, end = rows.row0 + rows.n;
+            const float2 d = few_tile<D>(p, s, row0, end, h);
+            if (!waited) pdl_wait();
+            waited = true;
+            float* at = p.delta + (int64_t)h * p.plan.total_q + s.q_off + row0 + g;
+            if ((lane & 3) == 0 && row0 + g < end) at[0] = d.x;
+            if ((lane & 3) == 0 && row0 + g + 8 < end) at[8] = d.y;
+        }
+    }
+    if (!waited) pdl_wait();
+}
+
 // The P that dS = P (dP - Delta) multiplies with.  Dense: as rounded to bf16 for P^T dO.
 // Packed: as computed, in fp32 (dQ and dK then carry two roundings to bf16, of dS and their
 // own, instead of three: an error of 0.0024 instead of 0.0030 relative to fp64; the outputs'
 // rounding alone is 0.0017).  dS is rounded because the tensor core multiplies 16-bit operands.
-// Delta is formed from O as the forward rounded it, the only O there is; in rows of few keys,
-// where one P is near 1, that rounding is felt most (0.0026).
+// Delta is formed from O as the forward rounded it, the only O there is, except in rows of few
+// keys, where that rounding is felt (few_rows).
 template <bool kExact>
 struct Probs {
     float v[kExact ? 64 : 1];
@@ -1405,6 +1548,19 @@ int launch_bwd_packed(const PackedBwdArgs& a, cudaStream_t st) {
                                                                     (int64_t)sm_count() * 8)),
                                    dim3(256), 0, st, static_cast<const __nv_bfloat16*>(a.O),
                                    static_cast<const __nv_bfloat16*>(a.dO), delta, rows, ds));
+    }
+    if (rows > 0 && a.total_kv > 0) {
+        FewParams f = {static_cast<const __nv_bfloat16*>(a.Q), static_cast<const __nv_bfloat16*>(a.K),
+                       static_cast<const __nv_bfloat16*>(a.V), static_cast<const __nv_bfloat16*>(a.dO),
+                       s[0], s[1], s[2], s[3], s[4], s[5], s[8], s[9], a.lse, delta, a.Hq, a.Hkv, a.causal,
+                       kFewKeys / 16, p.scale_log2, p.status, p.plan};
+        // full mask: as many warps a head as fill the GPU, if the rows are there
+        if (!a.causal)
+            f.strips = (int)std::max<int64_t>(1, std::min<int64_t>((a.total_q + 15) / 16,
+                                                                   sm_count() * 16ll / ((int64_t)a.B * a.Hq)));
+        const int64_t blocks = ((int64_t)a.B * a.Hq * f.strips + 7) / 8;
+        AMPB_CHECK_CUDA(launch_pdl(k_fa_bwd_few<D>, dim3((unsigned)std::min<int64_t>(blocks, sm_count() * 8ll)),
+                                   dim3(256), 0, st, f));
     }
     static std::atomic<uint64_t> allowed_kv{0}, allowed_q{0};
     AMPB_CHECK_CUDA(allow_smem_once(allowed_kv, k_fa_bwd_dkdv<D, true>, CF::SMEM_KV));

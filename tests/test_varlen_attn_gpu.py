@@ -567,3 +567,46 @@ def test_a_short_wait_limit_holds_for_steps_not_for_whole_items(cuda, amp_lib):
     finally:
         amp_lib.amp_set_wait_timeout_ns(0)
     assert all(map(torch.equal, want, got))
+
+
+def rounded(q, k, v, do, lens_q, lens_kv, causal):
+    """dQ and dK in fp64 and with dS and the results rounded to bf16: what rounding them costs."""
+    q, k, v, do = (x.double() for x in (q, k, v, do))
+    G, sc = q.shape[1] // k.shape[1], q.shape[2] ** -0.5
+    exact, near = [[torch.zeros_like(x) for x in (q, k)] for _ in range(2)]
+    a = b = 0
+    for lq, lk in zip(lens_q, lens_kv):
+        Q, K = slice(a, a + lq), slice(b, b + lk)
+        a, b = a + lq, b + lk
+        kk, vv = (x[K].repeat_interleave(G, 1) for x in (k, v))
+        s = sc * torch.einsum("ihd,jhd->hij", q[Q], kk)
+        if causal:
+            s = s.masked_fill(~torch.ones(lq, lk, dtype=torch.bool).tril(lk - lq), -torch.inf)
+        p = s.softmax(2).nan_to_num(0.0)
+        dp = torch.einsum("ihd,jhd->hij", do[Q], vv)
+        ds = p * (dp - (p * dp).sum(2, keepdim=True))
+        for out, x in ((exact, ds), (near, ds.bfloat16().double())):
+            out[0][Q] = sc * torch.einsum("hij,jhd->ihd", x, kk)
+            out[1][K] = sc * torch.einsum("hij,ihd->jhd", x, q[Q]).unflatten(1, (-1, G)).sum(2)
+    return exact, [x.bfloat16().double() for x in near]
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 8, 64), (8, 2, 128), (7, 1, 64)])
+@pytest.mark.parametrize("lens_q,lens_kv,causal", [
+    ([3] * 60, [3] * 60, True), ([8] * 50 + [20] * 20, [8] * 50 + [20] * 20, True), ([1, 33, 17, 90, 64, 700, 31], [1, 33, 17, 90, 64, 700, 31], True),
+    ([40, 9, 5, 16, 200], [20, 12, 32, 31, 3], True), ([40, 9, 5, 160, 3, 16], [20, 12, 32, 31, 0, 16], False), ([50] * 20, [33] * 20, False),
+], ids=["3", "8 and 20", "mixed", "other lengths", "full", "full, 33 keys"])
+def test_few_keys_cost_no_precision(lens_q, lens_kv, causal, Hq, Hkv, D, cuda, amp_lib):
+    """In a row of few keys Delta from the rounded O moved every dS by up to twice its own rounding.  What
+    is left is the rounding of dS and of the results; 10% are for rows of more than 32 keys, whose
+    Delta does come from O: there rounding O adds at most 1 / 33 of the variance for each of
+    O's and P's rounding, and the errors of dS in a row, which it shares, add up at most threefold."""
+    q, k, v, do, cu_q, cu_kv = make(lens_q, lens_kv, Hq, Hkv, D, seed=89)
+    got = run(q, k, v, do, cu_q, cu_kv, causal)
+    exact, near = rounded(q, k, v, do, lens_q, lens_kv, causal)
+    for name, e, n in zip(("dq", "dk"), exact, near):
+        mine = (got[name].double().cpu() - e).norm()
+        assert mine <= 1.1 * (n - e).norm(), (name, float(mine / (n - e).norm()))
+    check(got, reference(q, k, v, do, lens_q, lens_kv, causal), ALL)
+    again = run(q, k, v, do, cu_q, cu_kv, causal)
+    assert all(torch.equal(got[x], again[x]) for x in ALL)
