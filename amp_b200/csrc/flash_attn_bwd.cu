@@ -428,8 +428,10 @@ __global__ void __launch_bounds__(256, 2) k_fa_bwd_few(const __grid_constant__ F
     pdl_trigger();
     const int lane = threadIdx.x & 31, g = lane >> 2;
     bool waited = false;
-    // (B * Hq is below 2^30: varlen_check)
-    const unsigned total = (unsigned)p.plan.B * p.Hq * p.strips;
+    // (B * Hq is below 2^30: varlen_check.)  Sequences that the plan refused (varlen_make_plan) get no
+    // work here either.
+    const bool none = p.plan.lists && p.plan.first(0)[p.plan.B] == 0;
+    const unsigned total = none ? 0u : (unsigned)p.plan.B * p.Hq * p.strips;
     for (unsigned w = blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += gridDim.x * 8) {
         // heads first: the warps of a block share keys
         const unsigned bs = w / (unsigned)p.Hq;

@@ -610,3 +610,16 @@ def test_few_keys_cost_no_precision(lens_q, lens_kv, causal, Hq, Hkv, D, cuda, a
     check(got, reference(q, k, v, do, lens_q, lens_kv, causal), ALL)
     again = run(q, k, v, do, cu_q, cu_kv, causal)
     assert all(torch.equal(got[x], again[x]) for x in ALL)
+
+
+def test_overlapping_sequences_of_few_keys_get_no_work(cuda, amp_lib):
+    """All rows of a sequence of few keys have their Delta formed by themselves: 2^17 times a million
+    rows would be hours."""
+    T, B = 1 << 20, 1 << 18
+    q, k, v, do, _, _ = (x.cuda() for x in make([T], [16], 1, 1, 64, seed=97))
+    cu, cukv = (torch.tensor([0, n], dtype=torch.int32, device="cuda").repeat(B // 2) for n in (T, 16))
+    o, lse = torch.zeros_like(q), torch.zeros(1, T, device="cuda")
+    dq, dk, dv = (torch.full_like(x, 7.0) for x in (q, k, v))
+    attention.flash_attn_varlen_bwd(q, k, v, o, do, lse, cu, cukv, causal=False, dq=dq, dk=dk, dv=dv)
+    assert amp_lib.amp_device_status(1) == -1 and amp_lib.amp_device_status(1) == 0
+    assert all((x == 7.0).all() for x in (dq, dk, dv))
